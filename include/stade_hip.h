@@ -214,6 +214,67 @@ int32_t stade_hip_conv3x3_hv(float* loss, const float* lossb, const float* xp, f
                              float* lossd, const float* lossbd, const float* xpd, float* xpbd, const float* wd, float* wbd,
                              float* outd, float* outbd, hipStream_t stream);
 
+/* ---- operators of language models ---------------------------------------------------------
+ * No counterpart in the reference: what a model needs around the dense layers that the
+ * generated functions train.  They keep the conventions above (caller's device arrays, shadows
+ * accumulated, the stream, the errors, graph capture), with these differences:
+ *   - the primal function and the adjoint are two calls (`<k>` and `<k>_b`: a model's other layers
+ *     lie between them), and the adjoint reads its output's shadow and leaves it as it is;
+ *   - `add` != 0 accumulates into the shadows, as the generated code does; `add` = 0 sets them
+ *     (the first use after a reset: nothing is read, and no caller has to clear them);
+ *   - element types are arguments: STADE_HIP_F32, _BF16 or _F16.  Sums are formed in Float32 and
+ *     rounded once;
+ *   - a matrix (i_d, i_n) has a leading dimension (elements, at least i_d): columns may lie
+ *     apart.  In a row-major program it is an array of i_n rows of i_d values.
+ * Ids count from 1. */
+#define STADE_HIP_F32 0
+#define STADE_HIP_BF16 1
+#define STADE_HIP_F16 2
+
+/* y (i_d, i_t): y[:, t] = s * w[:, tok[t]], w (i_d, i_v).  Id 0 is "no token" (a zero column); any other
+ * id outside 1..i_v is taken as 0 and raises the device error flag. */
+int32_t stade_hip_embed(int64_t ty, int64_t tw, void* y, int64_t ldy, const void* w, int64_t ldw, const int64_t* tok, double s,
+                        int64_t i_d, int64_t i_v, int64_t i_t, hipStream_t stream);
+/* its adjoint: wb[:, v] (+)= s * sum of yb[:, t] over the t with tok[t] = v, by sorted tokens (no atomics: the same
+ * call gives the same bits).  s is a constant. */
+int32_t stade_hip_embed_b(int64_t ty, int64_t tw, const void* yb, int64_t ldyb, void* wb, int64_t ldwb, const int64_t* tok, double s,
+                          int64_t i_d, int64_t i_v, int64_t i_t, int64_t add, hipStream_t stream);
+/* order Int64[i_t]: the places 1..i_t in stable order of their ids (those of no id last); start Int64[i_v + 1]:
+ * start[v] (from 0) of the sorted places lie before id v + 1.  As `tok` of stade_hip_embed, `order` takes rows in
+ * that order; with ids that name experts, `start` is what stade_hip_expert_mul takes. */
+int32_t stade_hip_token_order(const int64_t* tok, int64_t* order, int64_t* start, int64_t i_v, int64_t i_t, hipStream_t stream);
+
+/* The 8-bit tape of a matrix (i_d, i_n): q Int8, a column's values at a stride of 32 * ceil(i_d / 32), and qs UInt8,
+ * one scale for each 32 of a column (a power of two: exponent + 127).  lengths: of q and of qs.  A value reads back as
+ * q * 2^(qs - 127), exactly; it is within max|x| / 127 of the 32 values' largest.  A group with a value that is not
+ * finite reads back as NaN.  q aligned to 8 bytes. */
+int32_t stade_hip_tape8_lengths(int64_t i_d, int64_t i_n, int64_t lengths[2]);
+int32_t stade_hip_tape8_store(int64_t type, const void* x, int64_t ldx, int8_t* q, uint8_t* qs, int64_t i_d, int64_t i_n,
+                              hipStream_t stream);
+int32_t stade_hip_tape8_load(int64_t type, const int8_t* q, const uint8_t* qs, void* x, int64_t ldx, int64_t i_d, int64_t i_n,
+                             hipStream_t stream);
+
+/* y = (x - mu) * rs * g + b for each column of x (i_d, i_n), mu its mean and rs = 1 / sqrt(variance + eps), Float32, kept
+ * for the adjoint (each may be null).  g, b (i_d) of type tg: Float32 or x's type; null: 1 and 0.  q, qs: if not null,
+ * the tape of x is written too. */
+int32_t stade_hip_layernorm(int64_t tx, int64_t tg, void* y, int64_t ldy, const void* x, int64_t ldx, const void* g, const void* b,
+                            float* mu, float* rs, int8_t* q, uint8_t* qs, int64_t i_d, int64_t i_n, double eps, hipStream_t stream);
+/* its adjoint: xb, gb, bb from yb and x, or x's tape (x null).  gb, bb Float32; xb, gb and bb may each be null. */
+int32_t stade_hip_layernorm_b(int64_t tx, int64_t tg, const void* yb, int64_t ldyb, const void* x, int64_t ldx, const int8_t* q,
+                              const uint8_t* qs, void* xb, int64_t ldxb, const void* g, float* gb, float* bb, const float* mu,
+                              const float* rs, int64_t i_d, int64_t i_n, int64_t add, hipStream_t stream);
+
+/* y[:, t] (+)= w[:, :, e] * x[:, t] for the columns t of expert e, start[e] <= t - 1 < start[e + 1] (Int64[i_e + 1], from 0,
+ * in increasing order, on the device; an expert may have none).  x (i_in, i_t), y (i_out, i_t), w (i_out, i_in, i_e).
+ * Columns of no expert become 0.  Offsets that decrease or lie outside 0..i_t raise the device error flag. */
+int32_t stade_hip_expert_mul(int64_t tx, void* y, int64_t ldy, const void* x, int64_t ldx, const void* w, const int64_t* start,
+                             int64_t i_in, int64_t i_out, int64_t i_t, int64_t i_e, int64_t add, hipStream_t stream);
+/* its adjoint: xb[:, t] (+)= w[:, :, e]' * yb[:, t] and wb[:, :, e] (+)= sum over e's columns of yb[:, t] * x[:, t]', from x
+ * or its tape (x null).  wb: Float32 or x's type; xb and wb may each be null. */
+int32_t stade_hip_expert_mul_b(int64_t tx, int64_t twb, const void* yb, int64_t ldyb, const void* x, int64_t ldx, const int8_t* q,
+                               const uint8_t* qs, void* xb, int64_t ldxb, const void* w, void* wb, const int64_t* start, int64_t i_in,
+                               int64_t i_out, int64_t i_t, int64_t i_e, int64_t add, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

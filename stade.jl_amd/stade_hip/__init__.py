@@ -30,6 +30,8 @@ from .api import (  # noqa: F401
     burgers1d_b_ckpt, burgers1d_hv_ckpt, burgers1d_ckpt_lengths,
     mlp2_ce_b, mlp2_ce_d, mlp2_ce_hv,
     conv3x3_b, conv3x3_d, conv3x3_hv,
+    embed, embed_b, token_order, tape8_lengths, tape8_store, tape8_load,
+    layernorm, layernorm_b, expert_mul, expert_mul_b,
     rng_normal, rng_uniform, rng_int_range, stable_seed,
 )
 from .emit import stade_hip_file  # noqa: F401

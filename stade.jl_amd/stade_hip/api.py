@@ -57,6 +57,15 @@ ENTRY_POINTS: dict[str, str] = {
     "stade_hip_conv3x3_b": "a" * 8 + "iiiii",
     "stade_hip_conv3x3_d": "a" * 8 + "iiiii",
     "stade_hip_conv3x3_hv": "a" * 8 + "iiiii" + "a" * 8,
+    "stade_hip_embed": "ii" + "aiaia" + "f" + "iii",
+    "stade_hip_embed_b": "ii" + "aiaia" + "f" + "iiii",
+    "stade_hip_token_order": "aaaii",
+    "stade_hip_tape8_store": "i" + "aiaa" + "ii",
+    "stade_hip_tape8_load": "i" + "aaai" + "ii",
+    "stade_hip_layernorm": "ii" + "aiai" + "aaaaaa" + "iif",
+    "stade_hip_layernorm_b": "ii" + "aiaiaaai" + "aaaaa" + "iii",
+    "stade_hip_expert_mul": "i" + "aiaiaa" + "iiiii",
+    "stade_hip_expert_mul_b": "ii" + "aiaiaaaiaaa" + "iiiii",
 }
 
 _CT = {"a": P, "i": I64, "f": F64, "r": F64P}
@@ -535,3 +544,221 @@ def conv3x3_hv(loss, lossb, xp, xpb, w, wb, out, outb, i_nb, i_c, i_k, i_h, i_w,
     t = _conv_args(("lossd", "lossbd", "xpd", "xpbd", "wd", "wbd", "outd", "outbd"),
                    (lossd, lossbd, xpd, xpbd, wd, wbd, outd, outbd), s)
     _call("stade_hip_conv3x3_hv", a + [N, C, K, H, W] + t, _stream_of(xp))
+
+
+# ------------------------------------------------------------------------------------------
+# operators of language models: token rows, the 8-bit tape, layer norm, products by expert
+# ------------------------------------------------------------------------------------------
+# A matrix (i_d, i_n) is a flat contiguous tensor, or an (i_n, i_d) tensor whose rows may lie
+# apart (stride(1) == 1, stride(0) >= i_d).  Element types are the tensors' own.
+
+_CODES: dict = {}
+
+
+def _code(name: str, t) -> int:
+    import torch
+    if not _CODES:
+        _CODES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
+    try:
+        return _CODES[t.dtype]
+    except (AttributeError, KeyError):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name}: expected a torch tensor on a GPU, got {type(t).__name__}") from None
+        raise TypeError(f"{name}: dtype {t.dtype}, expected float32, bfloat16 or float16") from None
+
+
+def _mat(name: str, t, d: int, n: int, dtype=None):
+    """(device pointer, leading dimension) of a matrix (d, n)."""
+    import torch
+    if isinstance(t, torch.Tensor) and t.is_cuda and (dtype is None or t.dtype is dtype):
+        if t.is_contiguous() and t.numel() == d * n:
+            return t.data_ptr(), d
+        if t.dim() == 2 and t.shape[0] == n and t.shape[1] == d and (d <= 1 or t.stride(1) == 1) and (n <= 1 or t.stride(0) >= d):
+            return t.data_ptr(), t.stride(0) if n > 1 else d
+        if t.dim() == 2 and t.numel() == d * n:
+            raise ValueError(f"{name}: strides {tuple(t.stride())}; rows of {d} must be contiguous and must not overlap")
+    return _arr(name, t, dtype or t.dtype if isinstance(t, torch.Tensor) else None, d * n), d
+
+
+def _opt(name: str, t, dtype, numel: int):
+    return None if t is None else _arr(name, t, dtype, numel)
+
+
+def _sizes(**kw) -> list:
+    out = []
+    for k, v in kw.items():
+        v = _int(k, v)
+        if v < 0:
+            raise ValueError(f"{k} is negative")
+        out.append(v)
+    return out
+
+
+def _one_device(*ts):
+    """The tensors' device must be one, and the current one (the library works on the current
+    device, as the other functions do)."""
+    import torch
+    devs = {t.get_device() for t in ts if t is not None}
+    if len(devs) != 1 or devs != {torch.cuda.current_device()}:
+        raise ValueError(f"tensors on GPUs {sorted(devs)}: all must be on the current one ({torch.cuda.current_device()})")
+
+
+def _flag(fn: str, check: bool, what: str):
+    if check and device_error():
+        raise StadeHipBoundsError(f"{fn}: {what}")
+
+
+def embed(y, w, tok, s, i_d, i_v, i_t, check=False):
+    """y[:, t] = s * w[:, tok[t]] for ids tok (Int64, 1..i_v; 0 is "no token": a zero column).
+    y (i_d, i_t), w (i_d, i_v).  Any other id is taken as 0; check=True raises StadeHipBoundsError
+    for one (one synchronisation)."""
+    import torch
+    d, v, t = _sizes(i_d=i_d, i_v=i_v, i_t=i_t)
+    ty, tw = _code("y", y), _code("w", w)
+    (yp, ldy), (wp, ldw) = _mat("y", y, d, t), _mat("w", w, d, v)
+    a = [ty, tw, yp, ldy, wp, ldw, _arr("tok", tok, torch.int64, t), float(s), d, v, t]
+    _one_device(y, w, tok)
+    _call("stade_hip_embed", a, _stream_of(y))
+    _flag("embed", check, "an id is outside 0..i_v")
+
+
+def embed_b(yb, wb, tok, s, i_d, i_v, i_t, add=True, check=False):
+    """Adjoint of embed: wb[:, v] += s * the sum of yb[:, t] over the t with tok[t] = v (add=False:
+    wb is set).  By sorted tokens, in fixed order: the same call gives the same bits."""
+    import torch
+    d, v, t = _sizes(i_d=i_d, i_v=i_v, i_t=i_t)
+    ty, tw = _code("yb", yb), _code("wb", wb)
+    (yp, ldy), (wp, ldw) = _mat("yb", yb, d, t), _mat("wb", wb, d, v)
+    a = [ty, tw, yp, ldy, wp, ldw, _arr("tok", tok, torch.int64, t), float(s), d, v, t, int(bool(add))]
+    _one_device(yb, wb, tok)
+    _call("stade_hip_embed_b", a, _stream_of(yb))
+    _flag("embed_b", check, "an id is outside 0..i_v")
+
+
+def token_order(tok, order, start, i_v, i_t, check=False):
+    """order (Int64[i_t]): the places 1..i_t in stable order of their ids, those without an id
+    last; start (Int64[i_v + 1]): how many of the sorted places lie before each id, and before the
+    end of the last.  `order` as the ids of `embed` takes rows in that order; for ids that name
+    experts, `start` is the `start` of expert_mul."""
+    import torch
+    v, t = _sizes(i_v=i_v, i_t=i_t)
+    a = [_arr("tok", tok, torch.int64, t), _arr("order", order, torch.int64, t), _arr("start", start, torch.int64, v + 1), v, t]
+    _one_device(tok, order, start)
+    _call("stade_hip_token_order", a, _stream_of(tok))
+    _flag("token_order", check, "an id is outside 0..i_v")
+
+
+def tape8_lengths(i_d, i_n) -> tuple[int, int]:
+    """Lengths of the 8-bit tape (q Int8, qs UInt8) of a matrix (i_d, i_n)."""
+    out = (ctypes.c_int64 * 2)()
+    L = lib()
+    L.stade_hip_tape8_lengths.argtypes = [I64, I64, ctypes.POINTER(ctypes.c_int64)]
+    L.stade_hip_tape8_lengths.restype = ctypes.c_int32
+    _check("stade_hip_tape8_lengths", L.stade_hip_tape8_lengths(_int("i_d", i_d), _int("i_n", i_n), out))
+    return int(out[0]), int(out[1])
+
+
+def _tape(q, qs, d: int, n: int):
+    import torch
+    g = -(-d // 32)
+    return _arr("q", q, torch.int8, 32 * g * n), _arr("qs", qs, torch.uint8, g * n)
+
+
+def tape8_store(x, q, qs, i_d, i_n):
+    """The 8-bit tape of x (i_d, i_n): groups of 32 of a column share a power-of-two scale."""
+    d, n = _sizes(i_d=i_d, i_n=i_n)
+    c = _code("x", x)
+    xp, ldx = _mat("x", x, d, n)
+    a = [c, xp, ldx, *_tape(q, qs, d, n), d, n]
+    _one_device(x, q, qs)
+    _call("stade_hip_tape8_store", a, _stream_of(x))
+
+
+def tape8_load(q, qs, x, i_d, i_n):
+    """The values that an 8-bit tape holds, into x (i_d, i_n)."""
+    d, n = _sizes(i_d=i_d, i_n=i_n)
+    c = _code("x", x)
+    xp, ldx = _mat("x", x, d, n)
+    a = [c, *_tape(q, qs, d, n), xp, ldx, d, n]
+    _one_device(x, q, qs)
+    _call("stade_hip_tape8_load", a, _stream_of(x))
+
+
+def _weights(g, b, x, d: int):
+    """(type code, g pointer, b pointer): both Float32, or both of x's type."""
+    some = g if g is not None else b
+    code = 0 if some is None else _code("g", some)
+    dtype = None if some is None else some.dtype
+    return code, _opt("g", g, dtype, d), _opt("b", b, dtype, d)
+
+
+def layernorm(y, x, g, b, mu, rs, i_d, i_n, eps=1e-5, tape=None):
+    """y = (x - mu) * rs * g + b by columns of x (i_d, i_n), with the column's mean mu and
+    rs = 1 / sqrt(variance + eps) (Float32[i_n], kept for the adjoint; None: not kept).  g, b of x's
+    type or Float32; None: 1 and 0.  tape = (q, qs): the 8-bit tape of x is written in the same pass."""
+    import torch
+    d, n = _sizes(i_d=i_d, i_n=i_n)
+    tx = _code("x", x)
+    (yp, ldy), (xp, ldx) = _mat("y", y, d, n, x.dtype), _mat("x", x, d, n)
+    tg, gp, bp = _weights(g, b, x, d)
+    qp, sp = _tape(*tape, d, n) if tape is not None else (None, None)
+    a = [tx, tg, yp, ldy, xp, ldx, gp, bp, _opt("mu", mu, torch.float32, n), _opt("rs", rs, torch.float32, n), qp, sp, d, n, float(eps)]
+    _one_device(y, x, g, b, mu, rs, *(tape or ()))
+    _call("stade_hip_layernorm", a, _stream_of(x))
+
+
+def layernorm_b(yb, x, xb, g, gb, bb, mu, rs, i_d, i_n, add=True, tape=None):
+    """Adjoint of layernorm from its output's shadow yb and its input x, or with x = None the tape
+    of x: xb, gb and bb are accumulated (add=False: set).  gb, bb Float32; xb, gb, bb may be None."""
+    import torch
+    d, n = _sizes(i_d=i_d, i_n=i_n)
+    if (x is None) == (tape is None):
+        raise ValueError("one of x and tape is needed, and not both")
+    tx = _code("yb", yb)
+    yp, ldy = _mat("yb", yb, d, n)
+    xp, ldx = _mat("x", x, d, n, yb.dtype) if x is not None else (None, d)
+    xbp, ldxb = _mat("xb", xb, d, n, yb.dtype) if xb is not None else (None, d)
+    tg, gp, _ = _weights(g, None, yb, d)
+    qp, sp = _tape(*tape, d, n) if tape is not None else (None, None)
+    a = [tx, tg, yp, ldy, xp, ldx, qp, sp, xbp, ldxb, gp, _opt("gb", gb, torch.float32, d), _opt("bb", bb, torch.float32, d),
+         _arr("mu", mu, torch.float32, n), _arr("rs", rs, torch.float32, n), d, n, int(bool(add))]
+    _one_device(yb, x, xb, g, gb, bb, mu, rs, *(tape or ()))
+    _call("stade_hip_layernorm_b", a, _stream_of(yb))
+
+
+def expert_mul(y, x, w, start, i_in, i_out, i_t, i_e, add=False, check=False):
+    """y[:, t] = w[:, :, e] * x[:, t] for the columns t of expert e, those that start[e] <= t - 1 < start[e + 1]
+    (Int64[i_e + 1], increasing from 0).  x (i_in, i_t), y (i_out, i_t), w (i_out, i_in, i_e); columns of no expert
+    become 0.  add=True: y is accumulated.  check=True raises StadeHipBoundsError for offsets that decrease
+    or lie outside 0..i_t (one synchronisation)."""
+    import torch
+    i, o, t, e = _sizes(i_in=i_in, i_out=i_out, i_t=i_t, i_e=i_e)
+    tx = _code("x", x)
+    (yp, ldy), (xp, ldx) = _mat("y", y, o, t, x.dtype), _mat("x", x, i, t)
+    a = [tx, yp, ldy, xp, ldx, _arr("w", w, x.dtype, i * o * e), _arr("start", start, torch.int64, e + 1), i, o, t, e, int(bool(add))]
+    _one_device(y, x, w, start)
+    _call("stade_hip_expert_mul", a, _stream_of(x))
+    _flag("expert_mul", check, "start decreases or lies outside 0..i_t")
+
+
+def expert_mul_b(yb, x, xb, w, wb, start, i_in, i_out, i_t, i_e, add=True, tape=None, check=False):
+    """Adjoint of expert_mul: xb[:, t] += w[:, :, e]' * yb[:, t] and wb[:, :, e] += the sum over e's columns of
+    yb[:, t] * x[:, t]' (add=False: set), x as itself or, with x = None, as its tape.  wb Float32 or of yb's
+    type; xb and wb may be None (w is needed for xb only, x or its tape for wb only)."""
+    import torch
+    i, o, t, e = _sizes(i_in=i_in, i_out=i_out, i_t=i_t, i_e=i_e)
+    if wb is not None and (x is None) == (tape is None):
+        raise ValueError("one of x and tape is needed, and not both")
+    ty = _code("yb", yb)
+    yp, ldy = _mat("yb", yb, o, t)
+    xp, ldx = _mat("x", x, i, t, yb.dtype) if x is not None else (None, i)
+    xbp, ldxb = _mat("xb", xb, i, t, yb.dtype) if xb is not None else (None, i)
+    qp, sp = _tape(*tape, i, t) if tape is not None else (None, None)
+    twb = _code("wb", wb) if wb is not None else 0
+    if wb is not None and wb.dtype not in (torch.float32, yb.dtype):
+        raise TypeError(f"wb: dtype {wb.dtype}, expected float32 or {yb.dtype}")
+    a = [ty, twb, yp, ldy, xp, ldx, qp, sp, xbp, ldxb, _opt("w", w, yb.dtype, i * o * e),
+         None if wb is None else _arr("wb", wb, wb.dtype, i * o * e), _arr("start", start, torch.int64, e + 1), i, o, t, e, int(bool(add))]
+    _one_device(yb, x, xb, w, wb, start, *(tape or ()))
+    _call("stade_hip_expert_mul_b", a, _stream_of(yb))
+    _flag("expert_mul_b", check, "start decreases or lies outside 0..i_t")
