@@ -24,6 +24,13 @@ struct Rows {
     int rows;
 };
 
+// the same value in every lane, in scalar registers
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    return (int64_t)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
+}
+__device__ __forceinline__ Rows uniform(const Rows& r) { return Rows{uniform(r.e), uniform(r.row), uniform(r.rows)}; }
+
 // start[i] in order and in range: the largest of the offsets up to i, each between 0 and t.  (Offsets
 // that are neither raise the device error flag; no row then has two experts.)
 //
@@ -104,103 +111,354 @@ __device__ __forceinline__ Rows expert_rows(const int64_t* start, int ne, int64_
 }
 
 // ------------------------------------------------------------------------------------------
-// the simple form: 64 x 64 of the result a block, 4 x 4 a thread, fp32 FMAs, any type and size
+// One product: tiles of BM x BN of the result on the matrix cores
 // ------------------------------------------------------------------------------------------
 struct Mul {
-    const void* a; int64_t lda;    // rows
-    const void* b; int64_t ldb;    // w, or yb for wb
+    const void* a; int64_t lda;            // rows (x, or yb for xb)
+    const void* b; int64_t ldb;            // w, or yb for wb
     void* c; int64_t ldc;
     const uint8_t* q; const uint8_t* qs;   // the rows' tape in place of a (wb)
     const int64_t* start;
     int ne;
     int64_t t;
-    int m, n, k;     // of one expert's product (m or k: its rows)
+    int m, n, k;       // of one expert's product (m of xb and y, k of wb: its rows)
+    int tiles_n;       // column tiles
+    int64_t pieces;    // row pieces (y, xb), or experts times row tiles (wb)
     int add;
     int32_t* flag;
 };
 
-constexpr int NT = 256, TM = 64, TN = 64, TK = 16;
 enum Form { Y = 0, XB = 1, WB = 2 };
 
-template <class T, class TC, int FORM, bool TAPE>
-__global__ __launch_bounds__(NT) void simple_kernel(Mul p) {
-    __shared__ float as[TK][TM + 4], bs[TK][TN + 4];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    Rows r;
-    int64_t m0;
-    if constexpr (FORM == WB) {
-        const int mt = (p.m + TM - 1) / TM;
-        r = expert_rows(p.start, p.ne, p.t, blockIdx.y / mt, p.flag);
-        m0 = (int64_t)(blockIdx.y % mt) * TM;
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+
+// Operand tiles in LDS, in 16-byte chunks of CE values.  A step takes BK values of k.
+//   k-contiguous operand (x and yb rows; w for xb): ROWS rows of 128 bytes; row r holds its chunk c at
+//     place c ^ (r & 7), so that eight lanes that read one chunk of eight rows meet all the banks.
+//   row-contiguous operand (w for y; x and yb for wb): BK rows of ROWS values.  The 16-bit types are
+//     read through the transposing LDS read (16 lanes: four k of 16 rows); the 64-byte pieces of
+//     row k lie at place p ^ (k & 3), so that the four rows it reads lie on different banks.
+template <class T> constexpr int kBK = 128 / (int)sizeof(T);
+template <class T> constexpr int kCE = 16 / (int)sizeof(T);
+
+// byte offset of chunk `c` of row `r` (KC), or of row k (not KC), in its tile
+template <class T, bool KC, int ROWS>
+__device__ __forceinline__ int chunk_at(int r, int c) {
+    if constexpr (KC) return r * 128 + ((c ^ (r & 7)) << 4);
+    else if constexpr (sizeof(T) == 2) return r * ROWS * 2 + ((((c >> 2) ^ (r & 3)) << 6) | ((c & 3) << 4));
+    else return r * ROWS * 4 + (c << 4);
+}
+
+// A thread's chunks of a tile: chunk number NT i + tid, in the order of the places, so that a wave's
+// lanes fill consecutive places.  (row, first value) of the operand's own indexes: KC: row of ROWS and
+// k; else k and row.
+template <class T, bool KC, int ROWS, int NT>
+__device__ __forceinline__ void my_chunk(int i, int& outer, int& inner) {
+    const int at = i * NT + threadIdx.x;
+    if constexpr (KC) {
+        outer = at >> 3;
+        inner = ((at & 7) ^ (outer & 7)) * kCE<T>;
     } else {
-        r = find_rows<TM>(p.start, p.ne, p.t, blockIdx.y, p.flag);
-        m0 = 0;
+        constexpr int PER = ROWS / kCE<T>;
+        outer = at / PER;
+        int c = at % PER;
+        if constexpr (sizeof(T) == 2) c = ((c >> 2) ^ (outer & 3)) << 2 | (c & 3);
+        inner = c * kCE<T>;
     }
-    if (r.e == -2) return;
-    const int n0 = blockIdx.x * TN, m = FORM == WB ? p.m : r.rows, k = FORM == WB ? r.rows : r.e < 0 ? 0 : p.k;
-    if (r.e < 0 && p.add) return;
-    const T* a = (const T*)p.a + (FORM == WB ? r.row * p.lda : r.row * p.lda);
-    const T* b = (const T*)p.b + (FORM == WB ? r.row * p.ldb : (int64_t)max(r.e, 0) * (FORM == Y ? (int64_t)p.k * p.n : (int64_t)p.k * p.n));
-    TC* c = (TC*)p.c + (FORM == WB ? (int64_t)r.e * p.m * p.n : r.row * p.ldc);
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < k; k0 += TK) {
-        for (int i = threadIdx.x; i < TK * TM; i += NT) {
-            const int kk = FORM == WB ? i / TM : i % TK, mm = FORM == WB ? i % TM : i / TK;
-            float v = 0.f;
-            if (k0 + kk < k && m0 + mm < m) {
-                if constexpr (FORM == WB) {
-                    if constexpr (TAPE) {
-                        const int64_t ng = tape8::groups(p.m), row = r.row + k0 + kk;
-                        const int64_t col = m0 + mm;
-                        v = (float)(int)(int8_t)p.q[row * ng * 32 + col] * tape8::unit(p.qs[row * ng + col / 32]);
-                    } else {
-                        v = (float)a[(int64_t)(k0 + kk) * p.lda + m0 + mm];
-                    }
+}
+
+// 16 bytes of the operand through registers: any alignment, zeros past `left` values
+template <class T>
+__device__ __forceinline__ v4u load_chunk(const T* p, int left) {
+    typedef T vec __attribute__((ext_vector_type(kCE<T>)));
+    typedef vec loose __attribute__((aligned(sizeof(T))));
+    vec v;
+    if (left >= kCE<T>) {
+        v = *reinterpret_cast<const loose*>(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kCE<T>; ++i) v[i] = i < left ? p[i] : (T)0.f;
+    }
+    return __builtin_bit_cast(v4u, v);
+}
+
+// An operand's staging.  The chunks of the step at k0 go from memory to registers (load), and
+// later to LDS (store); or straight to LDS (DIRECT: 16-byte aligned rows, whole chunks).
+// `rows`: of this tile; `kmax`: the product's k.
+template <class T, bool KC, int ROWS, int NT>
+struct Stage {
+    static constexpr int PER = ROWS * 128 / 16 / NT;
+    static_assert(ROWS * 8 % NT == 0, "whole chunks a thread");
+    const T* p;
+    int64_t ld;
+    int rows, kmax;
+
+    __device__ __forceinline__ void load(v4u (&v)[PER], int k0) const {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            int o, n;
+            my_chunk<T, KC, ROWS, NT>(i, o, n);
+            const int left = KC ? (o < rows ? kmax - k0 - n : 0) : (k0 + o < kmax ? rows - n : 0);
+            v[i] = load_chunk(KC ? p + (int64_t)o * ld + k0 + n : p + (int64_t)(k0 + o) * ld + n, left);
+        }
+    }
+    __device__ __forceinline__ static void store(const v4u (&v)[PER], char* lds) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) *reinterpret_cast<v4u*>(lds + (i * NT + threadIdx.x) * 16) = v[i];
+    }
+    // straight to LDS by buffer loads: lanes past the rows or past k get an offset past the buffer,
+    // and zeros
+    __device__ __forceinline__ void direct(char* lds, int k0) const {
+        const T* base = KC ? p + k0 : p + (int64_t)k0 * ld;
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), (short)0, 0x7fffffff, 0x00020000);
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            int o, n;
+            my_chunk<T, KC, ROWS, NT>(i, o, n);
+            const bool here = KC ? o < rows && k0 + n < kmax : k0 + o < kmax && n < rows;
+            const uint32_t off = here ? (uint32_t)o * (uint32_t)ld * sizeof(T) + n * sizeof(T) : 0x80000000u;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(lds + (i * NT + wave * 64) * 16), 16, off, 0,
+                                                     0, 0);
+        }
+    }
+};
+
+// the tape's staging (a row-contiguous operand): 8 bytes and a scale become 8 values, exactly
+template <class T, int ROWS, int NT>
+struct TapeStage {
+    static constexpr int CE = kCE<T>, PER = ROWS * 128 / 16 / NT;
+    const uint8_t* q; const uint8_t* qs;   // at the expert's first row
+    int64_t ng;
+    int col, rows, kmax;                   // the tile's first column of the tape's rows
+
+    struct Held { uint2 q[PER]; uint32_t s[PER]; };
+    __device__ __forceinline__ void load(Held& v, int k0) const {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            int o, n;
+            my_chunk<T, false, ROWS, NT>(i, o, n);
+            v.q[i] = make_uint2(0, 0);
+            v.s[i] = 0;
+            if (k0 + o < kmax && n < rows) {   // (a chunk past the last value is zeros in the tape)
+                const int64_t row = k0 + o;
+                const uint8_t* at = q + row * ng * tape8::kGroup + col + n;
+                if constexpr (CE == 8) v.q[i] = *reinterpret_cast<const uint2*>(at);
+                else v.q[i].x = *reinterpret_cast<const uint32_t*>(at);
+                v.s[i] = qs[row * ng + (col + n) / tape8::kGroup];
+            }
+        }
+    }
+    __device__ __forceinline__ static void store(const Held& v, char* lds) {
+        typedef T vec __attribute__((ext_vector_type(CE)));
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            // q + 128 as an unsigned byte, times the unit, less 128 units: exact
+            const float u = tape8::unit(v.s[i]), low = -128.f * u;
+            const uint32_t w[2] = {v.q[i].x ^ 0x80808080u, v.q[i].y ^ 0x80808080u};
+            vec x;
+#pragma unroll
+            for (int j = 0; j < CE; ++j) x[j] = (T)fmaf((float)((w[j >> 2] >> (8 * (j & 3))) & 0xffu), u, low);
+            *reinterpret_cast<v4u*>(lds + (i * NT + threadIdx.x) * 16) = __builtin_bit_cast(v4u, x);
+        }
+    }
+};
+
+// A lane's values of 32 rows from `row0` and the s-th quarter of a step: 16-bit types k = 16 s + 8 h + 0..7
+// of row lane % 32, h = lane / 32; fp32 k = 8 s + 4 h + 0..3.
+template <class T, bool KC, int ROWS>
+__device__ __forceinline__ v4u fragment(const char* lds, int row0, int s) {
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    if constexpr (KC) {
+        return *reinterpret_cast<const v4u*>(lds + chunk_at<T, true, ROWS>(row0 + (lane & 31), 2 * s + h));
+    } else if constexpr (sizeof(T) == 2) {
+        const int k = 16 * s + 8 * h + ((lane & 15) >> 2), seg = (row0 >> 5) ^ (k & 3);
+        const char* at = lds + k * ROWS * 2 + seg * 64 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+        typedef __attribute__((address_space(3))) v4s* lp;
+        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(at)), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(at + 4 * ROWS * 2));
+        typedef short v8s __attribute__((ext_vector_type(8)));
+        return __builtin_bit_cast(v4u, (v8s){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+    } else {
+        v4f v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const float*>(lds + (8 * s + 4 * h + j) * ROWS * 4 + (row0 + (lane & 31)) * 4);
+        return __builtin_bit_cast(v4u, v);
+    }
+}
+
+template <class T>
+__device__ __forceinline__ floatx16 multiply(v4u a, v4u b, floatx16 c) {
+    if constexpr (sizeof(T) == 4) {
+        const v4f x = __builtin_bit_cast(v4f, a), y = __builtin_bit_cast(v4f, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
+        return c;
+    } else if constexpr (Code<T>::value == STADE_HIP_BF16) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+}
+
+// The tile's place.  Blocks go round the 8 XCDs, each with an L2 of its own: an XCD gets a range of
+// tiles that lie together (kBand row pieces by all the columns), so that those which run at one
+// time share rows and columns in its L2.
+constexpr int kBand = 4;
+__device__ __forceinline__ bool my_tile(const Mul& p, int64_t& piece, int& tn) {
+    const int64_t total = p.pieces * p.tiles_n, per = (total + 7) / 8, id = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((blockIdx.x >> 3) >= per || id >= total) return false;
+    const int64_t band = id / (kBand * p.tiles_n), in = id - band * kBand * p.tiles_n, rows = min((int64_t)kBand, p.pieces - band * kBand);
+    tn = (int)(in / rows);
+    piece = band * kBand + in % rows;
+    return true;
+}
+
+template <class T, class TC, int FORM, bool TAPE, bool DIRECT, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void product_kernel(Mul p) {
+    constexpr int NT = 64 * WM * WN, MT = BM / WM / 32, NTL = BN / WN / 32, BK = kBK<T>;
+    constexpr bool AKC = FORM != WB, BKC = FORM == XB;
+    __shared__ char lds[2][(BM + BN) * 128];
+    int64_t piece;
+    int tn;
+    if (!my_tile(p, piece, tn)) return;
+    Rows r;
+    int m0 = 0;
+    if constexpr (FORM == WB) {
+        const int tiles_m = (p.m + BM - 1) / BM;
+        r = uniform(expert_rows(p.start, p.ne, p.t, (int)(piece / tiles_m), p.flag));
+        m0 = (int)(piece % tiles_m) * BM;
+    } else {
+        r = uniform(find_rows<BM>(p.start, p.ne, p.t, piece, p.flag));
+    }
+    if (r.e == -2 || (r.e < 0 && p.add)) return;
+    const int n0 = tn * BN, rows = FORM == WB ? min(BM, p.m - m0) : r.rows, cols = min(BN, p.n - n0);
+    const int k = FORM == WB ? r.rows : r.e < 0 ? 0 : p.k;
+    const int64_t e = r.e < 0 ? 0 : r.e;
+    const T* b = (const T*)p.b + (FORM == WB ? r.row * p.ldb + n0 : FORM == Y ? e * p.k * p.n + n0 : (e * p.n + n0) * p.k);
+    const Stage<T, BKC, BN, NT> sb{b, p.ldb, cols, k};
+    const Stage<T, AKC, BM, NT> sa{(const T*)p.a + r.row * p.lda + m0, p.lda, rows, k};
+    const int64_t ng = tape8::groups(p.m);
+    const TapeStage<T, BM, NT> st{p.q + r.row * ng * tape8::kGroup, p.qs + r.row * ng, ng, m0, rows, k};
+
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave / WN * MT * 32, wn = wave % WN * NTL * 32;
+    floatx16 acc[MT][NTL];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NTL; ++j)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) acc[i][j][x] = 0.f;
+
+    // (the weights come second: the operand order of the instruction gives each lane four
+    // consecutive columns of one row)
+    const auto compute = [&](const char* A, const char* B) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            v4u fa[MT], fb[NTL];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) fa[i] = fragment<T, AKC, BM>(A, wm + 32 * i, s);
+#pragma unroll
+            for (int j = 0; j < NTL; ++j) fb[j] = fragment<T, BKC, BN>(B, wn + 32 * j, s);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NTL; ++j) acc[i][j] = multiply<T>(fb[j], fa[i], acc[i][j]);
+        }
+    };
+    // While a step is multiplied from one pair of buffers, the next one comes into the other.
+    v4u ra[Stage<T, AKC, BM, NT>::PER], rb[Stage<T, BKC, BN, NT>::PER];
+    typename TapeStage<T, BM, NT>::Held rt;
+    const auto fetch = [&](char* A, char* B, int k0) {
+        if constexpr (TAPE) st.load(rt, k0);
+        else if constexpr (DIRECT) sa.direct(A, k0);
+        else sa.load(ra, k0);
+        if constexpr (DIRECT) sb.direct(B, k0);
+        else sb.load(rb, k0);
+    };
+    const auto settle = [&](char* A, char* B) {
+        if constexpr (TAPE) st.store(rt, A);
+        else if constexpr (!DIRECT) sa.store(ra, A);
+        if constexpr (!DIRECT) sb.store(rb, B);
+        if constexpr (DIRECT) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
+    if (k > 0) {
+        fetch(lds[0], lds[0] + BM * 128, 0);
+        settle(lds[0], lds[0] + BM * 128);
+        int turn = 0;
+        for (int k0 = BK; k0 < k; k0 += BK) {
+            char* next = lds[turn ^ 1];
+            fetch(next, next + BM * 128, k0);
+            compute(lds[turn], lds[turn] + BM * 128);
+            settle(next, next + BM * 128);
+            turn ^= 1;
+        }
+        compute(lds[turn], lds[turn] + BM * 128);
+    }
+    // lane: row lane % 32 of each 32, columns 8 g + 4 (lane / 32) + 0..3
+    TC* c = (TC*)p.c + (FORM == WB ? ((int64_t)r.e * p.m + m0) * p.n : r.row * p.ldc) + n0;
+    const int64_t ldc = FORM == WB ? p.n : p.ldc;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int row = wm + 32 * i + (lane & 31);
+        if (row >= rows) continue;
+#pragma unroll
+        for (int j = 0; j < NTL; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int col = wn + 32 * j + 8 * g + 4 * (lane >> 5);
+                if (col >= cols) continue;
+                float v[4];
+                TC* at = c + row * ldc + col;
+                if (p.add) {
+                    load_row(v, at, cols - col);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) v[x] += acc[i][j][4 * g + x];
                 } else {
-                    v = (float)a[(int64_t)mm * p.lda + k0 + kk];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) v[x] = acc[i][j][4 * g + x];
                 }
+                store_row(at, v, cols - col);
             }
-            as[kk][mm] = v;
-        }
-        for (int i = threadIdx.x; i < TK * TN; i += NT) {
-            const int kk = FORM == XB ? i % TK : i / TN, nn = FORM == XB ? i / TK : i % TN;
-            float v = 0.f;
-            if (k0 + kk < k && n0 + nn < p.n)
-                v = (float)(FORM == XB ? b[(int64_t)(n0 + nn) * p.ldb + k0 + kk] : b[(int64_t)(k0 + kk) * p.ldb + n0 + nn]);
-            bs[kk][nn] = v;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int kk = 0; kk < TK; ++kk) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(as[kk][ty * 4 + i], bs[kk][tx * 4 + j], acc[i][j]);
-        }
-        __syncthreads();
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t mm = m0 + ty * 4 + i;
-            const int nn = n0 + tx * 4 + j;
-            if (mm < m && nn < p.n) {
-                TC* at = c + mm * (FORM == WB ? (int64_t)p.n : p.ldc) + nn;
-                *at = (TC)(p.add ? (float)*at + acc[i][j] : acc[i][j]);
-            }
-        }
+}
+
+template <class T, class TC, int FORM, bool TAPE, bool DIRECT, int BM, int BN, int WM, int WN>
+int32_t launch(Mul p, hipStream_t stream, const char* name) {
+    p.tiles_n = (p.n + BN - 1) / BN;
+    p.pieces = FORM == WB ? (int64_t)p.ne * ((p.m + BM - 1) / BM) : (p.t + BM - 1) / BM + p.ne + 2;
+    const int64_t blocks = (p.pieces * p.tiles_n + 7) / 8 * 8;
+    if (blocks > (1 << 23)) return set_error(STADE_HIP_ERANGE, "%s: more than 2^23 tiles", name);
+    STADE_TIMED(name, stream, product_kernel<T, TC, FORM, TAPE, DIRECT, BM, BN, WM, WN><<<(unsigned)blocks, 64 * WM * WN, 0, stream>>>(p));
+    STADE_LAUNCHED(name);
+    return STADE_HIP_OK;
+}
+
+// whether all chunks of a matrix are whole and aligned, and a tile's offsets fit 31 bits
+inline bool whole(const void* p, int64_t ld, int64_t d, int64_t tile, size_t size) {
+    return (uintptr_t)p % 16 == 0 && ld * size % 16 == 0 && d * size % 16 == 0 && tile * ld * (int64_t)size < (1ll << 31);
 }
 
 template <class T, class TC, int FORM, bool TAPE>
 int32_t run(const Mul& p, hipStream_t stream, const char* name) {
-    const int64_t pieces = FORM == WB ? (int64_t)p.ne * ((p.m + TM - 1) / TM) : (p.t + TM - 1) / TM + p.ne + 2;
-    // (grid y is limited to 65535: the rest in further launches would need an offset)
-    if (pieces > 65535) return set_error(STADE_HIP_ERANGE, "%s: more than 65535 row tiles", name);
-    const dim3 grid((unsigned)((p.n + TN - 1) / TN), (unsigned)pieces);
-    STADE_TIMED(name, stream, simple_kernel<T, TC, FORM, TAPE><<<grid, NT, 0, stream>>>(p));
-    STADE_LAUNCHED(name);
-    return STADE_HIP_OK;
+    if constexpr (sizeof(T) == 4) {
+        return launch<T, TC, FORM, TAPE, false, 128, 128, 2, 2>(p, stream, name);
+    } else {
+        const bool direct = (TAPE || whole(p.a, p.lda, FORM == WB ? p.m : p.k, 256, sizeof(T))) &&
+                            whole(p.b, p.ldb, FORM == XB ? p.k : p.n, 256, sizeof(T));
+        const int64_t big = ((FORM == WB ? (int64_t)p.m * p.ne : p.t + 128 * (int64_t)p.ne) + 255) / 256 * ((p.n + 255) / 256);
+        if (big >= 192) {
+            if (direct) return launch<T, TC, FORM, TAPE, true, 256, 256, 2, 4>(p, stream, name);
+            return launch<T, TC, FORM, TAPE, false, 256, 256, 2, 4>(p, stream, name);
+        }
+        if (direct) return launch<T, TC, FORM, TAPE, true, 128, 128, 2, 2>(p, stream, name);
+        return launch<T, TC, FORM, TAPE, false, 128, 128, 2, 2>(p, stream, name);
+    }
 }
 
 int32_t check(const char* fn, int64_t tx, const int64_t* start, int64_t i_in, int64_t i_out, int64_t i_t, int64_t i_e) {
