@@ -9,6 +9,7 @@
 #include "tape8.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace stade {
 namespace {
@@ -31,64 +32,81 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
 }
 __device__ __forceinline__ Rows uniform(const Rows& r) { return Rows{uniform(r.e), uniform(r.row), uniform(r.rows)}; }
 
-// start[i] in order and in range: the largest of the offsets up to i, each between 0 and t.  (Offsets
-// that are neither raise the device error flag; no row then has two experts.)
-//
-// The job-th piece of at most BM rows, all experts' pieces counted in order, then those of the
-// rows before the first expert and after the last: every wave finds it by itself, 64 experts at a
-// time.  No rows: e = -2.
+// The experts' offsets 64 at a time, one a lane: lane l has boundary i = base + l, in order and in range
+// (the largest of the offsets up to i, each between 0 and t: offsets that are neither raise the device
+// error flag, and no row has two experts).  Segment i, the rows between boundaries i - 1 and i,
+// belongs to expert i - 1.
+struct Chunk {
+    int64_t from, end;       // segment i
+    int64_t before, mine;    // pieces of the segments before i (from segment 1 on), and of i
+};
 template <int BM>
-__device__ __forceinline__ Rows find_rows(const int64_t* start, int ne, int64_t t, int64_t job, int32_t* flag) {
-    const int lane = threadIdx.x & 63;
-    int64_t reach = 0, first = 0, pieces = 0;
-    Rows r{-2, 0, 0};
-    // boundary i of 0..ne: expert i - 1's end; segment i lies between boundaries i - 1 and i.
-    // Segment 0 is the rows before the first expert; it is counted after the experts.
-    for (int base = 0; base <= ne; base += 64) {
-        const int i = base + lane;
-        const int64_t raw = i <= ne ? start[i] : t;
-        int64_t end = min(max(raw, (int64_t)0), t);
+__device__ __forceinline__ Chunk scan(const int64_t* start, int ne, int64_t t, int base, int64_t reach, int64_t pieces, int32_t* flag) {
+    const int lane = threadIdx.x & 63, i = base + lane;
+    const int64_t raw = i <= ne ? start[i] : 0;
+    Chunk c;
+    c.end = i <= ne ? min(max(raw, (int64_t)0), t) : 0;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int64_t up = __shfl_up(end, o, 64);
-            if (lane >= o) end = max(end, up);
-        }
-        end = max(end, reach);
-        if (i <= ne && end != raw && flag) *flag = kErrIndex;
-        int64_t from = __shfl_up(end, 1, 64);
-        if (lane == 0) from = reach;
-        if (base == 0) first = __shfl(end, 0, 64);
-        const int64_t mine = i >= 1 && i <= ne ? (end - from + BM - 1) / BM : 0;
-        int64_t sum = mine;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t up = __shfl_up(c.end, o, 64);
+        if (lane >= o) c.end = max(c.end, up);
+    }
+    c.end = max(c.end, reach);
+    if (i <= ne && c.end != raw && flag) *flag = kErrIndex;
+    c.from = __shfl_up(c.end, 1, 64);
+    if (lane == 0) c.from = reach;
+    c.mine = i >= 1 && i <= ne ? (c.end - c.from + BM - 1) / BM : 0;
+    int64_t sum = c.mine;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int64_t up = __shfl_up(sum, o, 64);
-            if (lane >= o) sum += up;
-        }
-        const int64_t before = pieces + sum - mine;
-        const uint64_t hit = __ballot(mine > 0 && job >= before && job < before + mine);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            const int64_t row = __shfl(from, l, 64) + (job - __shfl(before, l, 64)) * BM;
-            r.e = base + l - 1;
-            r.row = row;
-            r.rows = (int)min((int64_t)BM, __shfl(end, l, 64) - row);
-            return r;
-        }
-        pieces += __shfl(sum, 63, 64);
-        reach = __shfl(end, 63, 64);
-        if (base + 64 > ne) reach = __shfl(end, ne - base, 64);
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t up = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += up;
     }
-    job -= pieces;
-    const int64_t head = (first + BM - 1) / BM;
-    const int64_t row = job < head ? job * BM : reach + (job - head) * BM, end = job < head ? first : t;
-    if (row < end) {
-        r.e = -1;
-        r.row = row;
-        r.rows = (int)min((int64_t)BM, end - row);
-    }
-    return r;
+    c.before = pieces + sum - c.mine;
+    return c;
 }
+
+// All pieces of at most BM rows: the experts', in order, then those of the rows before the first
+// expert and after the last.  Every wave finds them by itself.
+template <int BM>
+struct Pieces {
+    const int64_t* start;
+    int ne;
+    int64_t t;
+    Chunk first;
+    int64_t experts, head, reach;   // pieces of the experts; rows before the first; the last one's end
+
+    __device__ __forceinline__ Pieces(const int64_t* start_, int ne_, int64_t t_, int32_t* flag) : start(start_), ne(ne_), t(t_) {
+        first = scan<BM>(start, ne, t, 0, 0, 0, flag);
+        head = uniform((int64_t)__shfl(first.end, 0, 64));
+        Chunk c = first;
+        for (int base = 64; base <= ne; base += 64)
+            c = scan<BM>(start, ne, t, base, __shfl(c.end, 63, 64), __shfl(c.before + c.mine, 63, 64), flag);
+        experts = uniform((int64_t)__shfl(c.before + c.mine, 63, 64));
+        reach = uniform((int64_t)__shfl(c.end, 63, 64));
+    }
+    __device__ __forceinline__ int64_t count() const { return experts + (head + BM - 1) / BM + (t - reach + BM - 1) / BM; }
+    __device__ __forceinline__ Rows at(int64_t piece) const {
+        if (piece >= experts) {
+            piece -= experts;
+            const int64_t heads = (head + BM - 1) / BM;
+            const int64_t row = piece < heads ? piece * BM : reach + (piece - heads) * BM, end = piece < heads ? head : t;
+            return Rows{-1, row, (int)min((int64_t)BM, end - row)};
+        }
+        Chunk c = first;
+        for (int base = 0;;) {
+            const uint64_t hit = __ballot(c.mine > 0 && piece >= c.before && piece < c.before + c.mine);
+            if (hit) {
+                const int l = __builtin_ctzll(hit);
+                const int64_t row = __shfl(c.from, l, 64) + (piece - __shfl(c.before, l, 64)) * BM;
+                return uniform(Rows{base + l - 1, row, (int)min((int64_t)BM, __shfl(c.end, l, 64) - row)});
+            }
+            base += 64;   // (a piece below `experts` is found before the offsets end)
+            if (base > ne) return Rows{-1, 0, 0};
+            c = scan<BM>(start, ne, t, base, __shfl(c.end, 63, 64), __shfl(c.before + c.mine, 63, 64), nullptr);
+        }
+    }
+};
 
 // expert e's rows
 __device__ __forceinline__ Rows expert_rows(const int64_t* start, int ne, int64_t t, int e, int32_t* flag) {
@@ -123,8 +141,9 @@ struct Mul {
     int64_t t;
     int m, n, k;       // of one expert's product (m of xb and y, k of wb: its rows)
     int tiles_n;       // column tiles
-    int64_t pieces;    // row pieces (y, xb), or experts times row tiles (wb)
+    int64_t pieces;    // row pieces at most (y, xb), or experts times row tiles (wb)
     int add;
+    int cus;           // of the device
     int32_t* flag;
 };
 
@@ -141,16 +160,22 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 //   k-contiguous operand (x and yb rows; w for xb): ROWS rows of 128 bytes; row r holds its chunk c at
 //     place c ^ (r & 7), so that eight lanes that read one chunk of eight rows meet all the banks.
 //   row-contiguous operand (w for y; x and yb for wb): BK rows of ROWS values.  The 16-bit types are
-//     read through the transposing LDS read (16 lanes: four k of 16 rows); the 64-byte pieces of
-//     row k lie at place p ^ (k & 3), so that the four rows it reads lie on different banks.
+//     read through the transposing LDS read (16 lanes: four k of 16 rows, 32 bytes of each); the 32-byte
+//     pieces of row k lie at place p ^ turn_of(k), so that no two of the eight pieces that half a wave reads,
+//     be it lanes 0..31 or every other 16, lie on the same banks.
 template <class T> constexpr int kBK = 128 / (int)sizeof(T);
 template <class T> constexpr int kCE = 16 / (int)sizeof(T);
+
+template <int ROWS>
+__device__ __forceinline__ int turn_of(int k) {
+    return ((k & 3) << 1 | (k >> 3 & 1)) & (ROWS / 16 - 1);
+}
 
 // byte offset of chunk `c` of row `r` (KC), or of row k (not KC), in its tile
 template <class T, bool KC, int ROWS>
 __device__ __forceinline__ int chunk_at(int r, int c) {
     if constexpr (KC) return r * 128 + ((c ^ (r & 7)) << 4);
-    else if constexpr (sizeof(T) == 2) return r * ROWS * 2 + ((((c >> 2) ^ (r & 3)) << 6) | ((c & 3) << 4));
+    else if constexpr (sizeof(T) == 2) return r * ROWS * 2 + ((((c >> 1) ^ turn_of<ROWS>(r)) << 5) | ((c & 1) << 4));
     else return r * ROWS * 4 + (c << 4);
 }
 
@@ -167,7 +192,7 @@ __device__ __forceinline__ void my_chunk(int i, int& outer, int& inner) {
         constexpr int PER = ROWS / kCE<T>;
         outer = at / PER;
         int c = at % PER;
-        if constexpr (sizeof(T) == 2) c = ((c >> 2) ^ (outer & 3)) << 2 | (c & 3);
+        if constexpr (sizeof(T) == 2) c = ((c >> 1) ^ turn_of<ROWS>(outer)) << 1 | (c & 1);
         inner = c * kCE<T>;
     }
 }
@@ -187,6 +212,14 @@ __device__ __forceinline__ v4u load_chunk(const T* p, int left) {
     return __builtin_bit_cast(v4u, v);
 }
 
+// 16 bytes a lane from the buffer `r` at `off` to LDS, the wave's lanes from `at` on.  In assembly because
+// of the waits: for the builtin the compiler waits for all loads before the next LDS read of any
+// kind, as it cannot tell the buffers apart, and nothing is left in flight during the products.  It has
+// no output register (m0 is reserved: the compiler keeps nothing in it); wait_loads below counts it.
+__device__ __forceinline__ void load_to_lds(v4u r, uint32_t off, uint32_t at) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(r), "s"(at) : "memory");
+}
+
 // An operand's staging.  The chunks of the step at k0 go from memory to registers (load), and
 // later to LDS (store); or straight to LDS (DIRECT: 16-byte aligned rows, whole chunks).
 // `rows`: of this tile; `kmax`: the product's k.
@@ -198,33 +231,27 @@ struct Stage {
     int64_t ld;
     int rows, kmax;
 
-    __device__ __forceinline__ void load(v4u (&v)[PER], int k0) const {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            int o, n;
-            my_chunk<T, KC, ROWS, NT>(i, o, n);
-            const int left = KC ? (o < rows ? kmax - k0 - n : 0) : (k0 + o < kmax ? rows - n : 0);
-            v[i] = load_chunk(KC ? p + (int64_t)o * ld + k0 + n : p + (int64_t)(k0 + o) * ld + n, left);
-        }
+    using Held = v4u;
+    __device__ __forceinline__ void load(Held& v, int i, int k0) const {
+        int o, n;
+        my_chunk<T, KC, ROWS, NT>(i, o, n);
+        const int left = KC ? (o < rows ? kmax - k0 - n : 0) : (k0 + o < kmax ? rows - n : 0);
+        v = load_chunk(KC ? p + (int64_t)o * ld + k0 + n : p + (int64_t)(k0 + o) * ld + n, left);
     }
-    __device__ __forceinline__ static void store(const v4u (&v)[PER], char* lds) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) *reinterpret_cast<v4u*>(lds + (i * NT + threadIdx.x) * 16) = v[i];
+    __device__ __forceinline__ static void store(const Held& v, int i, char* lds) {
+        *reinterpret_cast<v4u*>(lds + (i * NT + threadIdx.x) * 16) = v;
     }
-    // straight to LDS by buffer loads: lanes past the rows or past k get an offset past the buffer,
-    // and zeros
-    __device__ __forceinline__ void direct(char* lds, int k0) const {
-        const T* base = KC ? p + k0 : p + (int64_t)k0 * ld;
-        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), (short)0, 0x7fffffff, 0x00020000);
-        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // straight to LDS: lanes past the rows or past k get an offset past the buffer, and zeros
+    __device__ __forceinline__ void direct(const char* lds, int k0) const {
+        const uint64_t base = (uint64_t)(KC ? p + k0 : p + (int64_t)k0 * ld);
+        const v4u r = {(uint32_t)base, (uint32_t)(base >> 32) & 0xffffu, 0x7fffffffu, 0x00020000u};
+        const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)lds + uniform((int)(threadIdx.x >> 6)) * 1024;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             int o, n;
             my_chunk<T, KC, ROWS, NT>(i, o, n);
             const bool here = KC ? o < rows && k0 + n < kmax : k0 + o < kmax && n < rows;
-            const uint32_t off = here ? (uint32_t)o * (uint32_t)ld * sizeof(T) + n * sizeof(T) : 0x80000000u;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(lds + (i * NT + wave * 64) * 16), 16, off, 0,
-                                                     0, 0);
+            load_to_lds(r, here ? (uint32_t)o * (uint32_t)ld * sizeof(T) + n * sizeof(T) : 0x80000000u, at + i * NT * 16);
         }
     }
 };
@@ -237,35 +264,33 @@ struct TapeStage {
     int64_t ng;
     int col, rows, kmax;                   // the tile's first column of the tape's rows
 
-    struct Held { uint2 q[PER]; uint32_t s[PER]; };
-    __device__ __forceinline__ void load(Held& v, int k0) const {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            int o, n;
-            my_chunk<T, false, ROWS, NT>(i, o, n);
-            v.q[i] = make_uint2(0, 0);
-            v.s[i] = 0;
-            if (k0 + o < kmax && n < rows) {   // (a chunk past the last value is zeros in the tape)
-                const int64_t row = k0 + o;
-                const uint8_t* at = q + row * ng * tape8::kGroup + col + n;
-                if constexpr (CE == 8) v.q[i] = *reinterpret_cast<const uint2*>(at);
-                else v.q[i].x = *reinterpret_cast<const uint32_t*>(at);
-                v.s[i] = qs[row * ng + (col + n) / tape8::kGroup];
-            }
-        }
+    // (by buffer loads, one for the bytes and one for the scale at every step: chunks past the rows or
+    // past k are zeros, and the loads in flight can be counted)
+    static constexpr int LOADS = 2 * PER;
+    typedef uint32_t Bytes __attribute__((ext_vector_type(CE / 4)));
+    struct Held { Bytes q; uint8_t s; };
+    __device__ __forceinline__ void load(Held& v, int i, int k0) const {
+        const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(q + (int64_t)k0 * ng * tape8::kGroup), (short)0,
+                                                                            0x7fffffff, 0x00020000);
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(qs + (int64_t)k0 * ng), (short)0, 0x7fffffff,
+                                                                            0x00020000);
+        int o, n;
+        my_chunk<T, false, ROWS, NT>(i, o, n);
+        const bool here = k0 + o < kmax && n < rows;   // (a chunk past the last value is zeros in the tape)
+        const uint32_t at = (uint32_t)o * (uint32_t)ng;
+        const uint32_t oq = here ? at * tape8::kGroup + col + n : 0x80000000u, os = here ? at + (col + n) / tape8::kGroup : 0x80000000u;
+        if constexpr (CE == 8) v.q = __builtin_bit_cast(Bytes, __builtin_amdgcn_raw_buffer_load_b64(rq, oq, 0, 0));
+        else v.q = (Bytes)(__builtin_amdgcn_raw_buffer_load_b32(rq, oq, 0, 0));
+        v.s = __builtin_amdgcn_raw_buffer_load_b8(rs, os, 0, 0);
     }
-    __device__ __forceinline__ static void store(const Held& v, char* lds) {
+    __device__ __forceinline__ static void store(const Held& v, int i, char* lds) {
         typedef T vec __attribute__((ext_vector_type(CE)));
+        // q + 128 as an unsigned byte, times the unit, less 128 units: exact
+        const float u = tape8::unit(v.s), low = -128.f * u;
+        vec x;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            // q + 128 as an unsigned byte, times the unit, less 128 units: exact
-            const float u = tape8::unit(v.s[i]), low = -128.f * u;
-            const uint32_t w[2] = {v.q[i].x ^ 0x80808080u, v.q[i].y ^ 0x80808080u};
-            vec x;
-#pragma unroll
-            for (int j = 0; j < CE; ++j) x[j] = (T)fmaf((float)((w[j >> 2] >> (8 * (j & 3))) & 0xffu), u, low);
-            *reinterpret_cast<v4u*>(lds + (i * NT + threadIdx.x) * 16) = __builtin_bit_cast(v4u, x);
-        }
+        for (int j = 0; j < CE; ++j) x[j] = (T)fmaf((float)(((v.q[j >> 2] ^ 0x80808080u) >> (8 * (j & 3))) & 0xffu), u, low);
+        *reinterpret_cast<v4u*>(lds + (i * NT + threadIdx.x) * 16) = __builtin_bit_cast(v4u, x);
     }
 };
 
@@ -277,8 +302,8 @@ __device__ __forceinline__ v4u fragment(const char* lds, int row0, int s) {
     if constexpr (KC) {
         return *reinterpret_cast<const v4u*>(lds + chunk_at<T, true, ROWS>(row0 + (lane & 31), 2 * s + h));
     } else if constexpr (sizeof(T) == 2) {
-        const int k = 16 * s + 8 * h + ((lane & 15) >> 2), seg = (row0 >> 5) ^ (k & 3);
-        const char* at = lds + k * ROWS * 2 + seg * 64 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+        const int k = 16 * s + 8 * h + ((lane & 15) >> 2), seg = ((row0 >> 4) + ((lane >> 4) & 1)) ^ turn_of<ROWS>(k);
+        const char* at = lds + k * ROWS * 2 + seg * 32 + (lane & 3) * 8;
         typedef __attribute__((address_space(3))) v4s* lp;
         const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(at)), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(at + 4 * ROWS * 2));
         typedef short v8s __attribute__((ext_vector_type(8)));
@@ -305,45 +330,73 @@ __device__ __forceinline__ floatx16 multiply(v4u a, v4u b, floatx16 c) {
     }
 }
 
-// The tile's place.  Blocks go round the 8 XCDs, each with an L2 of its own: an XCD gets a range of
-// tiles that lie together (kBand row pieces by all the columns), so that those which run at one
-// time share rows and columns in its L2.
+// A tile's place in the order of the tiles: kBand row pieces by all the columns, band after band, so that
+// the tiles which run at one time share rows and columns in L2.
 constexpr int kBand = 4;
-__device__ __forceinline__ bool my_tile(const Mul& p, int64_t& piece, int& tn) {
-    const int64_t total = p.pieces * p.tiles_n, per = (total + 7) / 8, id = (int64_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if ((blockIdx.x >> 3) >= per || id >= total) return false;
-    const int64_t band = id / (kBand * p.tiles_n), in = id - band * kBand * p.tiles_n, rows = min((int64_t)kBand, p.pieces - band * kBand);
+__device__ __forceinline__ void tile_place(int64_t id, int64_t pieces, int tiles_n, int64_t& piece, int& tn) {
+    const int64_t band = id / (kBand * tiles_n), in = id - band * kBand * tiles_n, rows = min((int64_t)kBand, pieces - band * kBand);
     tn = (int)(in / rows);
     piece = band * kBand + in % rows;
+}
+// Blocks go round the 8 XCDs, each with an L2 of its own: an XCD gets a range of the tiles that lie
+// together; of wb, whose experts differ in their work, a range of each expert's tiles.  items(): how many
+// numbers there are (some without a tile); item_place(): a number's tile, or false.
+template <int FORM>
+__device__ __forceinline__ int64_t items(const Mul& p, int64_t pieces) {
+    if constexpr (FORM == WB) return (pieces / p.ne * p.tiles_n + 7) / 8 * 8 * p.ne;
+    else return (pieces * p.tiles_n + 7) / 8 * 8;
+}
+template <int FORM>
+__device__ __forceinline__ bool item_place(const Mul& p, int64_t item, int64_t pieces, int64_t& piece, int& tn) {
+    if constexpr (FORM == WB) {
+        const int64_t mine = pieces / p.ne, per = (mine * p.tiles_n + 7) / 8, slot = item >> 3, e = slot / per;
+        const int64_t id = ((item + e) & 7) * per + slot - e * per;   // (turned by e: few tiles an expert go round too)
+        if (id >= mine * p.tiles_n) return false;
+        tile_place(id, mine, p.tiles_n, piece, tn);
+        piece += e * mine;
+    } else {
+        const int64_t total = pieces * p.tiles_n, per = (total + 7) / 8, id = (item & 7) * per + (item >> 3);
+        if (id >= total || (item >> 3) >= per) return false;
+        tile_place(id, pieces, p.tiles_n, piece, tn);
+    }
     return true;
 }
 
-template <class T, class TC, int FORM, bool TAPE, bool DIRECT, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void product_kernel(Mul p) {
-    constexpr int NT = 64 * WM * WN, MT = BM / WM / 32, NTL = BN / WN / 32, BK = kBK<T>;
+// wait until at most N of the wave's loads are under way
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    static_assert(N < 64);
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// One tile by a block.  ST buffers in LDS go round.  Straight loads of a step are issued ST - 1 steps before
+// it; what comes through registers is loaded two steps before and put into LDS one step before, a part
+// between each two quarters of the products.  One barrier a step: behind it the next step's tiles are
+// whole, and the buffer of this one is free.
+// The tile: rows m0 .. of the piece r (y, xb), or of expert r.e's weights (wb); columns n0 .. .
+template <class T, class TC, int FORM, bool TAPE, bool DIRECT, int BM, int BN, int WM, int WN, int ST>
+struct Tile {
+    static constexpr int NT = 64 * WM * WN, MT = BM / WM / 32, NTL = BN / WN / 32, BK = kBK<T>, LDS = ST * (BM + BN) * 128;
+    static_assert(ST == 2 || (DIRECT && !TAPE), "more buffers are for straight loads");
+    static __device__ __forceinline__ void run(const Mul& p, const Rows& r, int m0, int n0, char* lds) {
+    const int rows = min(BM, (FORM == WB ? p.m : r.rows) - m0), cols = min(BN, p.n - n0);
+    if (rows <= 0 || cols <= 0) return;
     constexpr bool AKC = FORM != WB, BKC = FORM == XB;
-    __shared__ char lds[2][(BM + BN) * 128];
-    int64_t piece;
-    int tn;
-    if (!my_tile(p, piece, tn)) return;
-    Rows r;
-    int m0 = 0;
-    if constexpr (FORM == WB) {
-        const int tiles_m = (p.m + BM - 1) / BM;
-        r = uniform(expert_rows(p.start, p.ne, p.t, (int)(piece / tiles_m), p.flag));
-        m0 = (int)(piece % tiles_m) * BM;
-    } else {
-        r = uniform(find_rows<BM>(p.start, p.ne, p.t, piece, p.flag));
-    }
-    if (r.e == -2 || (r.e < 0 && p.add)) return;
-    const int n0 = tn * BN, rows = FORM == WB ? min(BM, p.m - m0) : r.rows, cols = min(BN, p.n - n0);
-    const int k = FORM == WB ? r.rows : r.e < 0 ? 0 : p.k;
+    using SA = std::conditional_t<TAPE, TapeStage<T, BM, NT>, Stage<T, AKC, BM, NT>>;
+    using SB = Stage<T, BKC, BN, NT>;
+    const int k = FORM == WB ? r.rows : r.e < 0 ? 0 : p.k, steps = (k + BK - 1) / BK;
     const int64_t e = r.e < 0 ? 0 : r.e;
     const T* b = (const T*)p.b + (FORM == WB ? r.row * p.ldb + n0 : FORM == Y ? e * p.k * p.n + n0 : (e * p.n + n0) * p.k);
-    const Stage<T, BKC, BN, NT> sb{b, p.ldb, cols, k};
-    const Stage<T, AKC, BM, NT> sa{(const T*)p.a + r.row * p.lda + m0, p.lda, rows, k};
-    const int64_t ng = tape8::groups(p.m);
-    const TapeStage<T, BM, NT> st{p.q + r.row * ng * tape8::kGroup, p.qs + r.row * ng, ng, m0, rows, k};
+    const SB sb{b, p.ldb, cols, k};
+    SA sa;
+    if constexpr (TAPE) {
+        const int64_t ng = tape8::groups(p.m);
+        sa = SA{p.q + r.row * ng * tape8::kGroup, p.qs + r.row * ng, ng, m0, rows, k};
+    } else {
+        sa = SA{(const T*)p.a + (FORM == WB ? r.row * p.lda + m0 : (r.row + m0) * p.lda), p.lda, rows, k};
+    }
 
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave / WN * MT * 32, wn = wave % WN * NTL * 32;
     floatx16 acc[MT][NTL];
@@ -354,87 +407,225 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Mul p) {
 #pragma unroll
             for (int x = 0; x < 16; ++x) acc[i][j][x] = 0.f;
 
-    // (the weights come second: the operand order of the instruction gives each lane four
-    // consecutive columns of one row)
-    const auto compute = [&](const char* A, const char* B) {
+    const auto buffer = [&](int t) { return lds + t % ST * ((BM + BN) * 128); };
+    constexpr bool AREG = TAPE || !DIRECT, BREG = !DIRECT;
+    typename SA::Held ra[AREG ? SA::PER : 1];
+    typename SB::Held rb[BREG ? SB::PER : 1];
+    const auto straight = [&](int t) {
+        char* at = buffer(t);
+        if constexpr (!AREG) sa.direct(at, t * BK);
+        if constexpr (!BREG) sb.direct(at + BM * 128, t * BK);
+    };
+    // part s of 4: what the registers hold goes to `at`, and step t's values take its place
+    const auto part = [&](int s, char* at, int t, bool put, bool get) {
+        if constexpr (AREG) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            v4u fa[MT], fb[NTL];
+            for (int i = SA::PER * s / 4; i < SA::PER * (s + 1) / 4; ++i) {
+                if (put) SA::store(ra[i], i, at);
+                if (get) sa.load(ra[i], i, t * BK);
+            }
+        }
+        if constexpr (BREG) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i) fa[i] = fragment<T, AKC, BM>(A, wm + 32 * i, s);
-#pragma unroll
-            for (int j = 0; j < NTL; ++j) fb[j] = fragment<T, BKC, BN>(B, wn + 32 * j, s);
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NTL; ++j) acc[i][j] = multiply<T>(fb[j], fa[i], acc[i][j]);
+            for (int i = SB::PER * s / 4; i < SB::PER * (s + 1) / 4; ++i) {
+                if (put) SB::store(rb[i], i, at + BM * 128);
+                if (get) sb.load(rb[i], i, t * BK);
+            }
         }
     };
-    // While a step is multiplied from one pair of buffers, the next one comes into the other.
-    v4u ra[Stage<T, AKC, BM, NT>::PER], rb[Stage<T, BKC, BN, NT>::PER];
-    typename TapeStage<T, BM, NT>::Held rt;
-    const auto fetch = [&](char* A, char* B, int k0) {
-        if constexpr (TAPE) st.load(rt, k0);
-        else if constexpr (DIRECT) sa.direct(A, k0);
-        else sa.load(ra, k0);
-        if constexpr (DIRECT) sb.direct(B, k0);
-        else sb.load(rb, k0);
+    // the fragments of quarter s of step t, into one of two sets of registers
+    v4u fa[2][MT], fb[2][NTL];
+    const auto read = [&](int t, int s) {
+        const char *A = buffer(t), *B = A + BM * 128;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) fa[s & 1][i] = fragment<T, AKC, BM>(A, wm + 32 * i, s);
+#pragma unroll
+        for (int j = 0; j < NTL; ++j) fb[s & 1][j] = fragment<T, BKC, BN>(B, wn + 32 * j, s);
     };
-    const auto settle = [&](char* A, char* B) {
-        if constexpr (TAPE) st.store(rt, A);
-        else if constexpr (!DIRECT) sa.store(ra, A);
-        if constexpr (!DIRECT) sb.store(rb, B);
-        if constexpr (DIRECT) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const auto products = [&](int s) {
+        // (the weights come first: each lane gets four consecutive columns of one row)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NTL; ++j) acc[i][j] = multiply<T>(fb[s & 1][j], fa[s & 1][i], acc[i][j]);
+    };
+    if (steps > 0) {
+        if constexpr (AREG || BREG) {
+            // (past the last step the operands' guards give zeros)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) part(s, lds, 0, false, true);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) part(s, lds, 1, true, true);
+        }
+        for (int t = 0; t < ST - 1; ++t) straight(t);
+        if constexpr (DIRECT) wait_loads<TAPE ? 0 : (ST - 2) * (SA::PER + SB::PER)>();
         __syncthreads();
-    };
-    if (k > 0) {
-        fetch(lds[0], lds[0] + BM * 128, 0);
-        settle(lds[0], lds[0] + BM * 128);
-        int turn = 0;
-        for (int k0 = BK; k0 < k; k0 += BK) {
-            char* next = lds[turn ^ 1];
-            fetch(next, next + BM * 128, k0);
-            compute(lds[turn], lds[turn] + BM * 128);
-            settle(next, next + BM * 128);
-            turn ^= 1;
-        }
-        compute(lds[turn], lds[turn] + BM * 128);
+        straight(ST - 1);
+        read(0, 0);
     }
-    // lane: row lane % 32 of each 32, columns 8 g + 4 (lane / 32) + 0..3
-    TC* c = (TC*)p.c + (FORM == WB ? ((int64_t)r.e * p.m + m0) * p.n : r.row * p.ldc) + n0;
+    for (int t = 0; t < steps; ++t) {
+        char* next = buffer(t + 1);
+#pragma unroll
+        for (int s = 0; s < 3; ++s) {
+            read(t, s + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            products(s);
+            if constexpr (AREG || BREG) part(s, next, t + 2, true, true);
+        }
+        if constexpr (AREG || BREG) part(3, next, t + 2, true, true);
+        // the step's fragments are read and the next step's tiles are there (behind its straight loads
+        // only the tape's, or those of later steps, are under way): the buffer of step t is free
+        if constexpr (TAPE && DIRECT) wait_loads<TapeStage<T, BM, NT>::LOADS>();
+        else if constexpr (DIRECT) wait_loads<(ST - 2) * (SA::PER + SB::PER)>();
+        __syncthreads();
+        straight(t + ST);
+        read(t + 1, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        products(3);
+    }
+    if constexpr (DIRECT) wait_loads<0>();   // (of steps past the last: nothing may land after the block's end)
+    // A lane has row lane % 32 of each 32 and columns 8 g + 4 (lane / 32) + 0..3 of each 32: each wave
+    // turns 32 rows at a time in LDS of its own, so that a row's columns go out together (straight
+    // from the registers a store touches 32 rows with 16 or 32 bytes each: 7 us more for a 256 x 256 tile).
+    // The 16-byte chunks of row r lie at place c ^ (r & 7).
+    constexpr int CE = kCE<TC>, CHUNKS = NTL * 32 / CE;
+    static_assert(WM * WN * 32 * CHUNKS * 16 <= LDS && CHUNKS >= 4, "the waves' parts fit");
+    __syncthreads();
+    char* own = lds + wave * (32 * CHUNKS * 16);
+    TC* c = (TC*)p.c + (FORM == WB ? ((int64_t)r.e * p.m + m0) * p.n : (r.row + m0) * p.ldc) + n0;
     const int64_t ldc = FORM == WB ? p.n : p.ldc;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-        const int row = wm + 32 * i + (lane & 31);
-        if (row >= rows) continue;
+        const int row = lane & 31;
 #pragma unroll
         for (int j = 0; j < NTL; ++j)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const int col = wn + 32 * j + 8 * g + 4 * (lane >> 5);
-                if (col >= cols) continue;
-                float v[4];
-                TC* at = c + row * ldc + col;
-                if (p.add) {
-                    load_row(v, at, cols - col);
+                typedef TC vec __attribute__((ext_vector_type(4)));
+                vec v;
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) v[x] += acc[i][j][4 * g + x];
-                } else {
+                for (int x = 0; x < 4; ++x) v[x] = (TC)0.f;
+                if constexpr (sizeof(TC) == 4) {
 #pragma unroll
                     for (int x = 0; x < 4; ++x) v[x] = acc[i][j][4 * g + x];
+                    *reinterpret_cast<vec*>(own + (row * CHUNKS + ((8 * j + 2 * g + (lane >> 5)) ^ (row & 7 & (CHUNKS - 1)))) * 16) = v;
+                } else if (!p.add) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) v[x] = (TC)acc[i][j][4 * g + x];
+                    *reinterpret_cast<vec*>(own + (row * CHUNKS + ((4 * j + g) ^ (row & 7 & (CHUNKS - 1)))) * 16 + 8 * (lane >> 5)) = v;
                 }
-                store_row(at, v, cols - col);
             }
+        if (sizeof(TC) == 4 || !p.add) {
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int q = 0; q < 32 * CHUNKS / 64; ++q) {
+                const int at = q * 64 + lane, rr = at / CHUNKS, cc = at % CHUNKS, col = wn + cc * CE, mm = wm + 32 * i + rr;
+                typedef TC vec __attribute__((ext_vector_type(CE)));
+                const vec v = *reinterpret_cast<const vec*>(own + (rr * CHUNKS + (cc ^ (rr & 7 & (CHUNKS - 1)))) * 16);
+                if (mm < rows && col < cols) {
+                    float f[CE];
+                    TC* to = c + mm * ldc + col;
+                    if (p.add) {
+                        load_row(f, to, cols - col);
+#pragma unroll
+                        for (int x = 0; x < CE; ++x) f[x] += (float)v[x];
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < CE; ++x) f[x] = (float)v[x];
+                    }
+                    store_row(to, f, cols - col);
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+        } else {
+            // (16-bit results that add to what is there are rounded once: straight from the registers)
+            const int mm = wm + 32 * i + row;
+            if (mm < rows) {
+#pragma unroll
+                for (int j = 0; j < NTL; ++j)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int col = wn + 32 * j + 8 * g + 4 * (lane >> 5);
+                        if (col >= cols) continue;
+                        float f[4];
+                        TC* to = c + mm * ldc + col;
+                        load_row(f, to, cols - col);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) f[x] += acc[i][j][4 * g + x];
+                        store_row(to, f, cols - col);
+                    }
+            }
+        }
+    }
+    }
+};
+
+// the piece that holds tile `piece` of the pieces of BM rows, and its first row in it
+template <int FORM, int BM>
+__device__ __forceinline__ Rows piece_rows(const Mul& p, const Pieces<BM>* all, int64_t piece, int& m0) {
+    if constexpr (FORM == WB) {
+        const int tiles_m = (p.m + BM - 1) / BM;
+        m0 = (int)(piece % tiles_m) * BM;
+        return uniform(expert_rows(p.start, p.ne, p.t, (int)(piece / tiles_m), p.flag));
+    } else {
+        m0 = 0;
+        return all->at(piece);
     }
 }
 
-template <class T, class TC, int FORM, bool TAPE, bool DIRECT, int BM, int BN, int WM, int WN>
+// one size of tile
+template <class T, class TC, int FORM, bool TAPE, bool DIRECT, int BM, int BN, int WM, int WN, int ST>
+__global__ __launch_bounds__(64 * WM * WN) void product_kernel(Mul p) {
+    using One = Tile<T, TC, FORM, TAPE, DIRECT, BM, BN, WM, WN, ST>;
+    __shared__ char lds[One::LDS];
+    const Pieces<BM> all(p.start, FORM == WB ? 0 : p.ne, p.t, FORM == WB ? nullptr : p.flag);
+    const int64_t pieces = FORM == WB ? p.pieces : all.count();
+    int64_t piece;
+    int tn, m0;
+    if (blockIdx.x >= items<FORM>(p, pieces) || !item_place<FORM>(p, blockIdx.x, pieces, piece, tn)) return;
+    const Rows r = piece_rows<FORM, BM>(p, &all, piece, m0);
+    if (r.e < 0 && p.add) return;
+    One::run(p, r, m0, tn * BN, lds);
+}
+
+// Large tiles, 256 x 256, for as many whole rounds as the CUs make of them (one block a CU); the rest,
+// where it would leave half of the CUs or more idle, in 128 x 128 quarters: a round of those takes
+// less than half as long.
+template <class T, class TC, int FORM, bool TAPE, bool DIRECT>
+__global__ __launch_bounds__(512) void mixed_kernel(Mul p) {
+    using Large = Tile<T, TC, FORM, TAPE, DIRECT, 256, 256, 2, 4, 2>;
+    using Quarter = Tile<T, TC, FORM, TAPE, DIRECT, 128, 128, 2, 4, DIRECT && !TAPE ? 4 : 2>;
+    __shared__ char lds[Large::LDS > Quarter::LDS ? Large::LDS : Quarter::LDS];
+    const Pieces<256> all(p.start, FORM == WB ? 0 : p.ne, p.t, FORM == WB ? nullptr : p.flag);
+    const int64_t pieces = FORM == WB ? p.pieces : all.count(), total = items<FORM>(p, pieces);
+    const int64_t rest = total % p.cus, large = rest <= p.cus / 2 ? total - rest : total;
+    int64_t piece, item = blockIdx.x;
+    int tn, m0, quarter = -1;
+    if (item >= large) {   // (a tile's quarters lie 8 blocks apart: on one XCD)
+        const int64_t b = item - large;
+        quarter = (int)(b >> 3 & 3);
+        item = large + ((b >> 5) << 3 | (b & 7));
+        if (item >= total) return;
+    }
+    if (!item_place<FORM>(p, item, pieces, piece, tn)) return;
+    const Rows r = piece_rows<FORM, 256>(p, &all, piece, m0);
+    if (r.e < 0 && p.add) return;
+    if (quarter < 0) Large::run(p, r, m0, tn * 256, lds);
+    else Quarter::run(p, r, m0 + (quarter >> 1) * 128, tn * 256 + (quarter & 1) * 128, lds);
+}
+
+template <class T, class TC, int FORM, bool TAPE, bool DIRECT, int BM, int BN, int WM, int WN, int ST = 2>
 int32_t launch(Mul p, hipStream_t stream, const char* name) {
     p.tiles_n = (p.n + BN - 1) / BN;
     p.pieces = FORM == WB ? (int64_t)p.ne * ((p.m + BM - 1) / BM) : (p.t + BM - 1) / BM + p.ne + 2;
-    const int64_t blocks = (p.pieces * p.tiles_n + 7) / 8 * 8;
-    if (blocks > (1 << 23)) return set_error(STADE_HIP_ERANGE, "%s: more than 2^23 tiles", name);
-    STADE_TIMED(name, stream, product_kernel<T, TC, FORM, TAPE, DIRECT, BM, BN, WM, WN><<<(unsigned)blocks, 64 * WM * WN, 0, stream>>>(p));
+    const int64_t tiles = FORM == WB ? ((p.m + BM - 1) / BM * p.tiles_n + 7) / 8 * 8 * p.ne : (p.pieces * p.tiles_n + 7) / 8 * 8;
+    if (tiles > (1 << 22)) return set_error(STADE_HIP_ERANGE, "%s: more than 2^22 tiles", name);
+    if constexpr (BM == 256) {
+        const unsigned blocks = (unsigned)(tiles + 3 * ((p.cus / 2 + 7) / 8 * 8));
+        STADE_TIMED(name, stream, mixed_kernel<T, TC, FORM, TAPE, DIRECT><<<blocks, 512, 0, stream>>>(p));
+    } else {
+        STADE_TIMED(name, stream, product_kernel<T, TC, FORM, TAPE, DIRECT, BM, BN, WM, WN, ST><<<(unsigned)tiles, 64 * WM * WN, 0, stream>>>(p));
+    }
     STADE_LAUNCHED(name);
     return STADE_HIP_OK;
 }
@@ -451,13 +642,28 @@ int32_t run(const Mul& p, hipStream_t stream, const char* name) {
     } else {
         const bool direct = (TAPE || whole(p.a, p.lda, FORM == WB ? p.m : p.k, 256, sizeof(T))) &&
                             whole(p.b, p.ldb, FORM == XB ? p.k : p.n, 256, sizeof(T));
-        const int64_t big = ((FORM == WB ? (int64_t)p.m * p.ne : p.t + 128 * (int64_t)p.ne) + 255) / 256 * ((p.n + 255) / 256);
-        if (big >= 192) {
-            if (direct) return launch<T, TC, FORM, TAPE, true, 256, 256, 2, 4>(p, stream, name);
-            return launch<T, TC, FORM, TAPE, false, 256, 256, 2, 4>(p, stream, name);
+        // the tiles of 256 x 256 that the rows will make, half a tile more an expert
+        const int64_t est = (FORM == WB ? (int64_t)p.ne * ((p.m + 255) / 256) : p.t / 256 + (p.ne + 1) / 2) * ((p.n + 255) / 256);
+        // Few rows an expert (y and xb: at most 64): bound by reading w, so small tiles, many blocks and three or four
+        // steps in flight.  24 rows, 8 experts, 2048 x 4096: y 26.6 us (128 x 128 tiles 28.7, quarters 27.4), xb 24.8
+        // (45, 37).
+        const bool few = FORM != WB && p.t <= 64 * (int64_t)p.ne;
+        if (direct) {
+            if constexpr (FORM == Y) {
+                if (few) return launch<T, TC, FORM, TAPE, true, 64, 128, 1, 4, 3>(p, stream, name);
+            } else if constexpr (FORM == XB) {
+                if (few) return launch<T, TC, FORM, TAPE, true, 64, 64, 2, 2, 4>(p, stream, name);
+            }
+            // Less than a round of large tiles, more than one of quarters: 128 x 128 tiles of four waves, two
+            // blocks a CU.  4096 rows, 8 experts, 1024 x 1024: 22.8 us, with quarters 29.0; 1024 rows, 4 experts,
+            // 2048 x 2048, one round of quarters: 25.4 us, with these 28.4.
+            if (est < p.cus && 4 * est > p.cus) return launch<T, TC, FORM, TAPE, true, 128, 128, 2, 2>(p, stream, name);
+            return launch<T, TC, FORM, TAPE, true, 256, 256, 2, 4>(p, stream, name);
         }
-        if (direct) return launch<T, TC, FORM, TAPE, true, 128, 128, 2, 2>(p, stream, name);
-        return launch<T, TC, FORM, TAPE, false, 128, 128, 2, 2>(p, stream, name);
+        // Through registers: 1000 rows, 7 experts, 500 x 700 18 us, with large tiles and quarters 20.7; 24 rows, 8 experts,
+        // 2044 x 4100 55 us (113); 8000 rows 377 us, with large tiles 245.
+        if (few || 4 * est <= p.cus) return launch<T, TC, FORM, TAPE, false, 64, 64, 2, 2>(p, stream, name);
+        return launch<T, TC, FORM, TAPE, false, 256, 256, 2, 4>(p, stream, name);
     }
 }
 
@@ -468,6 +674,12 @@ int32_t check(const char* fn, int64_t tx, const int64_t* start, int64_t i_in, in
     if (int32_t rc = check_extent(fn, "i_t", i_t, kMostRows)) return rc;
     if (int32_t rc = check_extent(fn, "i_e", i_e, kMostExperts)) return rc;
     return start ? 0 : bad(fn, "start is null");
+}
+
+int cu_count() {
+    int dev = 0, cus = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 256;
+    return cus > 0 ? cus : 256;
 }
 
 int32_t* error_flag(Workspace* ws) { return (int32_t*)(ws->dscalars + kErrFlagSlot); }
@@ -492,6 +704,7 @@ int32_t stade_hip_expert_mul(int64_t tx, void* y, int64_t ldy, const void* x, in
     Mul p{};
     p.a = x; p.lda = ldx; p.b = w; p.ldb = i_out; p.c = y; p.ldc = ldy;
     p.start = start; p.ne = (int)i_e; p.t = i_t; p.n = (int)i_out; p.k = (int)i_in; p.add = add != 0; p.flag = error_flag(call.ws);
+    p.cus = cu_count();
     return with_type(tx, [&](auto t) -> int32_t { return run<decltype(t), decltype(t), Y, false>(p, stream, "expert_mul"); });
 }
 
@@ -515,6 +728,7 @@ int32_t stade_hip_expert_mul_b(int64_t tx, int64_t twb, const void* yb, int64_t 
     if (!call.ok()) return call.error();
     Mul p{};
     p.start = start; p.ne = (int)i_e; p.t = i_t; p.add = add != 0; p.flag = error_flag(call.ws);
+    p.cus = cu_count();
     return with_type(tx, [&](auto t) -> int32_t {
         using T = decltype(t);
         if (xb && i_t > 0) {
