@@ -196,3 +196,36 @@ def test_gradient_by_differences():
                              ((f(x, w + dw) - f(x, w - dw)) / 2, (wb.double() * c(dw).double()).sum(), size(x, w.abs() + dw.abs()))):
         # sums nest at most 80 deep on either side, and the shifted inputs are rounded once
         assert abs((ybd * got).sum() - want) <= 2 * 90 * U * (ybd.abs() * bound).sum()
+
+
+# sizes that make a round of the largest tiles and more (256 x 256 on 256 CUs): of y, of xb and of wb; whole
+# and aligned, and odd
+LARGE = [([700, 300, 513], 3, 64, 16384), ([700, 513], 0, 16384, 72), ([70, 0, 33], 0, 4104, 4096), ([700, 300, 513], 0, 67, 16389),
+         ([1213], 5, 16389, 35), ([70, 33], 0, 4099, 4103)]
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=IDS.get)
+@pytest.mark.parametrize("size", LARGE, ids=NAME)
+def test_large_tiles(size, dt):
+    import stade_hip
+    t, e, i, o, start, x, w, yb, g = _case(size, dt, seed=2)
+    print(f"expert_mul large {NAME(size)} {IDS[dt]}", flush=True)
+    xc, wc, ybc, sc = x.cuda(), w.cuda(), yb.cuda(), start.cuda()
+    y = torch.full((t, o), float("nan"), dtype=dt, device="cuda")
+    stade_hip.expert_mul(y, xc, wc, sc, i, o, t, e)
+    want, scale = _y(x.double(), w.double(), start)
+    within("y", y, want, U * (i + 4) * scale, dt)
+    xb = torch.full((t, i), float("nan"), dtype=dt, device="cuda")
+    wb = torch.full((e, i, o), float("nan"), device="cuda")
+    stade_hip.expert_mul_b(ybc, xc, xb, wc, wb, sc, i, o, t, e, add=False)
+    want, scale = _y(yb.double(), w.double().transpose(1, 2), start)
+    within("xb", xb, want, U * (o + 4) * scale, dt)
+    want, scale = _wb(x.double(), yb.double(), start, e)
+    within("wb", wb, want, U * (max(size[0]) + 8) * scale, torch.float32)
+    # from the tape, added to what is there
+    tape = new_tape(i, t)
+    stade_hip.tape8_store(xc, *tape, i, t)
+    base = wb.double().cpu()
+    stade_hip.expert_mul_b(ybc, None, None, None, wb, sc, i, o, t, e, tape=tape)
+    want, scale = _wb(tape_values(x.double()), yb.double(), start, e)
+    within("wb from the tape", wb, base + want, U * ((max(size[0]) + 8) * scale + 2 * (base + want).abs()), torch.float32)
