@@ -15,6 +15,7 @@
 #include "tape8.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace stade {
 namespace {
@@ -67,7 +68,7 @@ __device__ __forceinline__ void row_sum(float (&v)[NS], float* lds, int& turn) {
 
 template <int WPR> constexpr int block_of() { return WPR > 4 ? 64 * WPR : 256; }
 
-template <class T, class G, int VE, int NV, int WPR, bool TAPE>
+template <class T, class G, int VE, int NV, int WPR, bool TAPE, bool W>
 __global__ __launch_bounds__(block_of<WPR>()) void forward_kernel(Fwd p) {
     constexpr int NT = block_of<WPR>(), RPB = NT / (64 * WPR), STEP = 64 * WPR * VE;
     __shared__ float lds[2 * 16];
@@ -80,7 +81,7 @@ __global__ __launch_bounds__(block_of<WPR>()) void forward_kernel(Fwd p) {
         const T* x = (const T*)p.x + row * p.ldx;
         float v[NV][VE], s[1] = {0.f};
 #pragma unroll
-        for (int k = 0; k < NV; ++k) load_row(v[k], x + k * STEP + tr * VE, here ? d - (k * STEP + tr * VE) : 0);
+        for (int k = 0; k < NV; ++k) load_row<W>(v[k], x + k * STEP + tr * VE, here ? d - (k * STEP + tr * VE) : 0);
 #pragma unroll
         for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -92,7 +93,7 @@ __global__ __launch_bounds__(block_of<WPR>()) void forward_kernel(Fwd p) {
         for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int i = 0; i < VE; ++i) {
-                const float c = k * STEP + tr * VE + i < d ? v[k][i] - mu : 0.f;
+                const float c = k * STEP + tr * VE + (W ? 0 : i) < d ? v[k][i] - mu : 0.f;
                 s[0] += c * c;
             }
         row_sum<WPR, 1>(s, lds, turn);
@@ -116,14 +117,14 @@ __global__ __launch_bounds__(block_of<WPR>()) void forward_kernel(Fwd p) {
             const int col = k * STEP + tr * VE;
             if (col < d) {
                 float g[VE], b[VE];
-                if (p.g) load_row(g, (const G*)p.g + col, d - col);
-                if (p.b) load_row(b, (const G*)p.b + col, d - col);
+                if (p.g) load_row<W>(g, (const G*)p.g + col, d - col);
+                if (p.b) load_row<W>(b, (const G*)p.b + col, d - col);
 #pragma unroll
                 for (int i = 0; i < VE; ++i) {
                     const float h = (v[k][i] - mu) * rs;
                     v[k][i] = fmaf(h, p.g ? g[i] : 1.f, p.b ? b[i] : 0.f);
                 }
-                store_row(y + col, v[k], d - col);
+                store_row<W>(y + col, v[k], d - col);
             }
         }
     }
@@ -141,68 +142,125 @@ __device__ __forceinline__ void load_input(float (&v)[VE], const Bwd& p, int64_t
     }
 }
 
-template <class T, class G, int VE, int NV, int WPR, bool TAPE>
-__global__ __launch_bounds__(block_of<WPR>()) void backward_kernel(Bwd p) {
-    constexpr int NT = block_of<WPR>(), RPB = NT / (64 * WPR), STEP = 64 * WPR * VE;
+// a thread's values of a row as they come from memory, so that the next row's can be on their way
+// while this one's are worked on
+template <class T, int VE, bool TAPE, bool W>
+struct Raw {
+    typedef T vec __attribute__((ext_vector_type(VE)));
+    typedef uint8_t bytes __attribute__((ext_vector_type(VE)));
+    std::conditional_t<TAPE, bytes, vec> x;
+    vec yb;
+    uint8_t s;
+
+    __device__ __forceinline__ void load(const Bwd& p, int64_t row, int col) {
+        const int left = row < p.n ? p.d - col : 0;
+        if constexpr (TAPE) {
+            const int64_t ng = tape8::groups(p.d);
+            if (left > 0) {   // (the tape's rows are whole groups)
+                x = *reinterpret_cast<const bytes*>(p.q + row * ng * tape8::kGroup + col);
+                s = p.qs[row * ng + col / tape8::kGroup];
+            }
+        } else {
+            get(x, (const T*)p.x + row * p.ldx + col, left);
+        }
+        get(yb, (const T*)p.yb + row * p.ldyb + col, left);
+    }
+    static __device__ __forceinline__ void get(vec& v, const T* at, int left) {
+        if (W ? left > 0 : left >= VE) {
+            v = *reinterpret_cast<const typename Pack<T, VE>::loose*>(at);
+        } else if constexpr (!W) {
+#pragma unroll
+            for (int i = 0; i < VE; ++i) v[i] = i < left ? at[i] : (T)0.f;
+        }
+    }
+    __device__ __forceinline__ void values(float (&h)[VE], float (&a)[VE]) const {
+        if constexpr (TAPE) {
+            // q + 128 as an unsigned byte, times the unit, less 128 units: exact
+            const float u = tape8::unit(s), low = -128.f * u;
+#pragma unroll
+            for (int i = 0; i < VE; ++i) h[i] = fmaf((float)(uint8_t)(x[i] ^ 0x80), u, low);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VE; ++i) h[i] = (float)x[i];
+        }
+#pragma unroll
+        for (int i = 0; i < VE; ++i) a[i] = (float)yb[i];
+    }
+};
+
+template <class T, class G, int VE, int NV, int WPR, int NT, bool TAPE, bool W>
+__global__ __launch_bounds__(NT) void backward_kernel(Bwd p) {
+    constexpr int RPB = NT / (64 * WPR), STEP = 64 * WPR * VE;
     __shared__ float lds[2 * 16 * 2];
     __shared__ float sums[RPB > 1 ? 2 * NV * STEP : 1];
     int turn = 0;
     const int sub = threadIdx.x / (64 * WPR), tr = threadIdx.x % (64 * WPR), d = p.d;
-    float ag[NV][VE], ab[NV][VE];
+    float ag[NV][VE], ab[NV][VE], g[NV][VE];
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k) {
+        if (p.g) load_row<W>(g[k], (const G*)p.g + k * STEP + tr * VE, d - (k * STEP + tr * VE));
 #pragma unroll
-        for (int i = 0; i < VE; ++i) ag[k][i] = ab[k][i] = 0.f;
+        for (int i = 0; i < VE; ++i) {
+            ag[k][i] = ab[k][i] = 0.f;
+            if (!p.g) g[k][i] = 1.f;
+        }
+    }
     const int64_t trips = (p.n + RPB - 1) / RPB;
+    Raw<T, VE, TAPE, W> raw[NV];
+    int64_t row = (int64_t)blockIdx.x * RPB + sub;
+    float mu = row < p.n ? p.mu[row] : 0.f, rs = row < p.n ? p.rs[row] : 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) raw[k].load(p, row, k * STEP + tr * VE);
     for (int64_t trip = blockIdx.x; trip < trips; trip += gridDim.x) {
-        const int64_t row = trip * RPB + sub;
-        const bool here = row < p.n;
-        const float mu = here ? p.mu[row] : 0.f, rs = here ? p.rs[row] : 0.f;
+        const bool here = row < p.n;   // (the others run along for the barriers)
+        const int64_t next = row + (int64_t)gridDim.x * RPB;
+        const float m = mu, r = rs;
         float h[NV][VE], a[NV][VE], s[2] = {0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int col = k * STEP + tr * VE;
-#pragma unroll
-            for (int i = 0; i < VE; ++i) h[k][i] = 0.f;
-            if (here && col < d) load_input<T, VE, TAPE>(h[k], p, row, col);
-            load_row(a[k], (const T*)p.yb + row * p.ldyb + col, here ? d - col : 0);
+            raw[k].values(h[k], a[k]);
+            raw[k].load(p, next, k * STEP + tr * VE);
+        }
+        if (next < p.n) {
+            mu = p.mu[next];
+            rs = p.rs[next];
         }
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int col = k * STEP + tr * VE;
             if (here && col < d) {
-                float g[VE];
-                if (p.g) load_row(g, (const G*)p.g + col, d - col);
 #pragma unroll
                 for (int i = 0; i < VE; ++i) {
-                    const float xh = col + i < d ? (h[k][i] - mu) * rs : 0.f, yb = a[k][i];
-                    ag[k][i] += yb * xh;
+                    const float xh = W || col + i < d ? (h[k][i] - m) * r : 0.f, yb = a[k][i];
+                    ag[k][i] = fmaf(yb, xh, ag[k][i]);
                     ab[k][i] += yb;
                     h[k][i] = xh;
-                    a[k][i] = p.g ? yb * g[i] : yb;
+                    a[k][i] = yb * g[k][i];
                     s[0] += a[k][i];
-                    s[1] += a[k][i] * xh;
+                    s[1] = fmaf(a[k][i], xh, s[1]);
                 }
             }
         }
         row_sum<WPR, 2>(s, lds, turn);
-        if (!here || !p.xb) continue;
-        const float m0 = s[0] / (float)d, m1 = s[1] / (float)d;
-        T* xb = (T*)p.xb + row * p.ldxb;
+        if (here && p.xb) {
+            const float m0 = s[0] / (float)d, m1 = s[1] / (float)d;
+            T* xb = (T*)p.xb + row * p.ldxb;
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int col = k * STEP + tr * VE;
-            if (col < d) {
-                float o[VE];
-                if (p.add) load_row(o, xb + col, d - col);
+            for (int k = 0; k < NV; ++k) {
+                const int col = k * STEP + tr * VE;
+                if (col < d) {
+                    float o[VE];
+                    if (p.add) load_row<W>(o, xb + col, d - col);
 #pragma unroll
-                for (int i = 0; i < VE; ++i) {
-                    const float r = rs * (a[k][i] - m0 - h[k][i] * m1);
-                    a[k][i] = p.add ? o[i] + r : r;
+                    for (int i = 0; i < VE; ++i) {
+                        const float v = r * fmaf(-h[k][i], m1, a[k][i] - m0);
+                        a[k][i] = p.add ? o[i] + v : v;
+                    }
+                    store_row<W>(xb + col, a[k], d - col);
                 }
-                store_row(xb + col, a[k], d - col);
             }
         }
+        row = next;
     }
     if (!p.part) return;
     // the block's rows of partial sums joined, one after the other
@@ -349,25 +407,25 @@ __global__ __launch_bounds__(kLongNT) void backward_long_kernel(Bwd p) {
     }
 }
 
-// gb and bb from the blocks' partial sums: 32 columns a block, 8 threads a column, each over
-// its share of the partial rows in order, then the 8 in order.
-constexpr int kSumNT = 256;
+// gb and bb from the blocks' partial sums: 32 columns a block, 32 threads a column, each over its
+// share of the partial rows in order, then the 32 in order.
+constexpr int kSumNT = 1024;
 __global__ __launch_bounds__(kSumNT) void weight_sum_kernel(const float* part, int nparts, int d, float* gb, float* bb, int add) {
-    __shared__ float lds[8][33];
+    __shared__ float lds[32][33];
     const int c = threadIdx.x & 31, r = threadIdx.x >> 5, col = blockIdx.x * 32 + c;
     float* out = blockIdx.y ? bb : gb;
     const float* p = part + (blockIdx.y ? d : 0) + col;
     float s = 0.f;
     if (col < d) {
-        const int each = (nparts + 7) / 8, end = min(nparts, (r + 1) * each);
-#pragma unroll 8
+        const int each = (nparts + 31) / 32, end = min(nparts, (r + 1) * each);
+#pragma unroll 16
         for (int b = r * each; b < end; ++b) s += p[(int64_t)b * 2 * d];
     }
     lds[r][c] = s;
     __syncthreads();
     if (r == 0 && col < d && out) {
 #pragma unroll
-        for (int k = 1; k < 8; ++k) s += lds[k][c];
+        for (int k = 1; k < 32; ++k) s += lds[k][c];
         out[col] = add ? out[col] + s : s;
     }
 }
@@ -375,41 +433,46 @@ __global__ __launch_bounds__(kSumNT) void weight_sum_kernel(const float* part, i
 constexpr int kSumParts = 512;      // blocks of the reverse sweep at most: two a CU
 
 template <class T, class G, int VE, int NV, int WPR, bool TAPE>
-void start(const Fwd& p, unsigned, hipStream_t stream) {
-    constexpr int RPB = block_of<WPR>() / (64 * WPR);
+void start(const Fwd& p, hipStream_t stream) {
+    constexpr int NT = block_of<WPR>(), RPB = NT / (64 * WPR);
     const unsigned grid = (unsigned)std::min<int64_t>((p.n + RPB - 1) / RPB, 1 << 16);
-    forward_kernel<T, G, VE, NV, WPR, TAPE><<<grid, block_of<WPR>(), 0, stream>>>(p);
+    if (p.d % VE == 0) forward_kernel<T, G, VE, NV, WPR, TAPE, true><<<grid, NT, 0, stream>>>(p);
+    else forward_kernel<T, G, VE, NV, WPR, TAPE, false><<<grid, NT, 0, stream>>>(p);
 }
-template <class T, class G, int VE, int NV, int WPR, bool TAPE>
+template <class T, class G, int VE, int NV, int WPR, int NT, bool TAPE>
 void start(const Bwd& p, unsigned grid, hipStream_t stream) {
-    backward_kernel<T, G, VE, NV, WPR, TAPE><<<grid, block_of<WPR>(), 0, stream>>>(p);
+    if (p.d % VE == 0) backward_kernel<T, G, VE, NV, WPR, NT, TAPE, true><<<grid, NT, 0, stream>>>(p);
+    else backward_kernel<T, G, VE, NV, WPR, NT, TAPE, false><<<grid, NT, 0, stream>>>(p);
 }
 
-// The form by the row's length: the fewest waves a row whose registers hold it (8 vectors a thread
-// forward; 4 in the reverse sweep, which holds two rows and two sums).
+// The form by the row's length.  Forward: the fewest waves a row that hold it in 4 vectors a thread, from
+// 2048 on four waves.
 template <class T, class G, bool TAPE>
-void launch(const Fwd& p, unsigned grid, hipStream_t s) {
+void launch(const Fwd& p, hipStream_t s) {
     const int d = p.d;
-    if (d <= 128) start<T, G, 2, 1, 1, TAPE>(p, grid, s);
-    else if (d <= 512) start<T, G, 8, 1, 1, TAPE>(p, grid, s);
-    else if (d <= 1024) start<T, G, 8, 2, 1, TAPE>(p, grid, s);
-    else if (d <= 2048) start<T, G, 8, 4, 1, TAPE>(p, grid, s);
-    else if (d <= 4096) start<T, G, 8, 2, 4, TAPE>(p, grid, s);
-    else if (d <= 8192) start<T, G, 8, 4, 4, TAPE>(p, grid, s);
-    else if (d <= 16384) start<T, G, 8, 2, 16, TAPE>(p, grid, s);
-    else if (d <= 32768) start<T, G, 8, 4, 16, TAPE>(p, grid, s);
+    if (d <= 128) start<T, G, 2, 1, 1, TAPE>(p, s);
+    else if (d <= 512) start<T, G, 8, 1, 1, TAPE>(p, s);
+    else if (d <= 1024) start<T, G, 8, 2, 1, TAPE>(p, s);
+    else if (d <= 2048) start<T, G, 8, 1, 4, TAPE>(p, s);
+    else if (d <= 4096) start<T, G, 8, 4, 2, TAPE>(p, s);
+    else if (d <= 8192) start<T, G, 8, 4, 4, TAPE>(p, s);
+    else if (d <= 16384) start<T, G, 8, 2, 16, TAPE>(p, s);
+    else if (d <= 32768) start<T, G, 8, 4, 16, TAPE>(p, s);
     else forward_long_kernel<T, G, TAPE><<<(unsigned)std::min<int64_t>(p.n, 1 << 16), kLongNT, 0, s>>>(p);
 }
+// Reverse: one vector a thread up to 8192, so that two rows' values, their sums and the weights leave
+// room for 16 waves a CU.
+constexpr int back_rows(int64_t d) { return d <= 512 ? 8 : d <= 1024 ? 4 : d <= 2048 ? 2 : 1; }   // rows a block works on at a time
 template <class T, class G, bool TAPE>
 void launch(const Bwd& p, unsigned grid, hipStream_t s) {
     const int d = p.d;
-    if (d <= 128) start<T, G, 2, 1, 1, TAPE>(p, grid, s);
-    else if (d <= 512) start<T, G, 8, 1, 1, TAPE>(p, grid, s);
-    else if (d <= 1024) start<T, G, 8, 2, 1, TAPE>(p, grid, s);
-    else if (d <= 2048) start<T, G, 8, 1, 4, TAPE>(p, grid, s);
-    else if (d <= 4096) start<T, G, 8, 2, 4, TAPE>(p, grid, s);
-    else if (d <= 8192) start<T, G, 8, 4, 4, TAPE>(p, grid, s);
-    else if (d <= 16384) start<T, G, 8, 2, 16, TAPE>(p, grid, s);
+    if (d <= 128) start<T, G, 2, 1, 1, 512, TAPE>(p, grid, s);
+    else if (d <= 512) start<T, G, 8, 1, 1, 512, TAPE>(p, grid, s);
+    else if (d <= 1024) start<T, G, 8, 1, 2, 512, TAPE>(p, grid, s);
+    else if (d <= 2048) start<T, G, 8, 1, 4, 512, TAPE>(p, grid, s);
+    else if (d <= 4096) start<T, G, 8, 1, 8, 512, TAPE>(p, grid, s);
+    else if (d <= 8192) start<T, G, 8, 1, 16, 1024, TAPE>(p, grid, s);
+    else if (d <= 16384) start<T, G, 8, 4, 8, 512, TAPE>(p, grid, s);
     else backward_long_kernel<T, G, TAPE><<<grid, kLongNT, 0, s>>>(p);
 }
 
@@ -451,8 +514,8 @@ int32_t stade_hip_layernorm(int64_t tx, int64_t tg, void* y, int64_t ldy, const 
     const Fwd p{y, ldy, x, ldx, g, b, mu, rs, (uint8_t*)q, qs, (int)i_d, i_n, (float)eps};
     return with_types(tx, tg, [&](auto t, auto w) -> int32_t {
         STADE_TIMED("layernorm", stream, {
-            if (q) launch<decltype(t), decltype(w), true>(p, 0, stream);
-            else launch<decltype(t), decltype(w), false>(p, 0, stream);
+            if (q) launch<decltype(t), decltype(w), true>(p, stream);
+            else launch<decltype(t), decltype(w), false>(p, stream);
         });
         STADE_LAUNCHED("layernorm forward_kernel");
         return STADE_HIP_OK;
@@ -478,7 +541,7 @@ int32_t stade_hip_layernorm_b(int64_t tx, int64_t tg, const void* yb, int64_t ld
     const bool sums = gb || bb;
     if (!some && (!sums || add)) return STADE_HIP_OK;
     // a block's rows: enough blocks for two a CU, and no more (each leaves a row of partial sums)
-    const unsigned rpb = i_d <= 1024 ? 4 : 1;
+    const unsigned rpb = back_rows(i_d);
     const unsigned grid = (unsigned)std::min<int64_t>((i_n + rpb - 1) / rpb, kSumParts);
     WsCall call(stream);
     if (!call.ok()) return call.error();

@@ -35,10 +35,16 @@ struct Pack {
     typedef vec loose __attribute__((aligned(sizeof(T))));
 };
 
-// p[0..N) into v; values at and past `left` read as zero
-template <int N, class T>
+// p[0..N) into v; values at and past `left` read as zero.  WHOLE: `left` is a multiple of N (rows whose
+// length is one), and there are no tests value by value.
+template <bool WHOLE = false, int N, class T>
 __device__ __forceinline__ void load_row(float (&v)[N], const T* p, int left) {
-    if (left >= N) {
+    if constexpr (WHOLE) {
+        typename Pack<T, N>::vec x = {};
+        if (left > 0) x = *reinterpret_cast<const typename Pack<T, N>::loose*>(p);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = (float)x[i];
+    } else if (left >= N) {
         const typename Pack<T, N>::loose x = *reinterpret_cast<const typename Pack<T, N>::loose*>(p);
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = (float)x[i];
@@ -48,14 +54,14 @@ __device__ __forceinline__ void load_row(float (&v)[N], const T* p, int left) {
     }
 }
 
-template <int N, class T>
+template <bool WHOLE = false, int N, class T>
 __device__ __forceinline__ void store_row(T* p, const float (&v)[N], int left) {
-    if (left >= N) {
+    if (WHOLE ? left > 0 : left >= N) {
         typename Pack<T, N>::vec x;
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = (T)v[i];
         *reinterpret_cast<typename Pack<T, N>::loose*>(p) = x;
-    } else {
+    } else if constexpr (!WHOLE) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
             if (i < left) p[i] = (T)v[i];
