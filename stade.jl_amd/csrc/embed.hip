@@ -11,9 +11,10 @@
 //
 // embed_b adds no two rows by atomics: the ids are sorted first, and the sums go over the sorted
 // places in order, so the same call gives the same bits.  Launches:
-//   1. sort_block_kernel: block 0 sorts the ids in LDS (up to 16384 of them) while the
-//      other blocks, where wb is to be set, write the zero rows of ids that no token has.
-//   2. run_sum_kernel: the sorted places in chunks of kChunk; a wave adds 512 columns of a
+//   1. rank_kernel (up to 8192 tokens): every block finds the sorted places of some of them by counting,
+//      or sort_block_kernel (up to 16384): block 0 sorts the ids in LDS; the same blocks, or the others,
+//      write the zero rows of ids that no token has, where wb is to be set.
+//   2. run_sum_kernel: the sorted places in chunks; a wave adds 512 columns of a
 //      chunk's rows in fp32.  A run of one id that lies inside a chunk goes to wb at once; what a
 //      chunk holds of a run that spans chunks goes to a row of partial sums (at most two a chunk).
 //   3. run_join_kernel: for each run that spans chunks, its partial sums in order.
@@ -40,6 +41,8 @@ __device__ __forceinline__ uint32_t key_of(int64_t id, int64_t v, int32_t* flag)
 // ------------------------------------------------------------------------------------------
 // embed
 // ------------------------------------------------------------------------------------------
+// A row's last vector is moved back to end with the row (the values it shares with the one before are
+// written twice, the same): no tests value by value for rows of 8 or more.
 template <class TY, class TW>
 __global__ __launch_bounds__(NT) void embed_kernel(TY* y, int64_t ldy, const TW* w, int64_t ldw, const int64_t* tok, float s, int d, int64_t v,
                                                    int64_t t, int32_t* flag) {
@@ -47,9 +50,10 @@ __global__ __launch_bounds__(NT) void embed_kernel(TY* y, int64_t ldy, const TW*
     const int64_t jobs = t * strips, step = (int64_t)gridDim.x * (NT / 64);
     for (int64_t j = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6); j < jobs; j += step) {
         const int64_t row = j / strips;
-        const int col = (int)(j - row * strips) * kCols + lane * 8;
+        int col = (int)(j - row * strips) * kCols + lane * 8;
         const uint32_t key = key_of(tok[row], v, flag);
         if (col >= d) continue;
+        if (d >= 8) col = min(col, d - 8);
         float x[8];
         if (key < v) {
             load_row(x, w + (int64_t)key * ldw + col, d - col);
@@ -75,30 +79,32 @@ inline int bits_of(uint64_t most) {
     return b;
 }
 
-// exclusive sums of 512 counters per digit over the waves: cnt[w][b] becomes the first place of
-// wave w's items of digit b.  Threads 0..511 take a digit each.
-__device__ __forceinline__ void scan_bins(uint32_t (*cnt)[kBins], uint32_t* lds) {
+// Exclusive sums of the counters, digit by digit and wave by wave within it: cnt[w][b] becomes the first
+// place of wave w's items of digit b.  Thread b takes digit b.
+__device__ __forceinline__ void scan_bins(uint32_t (*cnt)[kBins], int bins, uint32_t* lds) {
     const int b = threadIdx.x, lane = b & 63, wave = b >> 6;
-    uint32_t total = 0;
-    if (b < kBins) {
-        for (int w = 0; w < kSortWaves; ++w) {
-            const uint32_t c = cnt[w][b];
-            cnt[w][b] = total;
-            total += c;
-        }
-    }
+    uint32_t c[kSortWaves], total = 0;
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) c[w] = b < bins ? cnt[w][b] : 0;   // (all in flight together)
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) total += c[w];
     uint32_t sum = total;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const uint32_t up = __shfl_up(sum, o, 64);
         if (lane >= o) sum += up;
     }
-    if (lane == 63) lds[wave] = sum;
+    if (lane == 63 && wave < kBins / 64) lds[wave] = sum;
     __syncthreads();
-    if (b < kBins) {
-        uint32_t first = sum - total;
-        for (int w = 0; w < wave; ++w) first += lds[w];
-        for (int w = 0; w < kSortWaves; ++w) cnt[w][b] += first;
+    if (b < bins) {
+        uint32_t at = sum - total;
+#pragma unroll
+        for (int w = 0; w < kBins / 64; ++w) at += w < wave ? lds[w] : 0;
+#pragma unroll
+        for (int w = 0; w < kSortWaves; ++w) {
+            cnt[w][b] = at;
+            at += c[w];
+        }
     }
     __syncthreads();
 }
@@ -109,7 +115,8 @@ __device__ __forceinline__ void scan_bins(uint32_t (*cnt)[kBins], uint32_t* lds)
 template <int K>
 __device__ __forceinline__ void sort_pass(uint32_t (&v)[K], int shift, int bits, uint32_t* items, uint32_t (*cnt)[kBins]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int i = threadIdx.x; i < kSortWaves * kBins; i += kSortNT) (&cnt[0][0])[i] = 0;
+    const int bins = 1 << bits;
+    for (int i = threadIdx.x; i < kSortWaves << bits; i += kSortNT) cnt[i >> bits][i & (bins - 1)] = 0;
     __syncthreads();
     volatile uint32_t* mine = cnt[wave];
     uint32_t rank[K];
@@ -129,7 +136,7 @@ __device__ __forceinline__ void sort_pass(uint32_t (&v)[K], int shift, int bits,
         __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();
-    scan_bins(cnt, items);   // (the items are in registers: their place holds the waves' sums)
+    scan_bins(cnt, bins, items);   // (the items are in registers: their place holds the waves' sums)
 #pragma unroll
     for (int k = 0; k < K; ++k) items[cnt[wave][(v[k] >> shift) & mask] + rank[k]] = v[k];
     __syncthreads();
@@ -205,17 +212,18 @@ __device__ __forceinline__ void zero_row(char* row, int64_t width) {
 
 constexpr int kZeroRows = 1024;   // ids a block looks for at a time
 
-// Blocks from 1 on: each takes a share of the ids, marks those that a token has (reading all
-// the tokens: they are few, and in L2) and clears the others' rows.
-__device__ __forceinline__ void zero_rows(const Sort& p, uint32_t* marks) {
-    const int64_t share = (p.v + gridDim.x - 2) / (gridDim.x - 1), first = (int64_t)(blockIdx.x - 1) * share;
+// Part `part` of `parts` of the ids: marks those that a token has (reading all the tokens' keys: they are
+// few, and in LDS or L2) and clears the others' rows.
+template <class Key>
+__device__ __forceinline__ void zero_rows(const Sort& p, int part, int parts, uint32_t* marks, Key&& key) {
+    const int64_t share = (p.v + parts - 1) / parts, first = (int64_t)part * share;
     const int64_t last = min(p.v, first + share);
     for (int64_t from = first; from < last; from += kZeroRows) {
         const int rows = (int)min((int64_t)kZeroRows, last - from);
         for (int i = threadIdx.x; i < kZeroRows; i += kSortNT) marks[i] = 0;
         __syncthreads();
         for (int i = threadIdx.x; i < p.n; i += kSortNT) {
-            const int64_t at = p.tok[i] - 1 - from;
+            const int64_t at = key(i) - from;
             if (at >= 0 && at < rows) marks[at] = 1;
         }
         __syncthreads();
@@ -225,12 +233,65 @@ __device__ __forceinline__ void zero_rows(const Sort& p, uint32_t* marks) {
     }
 }
 
+// The order of few tokens by counting: an item's place is the number of items before it, those of a
+// smaller key and those of its own key that came first.  Every block holds all the keys in LDS; a
+// wave takes an item at a time.  n^2 comparisons over all the CUs: 2 us for 5000 items, where the sort in
+// one block takes 10.  The same blocks then clear rows.
+constexpr int kRankMost = 8192;
+__global__ __launch_bounds__(kSortNT) void rank_kernel(Sort p) {
+    __shared__ uint32_t keys[kRankMost], marks[kZeroRows];
+    const int lane = threadIdx.x & 63, padded = (p.n + 255) / 256 * 256;
+    int64_t tok[kRankMost / kSortNT];
+#pragma unroll
+    for (int k = 0; k < kRankMost / kSortNT; ++k) {   // (all in flight together)
+        const int i = k * kSortNT + threadIdx.x;
+        tok[k] = i < p.n ? p.tok[i] : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < kRankMost / kSortNT; ++k) {
+        const int i = k * kSortNT + threadIdx.x;
+        if (i < padded) keys[i] = i < p.n ? key_of(tok[k], p.v, blockIdx.x == 0 ? p.flag : nullptr) : ~0u;
+    }
+    __syncthreads();
+    const auto below = [&](uint32_t key, int place) {   // items before (key, place)
+        int count = 0;
+        for (int j = lane * 4; j < padded; j += 256) {
+            const uint4 k = *reinterpret_cast<const uint4*>(keys + j);
+            count += k.x < key + (j < place);
+            count += k.y < key + (j + 1 < place);
+            count += k.z < key + (j + 2 < place);
+            count += k.w < key + (j + 3 < place);
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) count += __shfl_xor(count, o, 64);
+        return count;
+    };
+    const int waves = (int)gridDim.x * kSortWaves, ids = p.start ? (int)p.v + 1 : 0;
+    for (int w = (int)blockIdx.x * kSortWaves + (threadIdx.x >> 6); w < p.n + ids; w += waves) {
+        if (w < p.n) {
+            const uint32_t key = keys[w];
+            const int at = below(key, w);
+            if (lane == 0) {
+                if (p.key) p.key[at] = key;
+                if (p.place) p.place[at] = (uint32_t)w;
+                if (p.order) p.order[at] = (int64_t)w + 1;
+            }
+        } else {
+            const int at = below((uint32_t)(w - p.n), 0);
+            if (lane == 0) p.start[w - p.n] = at;
+        }
+    }
+    if (p.wb) {
+        zero_rows(p, blockIdx.x, gridDim.x, marks, [&](int i) { return (int64_t)keys[i]; });
+    }
+}
+
 template <int K>
 __global__ __launch_bounds__(kSortNT) void sort_block_kernel(Sort p) {
     __shared__ uint32_t items[K * kSortNT];
     __shared__ uint32_t cnt[kSortWaves][kBins];
     if (blockIdx.x > 0) {
-        zero_rows(p, &cnt[0][0]);
+        zero_rows(p, blockIdx.x - 1, gridDim.x - 1, &cnt[0][0], [&](int i) { return p.tok[i] - 1; });
         return;
     }
     sort_items<K>(p, items, cnt);
@@ -370,7 +431,8 @@ __global__ __launch_bounds__(NT) void zero_missing_kernel(const uint32_t* key, i
 // ------------------------------------------------------------------------------------------
 // sums over runs of one id
 // ------------------------------------------------------------------------------------------
-constexpr int kChunk = 32;   // sorted places a wave adds
+// Sorted places a wave adds: 16, or 8 where those make few waves.  (32: 16384 rows of 2048 take 50 us, 3001 of 515 19.)
+constexpr int kChunk = 16, kShortChunk = 8;
 
 struct Runs {
     const void* yb; int64_t ldyb;
@@ -378,35 +440,40 @@ struct Runs {
     const uint32_t* key; const uint32_t* place;
     float* part;         // two rows of d a chunk: of the run it begins with, and of the one it ends with
     float s;
-    int d, add;
+    int d, add, chunk;
     int64_t n, v;
 };
 
-template <class TW>
+template <class TW, bool W>
 __device__ __forceinline__ void put(const Runs& p, uint32_t key, int col, const float (&acc)[8]) {
     TW* out = (TW*)p.wb + (int64_t)key * p.ldwb + col;
     float o[8];
-    if (p.add) load_row(o, out, p.d - col);
+    if (p.add) load_row<W>(o, out, p.d - col);
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] = p.add ? fmaf(p.s, acc[i], o[i]) : p.s * acc[i];
-    store_row(out, o, p.d - col);
+    store_row<W>(out, o, p.d - col);
 }
 
-template <class TY, class TW>
+// W: no tests value by value.  A row's last vector is moved back to end with the row; what it shares with the
+// one before is written twice, the same.  (With `add` that is right within a wave, which reads before
+// it writes, but not where the last vector is a wave's only one: the values before it are another's.)
+template <class TY, class TW, bool W>
 __global__ __launch_bounds__(NT) void run_sum_kernel(Runs p) {
     const int strips = (p.d + kCols - 1) / kCols;
     const int64_t j = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6), chunk = j / strips;
-    const int64_t first = chunk * kChunk;
+    const int64_t first = chunk * p.chunk;
     if (first >= p.n) return;
-    const int lane = threadIdx.x & 63, col = (int)(j - chunk * strips) * kCols + lane * 8;
-    const int len = (int)min((int64_t)kChunk, p.n - first);
+    const int lane = threadIdx.x & 63;
+    int col = (int)(j - chunk * strips) * kCols + lane * 8;
+    if (W && col < p.d) col = min(col, p.d - 8);
+    const int len = (int)min((int64_t)p.chunk, p.n - first);
     // lane i: the chunk's i-th key and place; and the keys on both sides
     const uint32_t mykey = lane < len ? p.key[first + lane] : 0, myplace = lane < len ? p.place[first + lane] : 0;
     const uint32_t none = (uint32_t)p.v;
     const uint32_t prev = first > 0 ? p.key[first - 1] : ~0u, next = first + len < p.n ? p.key[first + len] : ~0u;
     float acc[8];
     bool begins = (uint32_t)__builtin_amdgcn_readlane((int)mykey, 0) != prev;   // the run began in this chunk
-    constexpr int AHEAD = 8;
+    constexpr int AHEAD = sizeof(TY) == 2 ? 16 : 8;   // rows on their way
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] = 0.f;
     for (int at = 0; at < len; at += AHEAD) {
@@ -415,7 +482,7 @@ __global__ __launch_bounds__(NT) void run_sum_kernel(Runs p) {
         for (int q = 0; q < AHEAD; ++q) {
             const int i = min(at + q, len - 1);
             const int64_t row = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)myplace, i);
-            load_row(x[q], (const TY*)p.yb + row * p.ldyb + col, p.d - col);
+            load_row<W>(x[q], (const TY*)p.yb + row * p.ldyb + col, p.d - col);
         }
 #pragma unroll
         for (int q = 0; q < AHEAD; ++q) {
@@ -429,8 +496,8 @@ __global__ __launch_bounds__(NT) void run_sum_kernel(Runs p) {
             if (i + 1 < len && after == key) continue;
             // the run's end in this chunk
             if (col < p.d) {
-                if (begins && after != key) put<TW>(p, key, col, acc);
-                else store_row(p.part + (chunk * 2 + (begins ? 1 : 0)) * p.d + col, acc, p.d - col);
+                if (begins && after != key) put<TW, W>(p, key, col, acc);
+                else store_row<W>(p.part + (chunk * 2 + (begins ? 1 : 0)) * p.d + col, acc, p.d - col);
             }
             begins = true;
 #pragma unroll
@@ -439,35 +506,40 @@ __global__ __launch_bounds__(NT) void run_sum_kernel(Runs p) {
     }
 }
 
-template <class TW>
+template <class TW, bool W>
 __global__ __launch_bounds__(NT) void run_join_kernel(Runs p) {
     const int strips = (p.d + kCols - 1) / kCols;
     const int64_t j = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6), chunk = j / strips;
-    const int64_t first = chunk * kChunk, past = first + kChunk;
+    const int64_t first = chunk * p.chunk, past = first + p.chunk;
     if (past >= p.n) return;
     // the run that ends this chunk begins in it and goes on in the next one
     const uint32_t key = p.key[past - 1];
     if (key == (uint32_t)p.v || p.key[past] != key) return;
     if (p.key[first] == key && first > 0 && p.key[first - 1] == key) return;
-    const int col = (int)(j - chunk * strips) * kCols + (threadIdx.x & 63) * 8;
+    int col = (int)(j - chunk * strips) * kCols + (threadIdx.x & 63) * 8;
+    if (W && col < p.d) col = min(col, p.d - 8);
+    // the first chunk that does not begin with the run's key, looked for in 64 chunks at a time
+    const int64_t chunks = (p.n + p.chunk - 1) / p.chunk;
+    int64_t lo = chunk + 1;
+    for (;;) {
+        const int64_t c = lo + (threadIdx.x & 63);
+        const uint64_t out = __ballot(c >= chunks || p.key[c * p.chunk] != key);
+        if (out) {
+            lo += __builtin_ctzll(out);
+            break;
+        }
+        lo += 64;
+    }
     if (col >= p.d) return;
     float acc[8], x[8];
-    load_row(acc, p.part + (chunk * 2 + 1) * p.d + col, p.d - col);
-    // how many chunks the run goes on over: the run's end by bisection over the chunks' first keys
-    const int64_t chunks = (p.n + kChunk - 1) / kChunk;
-    int64_t lo = chunk + 1, hi = chunks;
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (p.key[mid * kChunk] == key) lo = mid + 1;
-        else hi = mid;
-    }
+    load_row<W>(acc, p.part + (chunk * 2 + 1) * p.d + col, p.d - col);
 #pragma unroll 8
     for (int64_t c = chunk + 1; c < lo; ++c) {
-        load_row(x, p.part + c * 2 * p.d + col, p.d - col);
+        load_row<W>(x, p.part + c * 2 * p.d + col, p.d - col);
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[i] += x[i];
     }
-    put<TW>(p, key, col, acc);
+    put<TW, W>(p, key, col, acc);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -479,26 +551,31 @@ __global__ __launch_bounds__(NT) void run_join_kernel(Runs p) {
 size_t radix_blocks(int64_t n) { return (size_t)((n + kTile - 1) / kTile); }
 size_t radix_bytes(int64_t n) { return 2 * (size_t)n * 8 + radix_blocks(n) * kRadix * 4 + 256; }
 
+constexpr int64_t kFewIds = 1024;   // whose starts the sorting launch finds; more ids in a launch of their own
+
 bool one_block(int64_t n, int64_t v) {
-    return n <= kSortMost && bits_of((uint64_t)v) + bits_of((uint64_t)std::max<int64_t>(n - 1, 1)) <= 32;
+    return n <= kRankMost || (n <= kSortMost && bits_of((uint64_t)v) + bits_of((uint64_t)(n - 1)) <= 32);
 }
 
 int32_t sort(Sort s, bool zero, void* work, int cus, hipStream_t stream) {
     const int64_t n = s.n;
     s.key_bits = bits_of((uint64_t)s.v);
     if (one_block(n, s.v)) {
-        s.place_bits = bits_of((uint64_t)std::max<int64_t>(n - 1, 1));
         int64_t* start = s.start;
-        const bool apart = s.v > 4096;   // (one block would take long over many ids)
+        const bool apart = s.v > kFewIds;
         if (apart) s.start = nullptr;
-        // the blocks that clear rows: two a CU where the LDS leaves room
-        const unsigned grid = zero ? (unsigned)std::min<int64_t>(1 + s.v, 2 * cus) : 1;
+        if (!zero) s.wb = nullptr;
         STADE_TIMED("token_sort", stream, {
-            if (n <= 1 * kSortNT) sort_block_kernel<1><<<grid, kSortNT, 0, stream>>>(s);
-            else if (n <= 4 * kSortNT) sort_block_kernel<4><<<grid, kSortNT, 0, stream>>>(s);
-            else sort_block_kernel<16><<<grid, kSortNT, 0, stream>>>(s);
+            if (n <= kRankMost) {
+                const int64_t waves = (n + (s.start ? s.v + 1 : 0) + kSortWaves - 1) / kSortWaves;
+                rank_kernel<<<(unsigned)std::min<int64_t>(zero ? cus : waves, cus), kSortNT, 0, stream>>>(s);
+            } else {
+                // block 0 sorts; the others clear rows, one a CU
+                s.place_bits = bits_of((uint64_t)(n - 1));
+                sort_block_kernel<kSortMost / kSortNT><<<zero ? (unsigned)std::min<int64_t>(1 + s.v, cus) : 1, kSortNT, 0, stream>>>(s);
+            }
         });
-        STADE_LAUNCHED("embed sort_block_kernel");
+        STADE_LAUNCHED("embed rank_kernel or sort_block_kernel");
         if (apart && start) {
             STADE_TIMED("token_start", stream, start_kernel<<<(unsigned)((s.v + NT) / NT), NT, 0, stream>>>(s.key, n, s.v, start));
             STADE_LAUNCHED("embed start_kernel");
@@ -577,7 +654,7 @@ int32_t stade_hip_token_order(const int64_t* tok, int64_t* order, int64_t* start
     s.n = (int)i_t;
     s.flag = error_flag(call.ws);
     char* work = nullptr;
-    if (!one || i_v > 4096) {
+    if (!one || i_v > kFewIds) {
         const size_t keys = ((size_t)i_t * 4 + 255) / 256 * 256;
         if (!(work = (char*)scratch(keys + (one ? 0 : radix_bytes(i_t))))) return scratch_error();
         s.key = (uint32_t*)work;
@@ -637,7 +714,7 @@ int32_t stade_hip_embed_b(int64_t ty, int64_t tw, const void* yb, int64_t ldyb, 
     }
     WsCall call(stream);
     if (!call.ok()) return call.error();
-    const int64_t chunks = (i_t + kChunk - 1) / kChunk;
+    const int64_t strips = (i_d + kCols - 1) / kCols, chunk = i_t / kChunk * strips < 2048 ? kShortChunk : kChunk, chunks = (i_t + chunk - 1) / chunk;
     const size_t keys = ((size_t)i_t * 4 + 255) / 256 * 256, parts = ((size_t)chunks * 2 * (size_t)i_d * 4 + 255) / 256 * 256;
     const bool one = one_block(i_t, i_v);
     char* work = (char*)scratch(2 * keys + parts + (one ? 0 : radix_bytes(i_t)));
@@ -653,17 +730,23 @@ int32_t stade_hip_embed_b(int64_t ty, int64_t tw, const void* yb, int64_t ldyb, 
     o.row_bytes = row_bytes;
     o.width = width;
     if (int32_t rc = sort(o, !add && i_v > 0, work + 2 * keys + parts, cu_count(), stream)) return rc;
-    const Runs p{yb, ldyb, wb, ldwb, o.key, o.place, (float*)(work + 2 * keys), (float)s, (int)i_d, add != 0, i_t, i_v};
-    const int64_t jobs = chunks * ((i_d + kCols - 1) / kCols);
-    const unsigned grid = (unsigned)((jobs + NT / 64 - 1) / (NT / 64));
+    const Runs p{yb, ldyb, wb, ldwb, o.key, o.place, (float*)(work + 2 * keys), (float)s, (int)i_d, add != 0, (int)chunk, i_t, i_v};
+    const unsigned grid = (unsigned)((chunks * strips + NT / 64 - 1) / (NT / 64));
     return with_type(ty, [&](auto a) -> int32_t {
         return with_type(tw, [&](auto b) -> int32_t {
             using TY = decltype(a);
             using TW = decltype(b);
-            STADE_TIMED("embed_runs", stream, run_sum_kernel<TY, TW><<<grid, NT, 0, stream>>>(p));
+            const bool w = i_d >= 8 && (!add || i_d % kCols == 0 || i_d % kCols >= 8);
+            STADE_TIMED("embed_runs", stream, {
+                if (w) run_sum_kernel<TY, TW, true><<<grid, NT, 0, stream>>>(p);
+                else run_sum_kernel<TY, TW, false><<<grid, NT, 0, stream>>>(p);
+            });
             STADE_LAUNCHED("embed run_sum_kernel");
             if (chunks > 1) {
-                STADE_TIMED("embed_join", stream, run_join_kernel<TW><<<grid, NT, 0, stream>>>(p));
+                STADE_TIMED("embed_join", stream, {
+                    if (w) run_join_kernel<TW, true><<<grid, NT, 0, stream>>>(p);
+                    else run_join_kernel<TW, false><<<grid, NT, 0, stream>>>(p);
+                });
                 STADE_LAUNCHED("embed run_join_kernel");
             }
             return STADE_HIP_OK;

@@ -559,12 +559,12 @@ def _code(name: str, t) -> int:
     import torch
     if not _CODES:
         _CODES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
-    try:
-        return _CODES[t.dtype]
-    except (AttributeError, KeyError):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name}: expected a torch tensor on a GPU, got {type(t).__name__}") from None
-        raise TypeError(f"{name}: dtype {t.dtype}, expected float32, bfloat16 or float16") from None
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch tensor on a GPU, got {type(t).__name__}")
+    c = _CODES.get(t.dtype)
+    if c is None:
+        raise TypeError(f"{name}: dtype {t.dtype}, expected float32, bfloat16 or float16")
+    return c
 
 
 def _mat(name: str, t, d: int, n: int, dtype=None):
@@ -584,27 +584,26 @@ def _opt(name: str, t, dtype, numel: int):
     return None if t is None else _arr(name, t, dtype, numel)
 
 
-def _sizes(**kw) -> list:
-    out = []
-    for k, v in kw.items():
-        v = _int(k, v)
-        if v < 0:
-            raise ValueError(f"{k} is negative")
-        out.append(v)
-    return out
+def _nat(name: str, v) -> int:
+    if type(v) is not int:
+        v = _int(name, v)
+    if v < 0:
+        raise ValueError(f"{name} is negative")
+    return v
 
 
 def _one_device(*ts):
     """The tensors' device must be one, and the current one (the library works on the current
     device, as the other functions do)."""
     import torch
-    devs = {t.get_device() for t in ts if t is not None}
-    if len(devs) != 1 or devs != {torch.cuda.current_device()}:
-        raise ValueError(f"tensors on GPUs {sorted(devs)}: all must be on the current one ({torch.cuda.current_device()})")
+    cur = torch._C._cuda_getDevice()
+    for t in ts:
+        if t is not None and t.get_device() != cur:
+            raise ValueError(f"tensors on GPUs {sorted({u.get_device() for u in ts if u is not None})}: all must be on the current one ({cur})")
 
 
-def _flag(fn: str, check: bool, what: str):
-    if check and device_error():
+def _flag(fn: str, what: str):
+    if device_error():
         raise StadeHipBoundsError(f"{fn}: {what}")
 
 
@@ -613,26 +612,28 @@ def embed(y, w, tok, s, i_d, i_v, i_t, check=False):
     y (i_d, i_t), w (i_d, i_v).  Any other id is taken as 0; check=True raises StadeHipBoundsError
     for one (one synchronisation)."""
     import torch
-    d, v, t = _sizes(i_d=i_d, i_v=i_v, i_t=i_t)
+    d, v, t = _nat("i_d", i_d), _nat("i_v", i_v), _nat("i_t", i_t)
     ty, tw = _code("y", y), _code("w", w)
     (yp, ldy), (wp, ldw) = _mat("y", y, d, t), _mat("w", w, d, v)
     a = [ty, tw, yp, ldy, wp, ldw, _arr("tok", tok, torch.int64, t), float(s), d, v, t]
     _one_device(y, w, tok)
     _call("stade_hip_embed", a, _stream_of(y))
-    _flag("embed", check, "an id is outside 0..i_v")
+    if check:
+        _flag("embed", "an id is outside 0..i_v")
 
 
 def embed_b(yb, wb, tok, s, i_d, i_v, i_t, add=True, check=False):
     """Adjoint of embed: wb[:, v] += s * the sum of yb[:, t] over the t with tok[t] = v (add=False:
     wb is set).  By sorted tokens, in fixed order: the same call gives the same bits."""
     import torch
-    d, v, t = _sizes(i_d=i_d, i_v=i_v, i_t=i_t)
+    d, v, t = _nat("i_d", i_d), _nat("i_v", i_v), _nat("i_t", i_t)
     ty, tw = _code("yb", yb), _code("wb", wb)
     (yp, ldy), (wp, ldw) = _mat("yb", yb, d, t), _mat("wb", wb, d, v)
     a = [ty, tw, yp, ldy, wp, ldw, _arr("tok", tok, torch.int64, t), float(s), d, v, t, int(bool(add))]
     _one_device(yb, wb, tok)
     _call("stade_hip_embed_b", a, _stream_of(yb))
-    _flag("embed_b", check, "an id is outside 0..i_v")
+    if check:
+        _flag("embed_b", "an id is outside 0..i_v")
 
 
 def token_order(tok, order, start, i_v, i_t, check=False):
@@ -641,11 +642,12 @@ def token_order(tok, order, start, i_v, i_t, check=False):
     end of the last.  `order` as the ids of `embed` takes rows in that order; for ids that name
     experts, `start` is the `start` of expert_mul."""
     import torch
-    v, t = _sizes(i_v=i_v, i_t=i_t)
+    v, t = _nat("i_v", i_v), _nat("i_t", i_t)
     a = [_arr("tok", tok, torch.int64, t), _arr("order", order, torch.int64, t), _arr("start", start, torch.int64, v + 1), v, t]
     _one_device(tok, order, start)
     _call("stade_hip_token_order", a, _stream_of(tok))
-    _flag("token_order", check, "an id is outside 0..i_v")
+    if check:
+        _flag("token_order", "an id is outside 0..i_v")
 
 
 def tape8_lengths(i_d, i_n) -> tuple[int, int]:
@@ -666,7 +668,7 @@ def _tape(q, qs, d: int, n: int):
 
 def tape8_store(x, q, qs, i_d, i_n):
     """The 8-bit tape of x (i_d, i_n): groups of 32 of a column share a power-of-two scale."""
-    d, n = _sizes(i_d=i_d, i_n=i_n)
+    d, n = _nat("i_d", i_d), _nat("i_n", i_n)
     c = _code("x", x)
     xp, ldx = _mat("x", x, d, n)
     a = [c, xp, ldx, *_tape(q, qs, d, n), d, n]
@@ -676,7 +678,7 @@ def tape8_store(x, q, qs, i_d, i_n):
 
 def tape8_load(q, qs, x, i_d, i_n):
     """The values that an 8-bit tape holds, into x (i_d, i_n)."""
-    d, n = _sizes(i_d=i_d, i_n=i_n)
+    d, n = _nat("i_d", i_d), _nat("i_n", i_n)
     c = _code("x", x)
     xp, ldx = _mat("x", x, d, n)
     a = [c, *_tape(q, qs, d, n), xp, ldx, d, n]
@@ -697,7 +699,7 @@ def layernorm(y, x, g, b, mu, rs, i_d, i_n, eps=1e-5, tape=None):
     rs = 1 / sqrt(variance + eps) (Float32[i_n], kept for the adjoint; None: not kept).  g, b of x's
     type or Float32; None: 1 and 0.  tape = (q, qs): the 8-bit tape of x is written in the same pass."""
     import torch
-    d, n = _sizes(i_d=i_d, i_n=i_n)
+    d, n = _nat("i_d", i_d), _nat("i_n", i_n)
     tx = _code("x", x)
     (yp, ldy), (xp, ldx) = _mat("y", y, d, n, x.dtype), _mat("x", x, d, n)
     tg, gp, bp = _weights(g, b, x, d)
@@ -711,7 +713,7 @@ def layernorm_b(yb, x, xb, g, gb, bb, mu, rs, i_d, i_n, add=True, tape=None):
     """Adjoint of layernorm from its output's shadow yb and its input x, or with x = None the tape
     of x: xb, gb and bb are accumulated (add=False: set).  gb, bb Float32; xb, gb, bb may be None."""
     import torch
-    d, n = _sizes(i_d=i_d, i_n=i_n)
+    d, n = _nat("i_d", i_d), _nat("i_n", i_n)
     if (x is None) == (tape is None):
         raise ValueError("one of x and tape is needed, and not both")
     tx = _code("yb", yb)
@@ -732,13 +734,14 @@ def expert_mul(y, x, w, start, i_in, i_out, i_t, i_e, add=False, check=False):
     become 0.  add=True: y is accumulated.  check=True raises StadeHipBoundsError for offsets that decrease
     or lie outside 0..i_t (one synchronisation)."""
     import torch
-    i, o, t, e = _sizes(i_in=i_in, i_out=i_out, i_t=i_t, i_e=i_e)
+    i, o, t, e = _nat("i_in", i_in), _nat("i_out", i_out), _nat("i_t", i_t), _nat("i_e", i_e)
     tx = _code("x", x)
     (yp, ldy), (xp, ldx) = _mat("y", y, o, t, x.dtype), _mat("x", x, i, t)
     a = [tx, yp, ldy, xp, ldx, _arr("w", w, x.dtype, i * o * e), _arr("start", start, torch.int64, e + 1), i, o, t, e, int(bool(add))]
     _one_device(y, x, w, start)
     _call("stade_hip_expert_mul", a, _stream_of(x))
-    _flag("expert_mul", check, "start decreases or lies outside 0..i_t")
+    if check:
+        _flag("expert_mul", "start decreases or lies outside 0..i_t")
 
 
 def expert_mul_b(yb, x, xb, w, wb, start, i_in, i_out, i_t, i_e, add=True, tape=None, check=False):
@@ -746,7 +749,7 @@ def expert_mul_b(yb, x, xb, w, wb, start, i_in, i_out, i_t, i_e, add=True, tape=
     yb[:, t] * x[:, t]' (add=False: set), x as itself or, with x = None, as its tape.  wb Float32 or of yb's
     type; xb and wb may be None (w is needed for xb only, x or its tape for wb only)."""
     import torch
-    i, o, t, e = _sizes(i_in=i_in, i_out=i_out, i_t=i_t, i_e=i_e)
+    i, o, t, e = _nat("i_in", i_in), _nat("i_out", i_out), _nat("i_t", i_t), _nat("i_e", i_e)
     if wb is not None and (x is None) == (tape is None):
         raise ValueError("one of x and tape is needed, and not both")
     ty = _code("yb", yb)
@@ -761,4 +764,5 @@ def expert_mul_b(yb, x, xb, w, wb, start, i_in, i_out, i_t, i_e, add=True, tape=
          None if wb is None else _arr("wb", wb, wb.dtype, i * o * e), _arr("start", start, torch.int64, e + 1), i, o, t, e, int(bool(add))]
     _one_device(yb, x, xb, w, wb, start, *(tape or ()))
     _call("stade_hip_expert_mul_b", a, _stream_of(yb))
-    _flag("expert_mul_b", check, "start decreases or lies outside 0..i_t")
+    if check:
+        _flag("expert_mul_b", "start decreases or lies outside 0..i_t")
