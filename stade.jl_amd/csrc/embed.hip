@@ -18,7 +18,7 @@
 //      chunk's rows in fp32.  A run of one id that lies inside a chunk goes to wb at once; what a
 //      chunk holds of a run that spans chunks goes to a row of partial sums (at most two a chunk).
 //   3. run_join_kernel: for each run that spans chunks, its partial sums in order.
-// More tokens than one block sorts go through a radix sort over blocks, 8 bits a pass.
+// Up to 256 tokens take one launch, few_kernel.  More tokens than one block sorts go through a radix sort over blocks, 8 bits a pass.
 // Bound by HBM: yb read once, wb written once.
 #include "rows.hpp"
 
@@ -542,6 +542,62 @@ __global__ __launch_bounds__(NT) void run_join_kernel(Runs p) {
     put<TW, W>(p, key, col, acc);
 }
 
+// The whole adjoint of few tokens in one launch (three take 15 us whatever their work): every wave looks among
+// all the keys for those equal to its token's; the first such token's wave adds the rows of all, in
+// order.  The same blocks clear the rows of the ids that no token has.
+constexpr int kFewTokens = 256;
+template <class TY, class TW, bool W>
+__global__ __launch_bounds__(kSortNT) void few_kernel(Runs p, Sort o) {
+    __shared__ uint32_t keys[kFewTokens], marks[kZeroRows];
+    const int lane = threadIdx.x & 63, strips = (p.d + kCols - 1) / kCols;
+    if (threadIdx.x < kFewTokens)
+        keys[threadIdx.x] = (int)threadIdx.x < o.n ? key_of(o.tok[threadIdx.x], o.v, blockIdx.x == 0 ? o.flag : nullptr) : ~0u;
+    __syncthreads();
+    constexpr int Q = kFewTokens / 64, AHEAD = 8;
+    uint32_t mine[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) mine[q] = keys[q * 64 + lane];
+    const int jobs = o.n * strips, step = (int)gridDim.x * kSortWaves;
+    for (int j = (int)blockIdx.x * kSortWaves + (threadIdx.x >> 6); j < jobs; j += step) {
+        const int place = j / strips;
+        int col = (j - place * strips) * kCols + lane * 8;
+        if (W && col < p.d) col = min(col, p.d - 8);
+        const uint32_t key = keys[place];
+        if (key == (uint32_t)o.v) continue;
+        uint64_t same[Q];
+        bool first = true;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            same[q] = __ballot(mine[q] == key);
+            const int before = min(64, place - q * 64);   // places of this word that lie before this one
+            if (before > 0 && (same[q] & (before >= 64 ? ~0ull : (1ull << before) - 1))) first = false;
+        }
+        if (!first) continue;
+        float acc[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            uint64_t left = same[q];
+            while (left) {
+                float x[AHEAD][8];
+#pragma unroll
+                for (int a = 0; a < AHEAD; ++a) {
+                    const int row = q * 64 + (left ? __builtin_ctzll(left) : 0);
+                    load_row<W>(x[a], (const TY*)p.yb + (int64_t)row * p.ldyb + col, left ? p.d - col : 0);
+                    left &= left - 1;
+                }
+#pragma unroll
+                for (int a = 0; a < AHEAD; ++a)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) acc[i] += x[a][i];
+            }
+        }
+        if (col < p.d) put<TW, W>(p, key, col, acc);
+    }
+    if (o.wb) zero_rows(o, blockIdx.x, gridDim.x, marks, [&](int i) { return (int64_t)keys[i]; });
+}
+
 // ------------------------------------------------------------------------------------------
 // host
 // ------------------------------------------------------------------------------------------
@@ -714,7 +770,35 @@ int32_t stade_hip_embed_b(int64_t ty, int64_t tw, const void* yb, int64_t ldyb, 
     }
     WsCall call(stream);
     if (!call.ok()) return call.error();
-    const int64_t strips = (i_d + kCols - 1) / kCols, chunk = i_t / kChunk * strips < 2048 ? kShortChunk : kChunk, chunks = (i_t + chunk - 1) / chunk;
+    const int64_t strips = (i_d + kCols - 1) / kCols;
+    const bool w = i_d >= 8 && (!add || i_d % kCols == 0 || i_d % kCols >= 8);
+    if (i_t <= kFewTokens) {
+        Sort o{};
+        o.tok = tok;
+        o.v = i_v;
+        o.n = (int)i_t;
+        o.flag = error_flag(call.ws);
+        o.wb = add || i_v == 0 ? nullptr : (char*)wb;
+        o.row_bytes = row_bytes;
+        o.width = width;
+        Runs p{};
+        p.yb = yb; p.ldyb = ldyb; p.wb = wb; p.ldwb = ldwb; p.s = (float)s; p.d = (int)i_d; p.add = add != 0;
+        const int64_t cus = cu_count();
+        const unsigned grid = (unsigned)(o.wb ? cus : std::min<int64_t>((i_t * strips + kSortWaves - 1) / kSortWaves, 4 * cus));
+        return with_type(ty, [&](auto a) -> int32_t {
+            return with_type(tw, [&](auto b) -> int32_t {
+                using TY = decltype(a);
+                using TW = decltype(b);
+                STADE_TIMED("embed_few", stream, {
+                    if (w) few_kernel<TY, TW, true><<<grid, kSortNT, 0, stream>>>(p, o);
+                    else few_kernel<TY, TW, false><<<grid, kSortNT, 0, stream>>>(p, o);
+                });
+                STADE_LAUNCHED("embed few_kernel");
+                return STADE_HIP_OK;
+            });
+        });
+    }
+    const int64_t chunk = i_t / kChunk * strips < 2048 ? kShortChunk : kChunk, chunks = (i_t + chunk - 1) / chunk;
     const size_t keys = ((size_t)i_t * 4 + 255) / 256 * 256, parts = ((size_t)chunks * 2 * (size_t)i_d * 4 + 255) / 256 * 256;
     const bool one = one_block(i_t, i_v);
     char* work = (char*)scratch(2 * keys + parts + (one ? 0 : radix_bytes(i_t)));
@@ -736,7 +820,6 @@ int32_t stade_hip_embed_b(int64_t ty, int64_t tw, const void* yb, int64_t ldyb, 
         return with_type(tw, [&](auto b) -> int32_t {
             using TY = decltype(a);
             using TW = decltype(b);
-            const bool w = i_d >= 8 && (!add || i_d % kCols == 0 || i_d % kCols >= 8);
             STADE_TIMED("embed_runs", stream, {
                 if (w) run_sum_kernel<TY, TW, true><<<grid, NT, 0, stream>>>(p);
                 else run_sum_kernel<TY, TW, false><<<grid, NT, 0, stream>>>(p);

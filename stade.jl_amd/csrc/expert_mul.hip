@@ -144,6 +144,7 @@ struct Mul {
     int64_t pieces;    // row pieces at most (y, xb), or experts times row tiles (wb)
     int add;
     int cus;           // of the device
+    int split;         // slices of k (1: none); a slice's result goes to the c'th of so many whole results, fp32
     int32_t* flag;
 };
 
@@ -380,22 +381,29 @@ template <class T, class TC, int FORM, bool TAPE, bool DIRECT, int BM, int BN, i
 struct Tile {
     static constexpr int NT = 64 * WM * WN, MT = BM / WM / 32, NTL = BN / WN / 32, BK = kBK<T>, LDS = ST * (BM + BN) * 128;
     static_assert(ST == 2 || (DIRECT && !TAPE), "more buffers are for straight loads");
-    static __device__ __forceinline__ void run(const Mul& p, const Rows& r, int m0, int n0, char* lds) {
+    static __device__ __forceinline__ void run(const Mul& p, Rows r, int m0, int n0, char* lds, int slice = 0) {
     const int rows = min(BM, (FORM == WB ? p.m : r.rows) - m0), cols = min(BN, p.n - n0);
     if (rows <= 0 || cols <= 0) return;
     constexpr bool AKC = FORM != WB, BKC = FORM == XB;
     using SA = std::conditional_t<TAPE, TapeStage<T, BM, NT>, Stage<T, AKC, BM, NT>>;
     using SB = Stage<T, BKC, BN, NT>;
-    const int k = FORM == WB ? r.rows : r.e < 0 ? 0 : p.k, steps = (k + BK - 1) / BK;
+    int k = FORM == WB ? r.rows : r.e < 0 ? 0 : p.k, k_first = 0;
+    if (p.split > 1) {   // this slice's part of k
+        const int each = ((k + p.split - 1) / p.split + BK - 1) / BK * BK;
+        k_first = min(k, slice * each);
+        k = min(k - k_first, each);
+        if (FORM == WB) r.row += k_first;
+    }
+    const int steps = (k + BK - 1) / BK;
     const int64_t e = r.e < 0 ? 0 : r.e;
-    const T* b = (const T*)p.b + (FORM == WB ? r.row * p.ldb + n0 : FORM == Y ? e * p.k * p.n + n0 : (e * p.n + n0) * p.k);
+    const T* b = (const T*)p.b + (FORM == WB ? r.row * p.ldb + n0 : FORM == Y ? (e * p.k + k_first) * p.n + n0 : (e * p.n + n0) * p.k + k_first);
     const SB sb{b, p.ldb, cols, k};
     SA sa;
     if constexpr (TAPE) {
         const int64_t ng = tape8::groups(p.m);
         sa = SA{p.q + r.row * ng * tape8::kGroup, p.qs + r.row * ng, ng, m0, rows, k};
     } else {
-        sa = SA{(const T*)p.a + (FORM == WB ? r.row * p.lda + m0 : (r.row + m0) * p.lda), p.lda, rows, k};
+        sa = SA{(const T*)p.a + (FORM == WB ? r.row * p.lda + m0 : (r.row + m0) * p.lda + k_first), p.lda, rows, k};
     }
 
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave / WN * MT * 32, wn = wave % WN * NTL * 32;
@@ -493,6 +501,7 @@ struct Tile {
     __syncthreads();
     char* own = lds + wave * (32 * CHUNKS * 16);
     TC* c = (TC*)p.c + (FORM == WB ? ((int64_t)r.e * p.m + m0) * p.n : (r.row + m0) * p.ldc) + n0;
+    if (p.split > 1) c += slice * (FORM == WB ? (int64_t)p.ne * p.m : p.t) * p.n;
     const int64_t ldc = FORM == WB ? p.n : p.ldc;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
@@ -582,10 +591,12 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(Mul p) {
     const int64_t pieces = FORM == WB ? p.pieces : all.count();
     int64_t piece;
     int tn, m0;
-    if (blockIdx.x >= items<FORM>(p, pieces) || !item_place<FORM>(p, blockIdx.x, pieces, piece, tn)) return;
+    const int64_t all_items = items<FORM>(p, pieces);
+    const int slice = (int)(blockIdx.x / all_items);
+    if (slice >= p.split || !item_place<FORM>(p, blockIdx.x % all_items, pieces, piece, tn)) return;
     const Rows r = piece_rows<FORM, BM>(p, &all, piece, m0);
     if (r.e < 0 && p.add) return;
-    One::run(p, r, m0, tn * BN, lds);
+    One::run(p, r, m0, tn * BN, lds, slice);
 }
 
 // Large tiles, 256 x 256, for as many whole rounds as the CUs make of them (one block a CU); the rest,
@@ -614,6 +625,31 @@ __global__ __launch_bounds__(512) void mixed_kernel(Mul p) {
     else Quarter::run(p, r, m0 + (quarter >> 1) * 128, tn * 256 + (quarter & 1) * 128, lds);
 }
 
+// the slices' results added in order: 8 columns of a row a thread
+template <class TC>
+__global__ __launch_bounds__(256) void join_kernel(const float* part, int slices, TC* c, int64_t ldc, int64_t rows, int n, int add) {
+    const int vecs = (n + 7) / 8;
+    const int64_t all = rows * vecs;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / vecs;
+        const int col = (int)(i - row * vecs) * 8;
+        float sum[8], v[8];
+        load_row(sum, part + row * n + col, n - col);
+        for (int s = 1; s < slices; ++s) {
+            load_row(v, part + ((int64_t)s * rows + row) * n + col, n - col);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) sum[x] += v[x];
+        }
+        TC* to = c + row * ldc + col;
+        if (add) {
+            load_row(v, to, n - col);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) sum[x] += v[x];
+        }
+        store_row(to, sum, n - col);
+    }
+}
+
 template <class T, class TC, int FORM, bool TAPE, bool DIRECT, int BM, int BN, int WM, int WN, int ST = 2>
 int32_t launch(Mul p, hipStream_t stream, const char* name) {
     p.tiles_n = (p.n + BN - 1) / BN;
@@ -621,10 +657,11 @@ int32_t launch(Mul p, hipStream_t stream, const char* name) {
     const int64_t tiles = FORM == WB ? ((p.m + BM - 1) / BM * p.tiles_n + 7) / 8 * 8 * p.ne : (p.pieces * p.tiles_n + 7) / 8 * 8;
     if (tiles > (1 << 22)) return set_error(STADE_HIP_ERANGE, "%s: more than 2^22 tiles", name);
     if constexpr (BM == 256) {
+        p.split = 1;
         const unsigned blocks = (unsigned)(tiles + 3 * ((p.cus / 2 + 7) / 8 * 8));
         STADE_TIMED(name, stream, mixed_kernel<T, TC, FORM, TAPE, DIRECT><<<blocks, 512, 0, stream>>>(p));
     } else {
-        STADE_TIMED(name, stream, product_kernel<T, TC, FORM, TAPE, DIRECT, BM, BN, WM, WN, ST><<<(unsigned)tiles, 64 * WM * WN, 0, stream>>>(p));
+        STADE_TIMED(name, stream, product_kernel<T, TC, FORM, TAPE, DIRECT, BM, BN, WM, WN, ST><<<(unsigned)(tiles * p.split), 64 * WM * WN, 0, stream>>>(p));
     }
     STADE_LAUNCHED(name);
     return STADE_HIP_OK;
@@ -637,23 +674,55 @@ inline bool whole(const void* p, int64_t ld, int64_t d, int64_t tile, size_t siz
 
 template <class T, class TC, int FORM, bool TAPE>
 int32_t run(const Mul& p, hipStream_t stream, const char* name) {
+    const bool direct = (TAPE || whole(p.a, p.lda, FORM == WB ? p.m : p.k, 256, sizeof(T))) &&
+                        whole(p.b, p.ldb, FORM == XB ? p.k : p.n, 256, sizeof(T));
+    // the tiles of 256 x 256 that the rows will make, half a tile more an expert
+    const int64_t est = (FORM == WB ? (int64_t)p.ne * ((p.m + 255) / 256) : p.t / 256 + (p.ne + 1) / 2) * ((p.n + 255) / 256);
+    // Fewer tiles of 64 x 64 than CUs and a long k: k in slices, for two blocks a CU, where that saves 12 steps or more
+    // (a step takes a microsecond; the launch that adds the slices up takes five).  64 rows, 4 experts, 1672 x 2484, bf16: y
+    // 43.4 -> 31.3 us, xb 45.7 -> 25.8; 3584 rows, 2 experts, 128 x 295: wb 37 -> 20; in fp32 137 rows, 4 experts, 1856 x 256: y
+    // 71 -> 18.  Saving 8 steps: 1000 rows, 7 experts, 500 x 700, fp32: 18.7 -> 23.7.
+    {
+        const int64_t small = std::max<int64_t>(1, (FORM == WB ? (int64_t)p.ne * ((p.m + 63) / 64) : p.t / 64 + std::min<int64_t>(p.ne, p.t)) * ((p.n + 63) / 64));
+        const int64_t steps = (FORM == WB ? p.t / p.ne : p.k) / kBK<T>, slices = std::min<int64_t>(std::min<int64_t>(2 * p.cus / small, steps / 4), 32);
+        if (small < p.cus && slices >= 2 && steps - steps / slices >= 12) {
+            const int64_t rows = FORM == WB ? (int64_t)p.ne * p.m : p.t;
+            Mul q = p;
+            q.split = (int)slices;
+            q.add = 0;
+            q.ldc = p.n;
+            if (!(q.c = scratch((size_t)slices * rows * p.n * sizeof(float)))) return scratch_error();
+            const int32_t rc = direct ? launch<T, float, FORM, TAPE, true, 64, 64, 2, 2, TAPE ? 2 : 4>(q, stream, name)
+                                      : launch<T, float, FORM, TAPE, false, 64, 64, 2, 2>(q, stream, name);
+            if (rc) return rc;
+            const unsigned grid = (unsigned)std::min<int64_t>((rows * ((p.n + 7) / 8) + 255) / 256, 1 << 14);
+            STADE_TIMED("expert_mul_join", stream,
+                        join_kernel<TC><<<grid, 256, 0, stream>>>((const float*)q.c, q.split, (TC*)p.c, FORM == WB ? p.n : p.ldc, rows, p.n, p.add));
+            STADE_LAUNCHED("expert_mul join_kernel");
+            return STADE_HIP_OK;
+        }
+    }
+    // Few rows an expert (y and xb: at most 64): bound by reading w, so small tiles, many blocks and three or four
+    // steps in flight.  24 rows, 8 experts, 2048 x 4096, bf16: y 26.6 us (128 x 128 tiles 28.7, quarters 27.4), xb 24.8
+    // (45, 37).
+    const bool few = FORM != WB && p.t <= 64 * (int64_t)p.ne;
+    if constexpr (!TAPE) {
+        if (direct && few) {
+            if constexpr (FORM == Y) return launch<T, TC, FORM, TAPE, true, 64, 128, 1, 4, 3>(p, stream, name);
+            else return launch<T, TC, FORM, TAPE, true, 64, 64, 2, 2, 4>(p, stream, name);
+        }
+    }
     if constexpr (sizeof(T) == 4) {
+        // fp32 is bound by its matrix instructions: the tile that fills the CUs (1000 rows, 7 experts, 500 x 700: 64 x 64
+        // 18 us, 128 x 128 42; 8192 rows, 8 experts, 2048 x 1024: y 378 and 408, wb 302 and 272)
+        if (direct) {
+            if (est < 2 * p.cus) return launch<T, TC, FORM, TAPE, true, 64, 64, 2, 2, TAPE ? 2 : 4>(p, stream, name);
+            return launch<T, TC, FORM, TAPE, true, 128, 128, 2, 2>(p, stream, name);
+        }
+        if (est < 2 * p.cus) return launch<T, TC, FORM, TAPE, false, 64, 64, 2, 2>(p, stream, name);
         return launch<T, TC, FORM, TAPE, false, 128, 128, 2, 2>(p, stream, name);
     } else {
-        const bool direct = (TAPE || whole(p.a, p.lda, FORM == WB ? p.m : p.k, 256, sizeof(T))) &&
-                            whole(p.b, p.ldb, FORM == XB ? p.k : p.n, 256, sizeof(T));
-        // the tiles of 256 x 256 that the rows will make, half a tile more an expert
-        const int64_t est = (FORM == WB ? (int64_t)p.ne * ((p.m + 255) / 256) : p.t / 256 + (p.ne + 1) / 2) * ((p.n + 255) / 256);
-        // Few rows an expert (y and xb: at most 64): bound by reading w, so small tiles, many blocks and three or four
-        // steps in flight.  24 rows, 8 experts, 2048 x 4096: y 26.6 us (128 x 128 tiles 28.7, quarters 27.4), xb 24.8
-        // (45, 37).
-        const bool few = FORM != WB && p.t <= 64 * (int64_t)p.ne;
         if (direct) {
-            if constexpr (FORM == Y) {
-                if (few) return launch<T, TC, FORM, TAPE, true, 64, 128, 1, 4, 3>(p, stream, name);
-            } else if constexpr (FORM == XB) {
-                if (few) return launch<T, TC, FORM, TAPE, true, 64, 64, 2, 2, 4>(p, stream, name);
-            }
             // Less than a round of large tiles, more than one of quarters: 128 x 128 tiles of four waves, two
             // blocks a CU.  4096 rows, 8 experts, 1024 x 1024: 22.8 us, with quarters 29.0; 1024 rows, 4 experts,
             // 2048 x 2048, one round of quarters: 25.4 us, with these 28.4.
@@ -705,6 +774,7 @@ int32_t stade_hip_expert_mul(int64_t tx, void* y, int64_t ldy, const void* x, in
     p.a = x; p.lda = ldx; p.b = w; p.ldb = i_out; p.c = y; p.ldc = ldy;
     p.start = start; p.ne = (int)i_e; p.t = i_t; p.n = (int)i_out; p.k = (int)i_in; p.add = add != 0; p.flag = error_flag(call.ws);
     p.cus = cu_count();
+    p.split = 1;
     return with_type(tx, [&](auto t) -> int32_t { return run<decltype(t), decltype(t), Y, false>(p, stream, "expert_mul"); });
 }
 
@@ -729,6 +799,7 @@ int32_t stade_hip_expert_mul_b(int64_t tx, int64_t twb, const void* yb, int64_t 
     Mul p{};
     p.start = start; p.ne = (int)i_e; p.t = i_t; p.add = add != 0; p.flag = error_flag(call.ws);
     p.cus = cu_count();
+    p.split = 1;
     return with_type(tx, [&](auto t) -> int32_t {
         using T = decltype(t);
         if (xb && i_t > 0) {

@@ -22,8 +22,8 @@ def _tokens(g, t, v, kind):
     return tok
 
 
-SIZES = [(1, 1, 1), (1, 8, 5), (5, 513, 3), (31, 64, 40), (33, 7, 2), (64, 520, 1000), (1000, 65, 130), (1025, 16, 5000),
-         (4097, 9, 70000), (5000, 1030, 11)]
+SIZES = [(1, 1, 1), (1, 8, 5), (5, 513, 3), (31, 64, 40), (33, 7, 2), (64, 520, 1000), (256, 515, 40), (257, 72, 300), (1000, 65, 130), (1025, 16, 5000),
+         (4097, 9, 70000), (5000, 1030, 11), (9000, 33, 20000)]
 
 
 @pytest.mark.parametrize("ty", TYPES, ids=IDS.get)

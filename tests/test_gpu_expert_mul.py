@@ -198,6 +198,20 @@ def test_gradient_by_differences():
         assert abs((ybd * got).sum() - want) <= 2 * 90 * U * (ybd.abs() * bound).sum()
 
 
+# few tiles and a long k: of y, of xb and of wb; whole and aligned, and odd
+LONG = [([20, 0, 30], 3, 2000, 72), ([40], 1, 64, 2104), ([1500, 700], 2, 56, 64), ([20, 0, 30], 3, 2001, 71), ([40], 1, 65, 2103),
+        ([1500, 700], 2, 51, 67)]
+
+
+@pytest.mark.parametrize("add", [False, True], ids=["set", "add"])
+@pytest.mark.parametrize("dt", TYPES, ids=IDS.get)
+@pytest.mark.parametrize("size", LONG, ids=NAME)
+def test_long_k(size, dt, add):
+    test_forward(size, dt, add)
+    test_backward(size, dt, "x", add)
+    test_backward(size, dt, "tape", add)
+
+
 # sizes that make a round of the largest tiles and more (256 x 256 on 256 CUs): of y, of xb and of wb; whole
 # and aligned, and odd
 LARGE = [([700, 300, 513], 3, 64, 16384), ([700, 513], 0, 16384, 72), ([70, 0, 33], 0, 4104, 4096), ([700, 300, 513], 0, 67, 16389),
