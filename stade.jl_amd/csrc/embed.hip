@@ -206,8 +206,13 @@ __device__ __forceinline__ void zero_row(char* row, int64_t width) {
     const v4u z = {0, 0, 0, 0};
     const int lane = threadIdx.x & 63;
     const int64_t whole = width / 16 * 16;
-    for (int64_t o = lane * 16; o < whole; o += 64 * 16) *reinterpret_cast<loose4*>(row + o) = z;
-    for (int64_t o = whole + lane * 2; o < width; o += 64 * 2) *reinterpret_cast<uint16_t*>(row + o) = 0;
+    int64_t o = lane * 16;
+    for (; o + 3 * 1024 < whole; o += 4 * 1024) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) *reinterpret_cast<loose4*>(row + o + k * 1024) = z;
+    }
+    for (; o < whole; o += 1024) *reinterpret_cast<loose4*>(row + o) = z;
+    for (o = whole + lane * 2; o < width; o += 64 * 2) *reinterpret_cast<uint16_t*>(row + o) = 0;
 }
 
 constexpr int kZeroRows = 1024;   // ids a block looks for at a time
@@ -624,7 +629,7 @@ int32_t sort(Sort s, bool zero, void* work, int cus, hipStream_t stream) {
         STADE_TIMED("token_sort", stream, {
             if (n <= kRankMost) {
                 const int64_t waves = (n + (s.start ? s.v + 1 : 0) + kSortWaves - 1) / kSortWaves;
-                rank_kernel<<<(unsigned)std::min<int64_t>(zero ? cus : waves, cus), kSortNT, 0, stream>>>(s);
+                rank_kernel<<<(unsigned)std::min<int64_t>(zero ? 2 * cus : waves, 2 * cus), kSortNT, 0, stream>>>(s);
             } else {
                 // block 0 sorts; the others clear rows, one a CU
                 s.place_bits = bits_of((uint64_t)(n - 1));
@@ -784,7 +789,7 @@ int32_t stade_hip_embed_b(int64_t ty, int64_t tw, const void* yb, int64_t ldyb, 
         Runs p{};
         p.yb = yb; p.ldyb = ldyb; p.wb = wb; p.ldwb = ldwb; p.s = (float)s; p.d = (int)i_d; p.add = add != 0;
         const int64_t cus = cu_count();
-        const unsigned grid = (unsigned)(o.wb ? cus : std::min<int64_t>((i_t * strips + kSortWaves - 1) / kSortWaves, 4 * cus));
+        const unsigned grid = (unsigned)(o.wb ? 2 * cus : std::min<int64_t>((i_t * strips + kSortWaves - 1) / kSortWaves, 4 * cus));
         return with_type(ty, [&](auto a) -> int32_t {
             return with_type(tw, [&](auto b) -> int32_t {
                 using TY = decltype(a);
