@@ -198,15 +198,16 @@ __device__ __forceinline__ void my_chunk(int i, int& outer, int& inner) {
     }
 }
 
-// 16 bytes of the operand through registers: any alignment, zeros past `left` values
-template <class T>
-__device__ __forceinline__ v4u load_chunk(const T* p, int left) {
+// 16 bytes of the operand through registers, at any alignment: the first `left` values, and zeros.  PAST: what
+// lies behind them may come along instead of the zeros, as far as the matrix goes (`end`).
+template <bool PAST, class T>
+__device__ __forceinline__ v4u load_chunk(const T* p, int left, const T* end) {
     typedef T vec __attribute__((ext_vector_type(kCE<T>)));
     typedef vec loose __attribute__((aligned(sizeof(T))));
-    vec v;
-    if (left >= kCE<T>) {
+    vec v = {};
+    if (left >= kCE<T> || (PAST && left > 0 && p + kCE<T> <= end)) {
         v = *reinterpret_cast<const loose*>(p);
-    } else {
+    } else if (left > 0) {   // (rare, and every load is waited for: lanes without values stay out)
 #pragma unroll
         for (int i = 0; i < kCE<T>; ++i) v[i] = i < left ? p[i] : (T)0.f;
     }
@@ -231,13 +232,15 @@ struct Stage {
     const T* p;
     int64_t ld;
     int rows, kmax;
+    const T* end;    // of the whole matrix
 
     using Held = v4u;
     __device__ __forceinline__ void load(Held& v, int i, int k0) const {
         int o, n;
         my_chunk<T, KC, ROWS, NT>(i, o, n);
         const int left = KC ? (o < rows ? kmax - k0 - n : 0) : (k0 + o < kmax ? rows - n : 0);
-        v = load_chunk(KC ? p + (int64_t)o * ld + k0 + n : p + (int64_t)(k0 + o) * ld + n, left);
+        // (rows past the tile's make results that are not stored; k past the product's must be zeros)
+        v = load_chunk<!KC>(KC ? p + (int64_t)o * ld + k0 + n : p + (int64_t)(k0 + o) * ld + n, left, end);
     }
     __device__ __forceinline__ static void store(const Held& v, int i, char* lds) {
         *reinterpret_cast<v4u*>(lds + (i * NT + threadIdx.x) * 16) = v;
@@ -397,13 +400,14 @@ struct Tile {
     const int steps = (k + BK - 1) / BK;
     const int64_t e = r.e < 0 ? 0 : r.e;
     const T* b = (const T*)p.b + (FORM == WB ? r.row * p.ldb + n0 : FORM == Y ? (e * p.k + k_first) * p.n + n0 : (e * p.n + n0) * p.k + k_first);
-    const SB sb{b, p.ldb, cols, k};
+    const SB sb{b, p.ldb, cols, k, (const T*)p.b + (FORM == WB ? (p.t - 1) * p.ldb + p.n : (int64_t)p.ne * p.k * p.n)};
     SA sa;
     if constexpr (TAPE) {
         const int64_t ng = tape8::groups(p.m);
         sa = SA{p.q + r.row * ng * tape8::kGroup, p.qs + r.row * ng, ng, m0, rows, k};
     } else {
-        sa = SA{(const T*)p.a + (FORM == WB ? r.row * p.lda + m0 : (r.row + m0) * p.lda + k_first), p.lda, rows, k};
+        sa = SA{(const T*)p.a + (FORM == WB ? r.row * p.lda + m0 : (r.row + m0) * p.lda + k_first), p.lda, rows, k,
+                (const T*)p.a + (p.t - 1) * p.lda + (FORM == WB ? p.m : p.k)};
     }
 
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wm = wave / WN * MT * 32, wn = wave % WN * NTL * 32;

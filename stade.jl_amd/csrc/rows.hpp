@@ -50,7 +50,11 @@ __device__ __forceinline__ void load_row(float (&v)[N], const T* p, int left) {
         for (int i = 0; i < N; ++i) v[i] = (float)x[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = i < left ? (float)p[i] : 0.f;
+        for (int i = 0; i < N; ++i) v[i] = 0.f;
+        if (left > 0) {   // (lanes past the row stay out of the loads and their waits)
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = i < left ? (float)p[i] : 0.f;
+        }
     }
 }
 
@@ -62,9 +66,11 @@ __device__ __forceinline__ void store_row(T* p, const float (&v)[N], int left) {
         for (int i = 0; i < N; ++i) x[i] = (T)v[i];
         *reinterpret_cast<typename Pack<T, N>::loose*>(p) = x;
     } else if constexpr (!WHOLE) {
+        if (left > 0) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (i < left) p[i] = (T)v[i];
+            for (int i = 0; i < N; ++i)
+                if (i < left) p[i] = (T)v[i];
+        }
     }
 }
 
