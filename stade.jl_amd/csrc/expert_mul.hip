@@ -159,7 +159,7 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 
 // Operand tiles in LDS, in 16-byte chunks of CE values.  A step takes BK values of k.
 //   k-contiguous operand (x and yb rows; w for xb): ROWS rows of 128 bytes; row r holds its chunk c at
-//     place c ^ (r & 7), so that eight lanes that read one chunk of eight rows meet all the banks.
+//     place c ^ (r / 2 & 7), so that sixteen lanes that read one chunk of sixteen rows meet all the banks.
 //   row-contiguous operand (w for y; x and yb for wb): BK rows of ROWS values.  The 16-bit types are
 //     read through the transposing LDS read (16 lanes: four k of 16 rows, 32 bytes of each); the 32-byte
 //     pieces of row k lie at place p ^ turn_of(k), so that no two of the eight pieces that half a wave reads,
@@ -175,7 +175,7 @@ __device__ __forceinline__ int turn_of(int k) {
 // byte offset of chunk `c` of row `r` (KC), or of row k (not KC), in its tile
 template <class T, bool KC, int ROWS>
 __device__ __forceinline__ int chunk_at(int r, int c) {
-    if constexpr (KC) return r * 128 + ((c ^ (r & 7)) << 4);
+    if constexpr (KC) return r * 128 + ((c ^ (r >> 1 & 7)) << 4);
     else if constexpr (sizeof(T) == 2) return r * ROWS * 2 + ((((c >> 1) ^ turn_of<ROWS>(r)) << 5) | ((c & 1) << 4));
     else return r * ROWS * 4 + (c << 4);
 }
@@ -188,7 +188,7 @@ __device__ __forceinline__ void my_chunk(int i, int& outer, int& inner) {
     const int at = i * NT + threadIdx.x;
     if constexpr (KC) {
         outer = at >> 3;
-        inner = ((at & 7) ^ (outer & 7)) * kCE<T>;
+        inner = ((at & 7) ^ (outer >> 1 & 7)) * kCE<T>;
     } else {
         constexpr int PER = ROWS / kCE<T>;
         outer = at / PER;
