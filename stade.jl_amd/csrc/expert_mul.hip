@@ -490,10 +490,13 @@ struct Tile {
         if constexpr (TAPE && DIRECT) wait_loads<TapeStage<T, BM, NT>::LOADS>();
         else if constexpr (DIRECT) wait_loads<(ST - 2) * (SA::PER + SB::PER)>();
         __syncthreads();
-        straight(t + ST);
+        // (the loads in two parts around the products: all at once before them cost 4 % of a large product)
         read(t + 1, 0);
+        if constexpr (!AREG) sa.direct(buffer(t + ST), (t + ST) * BK);
         __builtin_amdgcn_sched_barrier(0);
         products(3);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!BREG) sb.direct(buffer(t + ST) + BM * 128, (t + ST) * BK);
     }
     if constexpr (DIRECT) wait_loads<0>();   // (of steps past the last: nothing may land after the block's end)
     // A lane has row lane % 32 of each 32 and columns 8 g + 4 (lane / 32) + 0..3 of each 32: each wave
