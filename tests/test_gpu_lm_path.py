@@ -110,3 +110,16 @@ def test_graph_replays_match_eager():
         for k, v in s.results().items():
             assert torch.equal(v, eager[k]), f"replay {rep}: {k}"
         _ = torch.randn(1000, device="cuda").sum().item()
+
+
+def test_example_learns():
+    """The example's model fits its tokens' targets: the loss falls at first and ends below a half of
+    its start (no bound on how far: plain gradient descent)."""
+    import importlib.util
+    from helpers import ROOT
+    spec = importlib.util.spec_from_file_location("lm_step", ROOT / "examples" / "lm_step.py")
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    print("language-model example", flush=True)
+    losses = mod.main(steps=40)
+    assert losses[1] < losses[0] and losses[-1] < 0.5 * losses[0], losses
