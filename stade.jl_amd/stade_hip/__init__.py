@@ -13,6 +13,11 @@ Julia function it stands for (`<k>_b`, `<k>_d`, `<k>_hv` of stade.jl_amd/corpus/
   the scalar shadows, bare if one, a tuple otherwise; the HVP returns (xb, xbd) pairs);
 * work is enqueued on torch's current stream of the tensors' device.
 
+The operators of language models (`embed`, `token_order`, `tape8_*`, `layernorm`, `expert_mul` and
+their adjoints `<k>_b`) have no generated counterpart.  They follow the same rules, with the
+primal function and the adjoint as two calls, matrices whose rows may lie apart, the element
+types float32, bfloat16 and float16, and `add=False` to set shadows instead of accumulating.
+
 This is the product path: there is no CPU fallback.  If the library is missing, or a
 tensor is not on a GPU, the call raises.
 """
