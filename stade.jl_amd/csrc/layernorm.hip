@@ -41,7 +41,8 @@ struct Bwd {
     const uint8_t* q; const uint8_t* qs;
     void* xb; int64_t ldxb;
     const void* g; const float* mu; const float* rs;
-    float* part;      // partial sums: (gb, bb) of a block, 2 * d values; null without gb and bb
+    float* part;      // partial sums: (gb, bb) of a block, 2 * d values; null without gb and bb,
+    float* gb; float* bb;   // or, for a launch of one block, the weights' shadows themselves (each may be null)
     int d; int64_t n; int add;
 };
 
@@ -267,7 +268,7 @@ __global__ __launch_bounds__(NT) void backward_kernel(Bwd p) {
         }
         row = next;
     }
-    if (!p.part) return;
+    if (!p.part && !p.gb && !p.bb) return;
     // the block's rows of partial sums joined, one after the other
     if constexpr (RPB > 1) {
         for (int r = 1; r < RPB; ++r) {
@@ -299,8 +300,24 @@ __global__ __launch_bounds__(NT) void backward_kernel(Bwd p) {
     for (int k = 0; k < NV; ++k) {
         const int col = k * STEP + tr * VE;
         if (col < d) {
-            store_row(part + col, ag[k], d - col);
-            store_row(part + d + col, ab[k], d - col);
+            if (p.part) {
+                store_row(part + col, ag[k], d - col);
+                store_row(part + d + col, ab[k], d - col);
+            } else {
+                float o[VE];
+                if (p.gb) {
+                    load_row(o, p.gb + col, p.add ? d - col : 0);
+#pragma unroll
+                    for (int i = 0; i < VE; ++i) o[i] += ag[k][i];
+                    store_row(p.gb + col, o, d - col);
+                }
+                if (p.bb) {
+                    load_row(o, p.bb + col, p.add ? d - col : 0);
+#pragma unroll
+                    for (int i = 0; i < VE; ++i) o[i] += ab[k][i];
+                    store_row(p.bb + col, o, d - col);
+                }
+            }
         }
     }
 }
@@ -435,6 +452,8 @@ __global__ __launch_bounds__(kSumNT) void weight_sum_kernel(const float* part, i
     }
 }
 
+constexpr int kOneBlock = 4;        // trips of one block in the reverse sweep that spare a second launch
+constexpr int kMostHeldBack = 16384;   // the longest row that the reverse sweep holds in registers
 constexpr int kSumParts = 512;      // blocks of the reverse sweep at most: two a CU
 
 template <class T, class G, int VE, int NV, int WPR, bool TAPE>
@@ -477,7 +496,7 @@ void launch(const Bwd& p, unsigned grid, hipStream_t s) {
     else if (d <= 2048) start<T, G, 8, 1, 4, 512, TAPE>(p, grid, s);
     else if (d <= 4096) start<T, G, 8, 1, 8, 512, TAPE>(p, grid, s);
     else if (d <= 8192) start<T, G, 8, 1, 16, 1024, TAPE>(p, grid, s);
-    else if (d <= 16384) start<T, G, 8, 4, 8, 512, TAPE>(p, grid, s);
+    else if (d <= kMostHeldBack) start<T, G, 8, 4, 8, 512, TAPE>(p, grid, s);
     else backward_long_kernel<T, G, TAPE><<<grid, kLongNT, 0, s>>>(p);
 }
 
@@ -547,14 +566,30 @@ int32_t stade_hip_layernorm_b(int64_t tx, int64_t tg, const void* yb, int64_t ld
     if (!some && (!sums || add)) return STADE_HIP_OK;
     // a block's rows: enough blocks for two a CU, and no more (each leaves a row of partial sums)
     const unsigned rpb = back_rows(i_d);
+    const int64_t trips = (i_n + rpb - 1) / rpb;
+    Bwd p{yb, ldyb, x, ldx, (const uint8_t*)q, qs, xb, ldxb, g, mu, rs, nullptr, nullptr, nullptr, (int)i_d, i_n, add != 0};
+    // Few rows: one block, which leaves gb and bb whole (each of its trips takes about a microsecond, the second
+    // launch and the scratch five).
+    if (some && trips <= kOneBlock && i_d <= kMostHeldBack) {
+        p.gb = gb;
+        p.bb = bb;
+        return with_types(tx, tg, [&](auto t, auto w) -> int32_t {
+            STADE_TIMED("layernorm_b", stream, {
+                if (q) launch<decltype(t), decltype(w), true>(p, 1, stream);
+                else launch<decltype(t), decltype(w), false>(p, 1, stream);
+            });
+            STADE_LAUNCHED("layernorm backward_kernel");
+            return STADE_HIP_OK;
+        });
+    }
     // (long rows: not over 256 MiB of partial sums, but 16 blocks at least)
     const int64_t most = std::min<int64_t>(kSumParts, std::max<int64_t>(16, ((int64_t)1 << 28) / (8 * i_d)));
-    const unsigned grid = (unsigned)std::min<int64_t>((i_n + rpb - 1) / rpb, most);
+    const unsigned grid = (unsigned)std::min<int64_t>(trips, most);
     WsCall call(stream);
     if (!call.ok()) return call.error();
     float* part = nullptr;
     if (sums && some && !(part = (float*)scratch((size_t)grid * 2 * (size_t)i_d * sizeof(float)))) return scratch_error();
-    const Bwd p{yb, ldyb, x, ldx, (const uint8_t*)q, qs, xb, ldxb, g, mu, rs, part, (int)i_d, i_n, add != 0};
+    p.part = part;
     return with_types(tx, tg, [&](auto t, auto w) -> int32_t {
         if (some) {
             STADE_TIMED("layernorm_b", stream, {
