@@ -300,11 +300,10 @@ struct TapeStage {
     }
     __device__ __forceinline__ static void store(const Held& v, int i, char* lds) {
         typedef T vec __attribute__((ext_vector_type(CE)));
-        // q + 128 as an unsigned byte, times the unit, less 128 units: exact
-        const float u = tape8::unit(v.s), low = -128.f * u;
+        const float u = tape8::unit(v.s);
         vec x;
 #pragma unroll
-        for (int j = 0; j < CE; ++j) x[j] = (T)fmaf((float)(((v.q[j >> 2] ^ 0x80808080u) >> (8 * (j & 3))) & 0xffu), u, low);
+        for (int j = 0; j < CE; ++j) x[j] = (T)tape8::value(v.q[j >> 2] ^ 0x80808080u, j & 3, u);
         *reinterpret_cast<v4u*>(lds + (i * NT + threadIdx.x) * 16) = __builtin_bit_cast(v4u, x);
     }
 };

@@ -13,10 +13,10 @@
 // atomics, the same bits at every call.  Sums are fp32 throughout.
 // Rows longer than the registers hold are read again for each of the sums.
 //
-// Measured on an MI355X (16384 x 4096 bf16, copy 4.7 TB/s): forward 56 us (4.8 TB/s), with the tape 87 (3.9);
-// reverse 86 us (4.7 TB/s), from the tape 100 (3.4: there the vector instructions count, some 25 a value
-// with the tape's).  In the reverse sweep the next row, its statistics and the weights are in registers before the
-// row's sums are waited for: without them 152 us.
+// Measured on an MI355X (16384 x 4096 bf16, copy 4.7 TB/s): forward 56 us (4.8 TB/s), with the tape 86 (4.0);
+// reverse 86 us (4.7 TB/s), from the tape 84 (4.0; the bytes turn into values by one conversion, one subtraction
+// and one product each).  In the reverse sweep the next row, its statistics and the weights are in registers
+// before the row's sums are waited for: without them 152 us.
 #include "tape8.hpp"
 
 #include <algorithm>
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(block_of<WPR>()) void forward_kernel(Fwd p) {
 #pragma unroll
             for (int i = 0; i < VE; ++i) {
                 const float c = k * STEP + tr * VE + (W ? 0 : i) < d ? v[k][i] - mu : 0.f;
-                s[0] += c * c;
+                s[0] = fmaf(c, c, s[0]);
             }
         row_sum<WPR, 1>(s, lds, turn);
         const float rs = 1.0f / sqrtf(s[0] / (float)d + p.eps);
@@ -153,8 +153,7 @@ __device__ __forceinline__ void load_input(float (&v)[VE], const Bwd& p, int64_t
 template <class T, int VE, bool TAPE, bool W>
 struct Raw {
     typedef T vec __attribute__((ext_vector_type(VE)));
-    typedef uint8_t bytes __attribute__((ext_vector_type(VE)));
-    std::conditional_t<TAPE, bytes, vec> x;
+    std::conditional_t<TAPE, tape8::Word<VE>, vec> x;
     vec yb;
     uint8_t s;
 
@@ -163,7 +162,7 @@ struct Raw {
         if constexpr (TAPE) {
             const int64_t ng = tape8::groups(p.d);
             if (left > 0) {   // (the tape's rows are whole groups)
-                x = *reinterpret_cast<const bytes*>(p.q + row * ng * tape8::kGroup + col);
+                x = *reinterpret_cast<const tape8::Word<VE>*>(p.q + row * ng * tape8::kGroup + col);
                 s = p.qs[row * ng + col / tape8::kGroup];
             }
         } else {
@@ -181,10 +180,7 @@ struct Raw {
     }
     __device__ __forceinline__ void values(float (&h)[VE], float (&a)[VE]) const {
         if constexpr (TAPE) {
-            // q + 128 as an unsigned byte, times the unit, less 128 units: exact
-            const float u = tape8::unit(s), low = -128.f * u;
-#pragma unroll
-            for (int i = 0; i < VE; ++i) h[i] = fmaf((float)(uint8_t)(x[i] ^ 0x80), u, low);
+            tape8::values(h, x, tape8::unit(s));
         } else {
 #pragma unroll
             for (int i = 0; i < VE; ++i) h[i] = (float)x[i];
@@ -345,7 +341,7 @@ __global__ __launch_bounds__(kLongNT) void forward_long_kernel(Fwd p) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float c = col + i < d ? v[i] - mu : 0.f;
-                s[0] += c * c;
+                s[0] = fmaf(c, c, s[0]);
             }
         }
         row_sum<16, 1>(s, lds, turn);

@@ -14,6 +14,8 @@
 
 #include "rows.hpp"
 
+#include <type_traits>
+
 namespace stade {
 namespace tape8 {
 
@@ -58,22 +60,22 @@ __device__ __forceinline__ uint32_t group_max(uint32_t v) {
     return v;
 }
 
-// A value as its byte.  Adding 1.5 * 2^23 rounds a small fp32 value to a whole number, to
-// nearest even, and leaves it in the low bits.  (A value that is not finite only meets inv = 0;
-// the median of NaN and two limits is one of the limits, and q is 0 there.)
-__device__ __forceinline__ uint32_t quantise1(float x, const Scale& s) {
-    const float v = __builtin_amdgcn_fmed3f(x * s.inv, -s.lim, s.lim);
-    return s.byte == 255u ? 0u : __float_as_uint(v + 12582912.f) & 0xffu;
-}
+// The whole numbers of N values as bytes, 4 a word.  Adding 1.5 * 2^23 rounds a small fp32 value to a
+// whole number, to nearest even, and leaves it in the low bits; v_perm_b32 takes the low bytes together.
+// (`keep`: nothing of a group that is not finite.)
 template <int N>
 __device__ __forceinline__ void put(uint8_t* q, const float (&x)[N], const Scale& s) {
     uint32_t w[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = quantise1(x[i], s);
-    if constexpr (N == 8)
-        *reinterpret_cast<uint2*>(q) = make_uint2(w[0] | w[1] << 8 | w[2] << 16 | w[3] << 24, w[4] | w[5] << 8 | w[6] << 16 | w[7] << 24);
-    else
-        *reinterpret_cast<uint16_t*>(q) = (uint16_t)(w[0] | w[1] << 8);
+    for (int i = 0; i < N; ++i) w[i] = __float_as_uint(__builtin_amdgcn_fmed3f(x[i] * s.inv, -s.lim, s.lim) + 12582912.f);
+    const uint32_t keep = s.byte == 255u ? 0u : ~0u;
+    const auto two = [](uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x0c0c0400u); };
+    if constexpr (N == 8) {
+        const auto four = [&](int i) { return __builtin_amdgcn_perm(two(w[i + 2], w[i + 3]), two(w[i], w[i + 1]), 0x05040100u) & keep; };
+        *reinterpret_cast<uint2*>(q) = make_uint2(four(0), four(4));
+    } else {
+        *reinterpret_cast<uint16_t*>(q) = (uint16_t)(two(w[0], w[1]) & keep);
+    }
 }
 
 // a lane's part of a group written, from the registers that hold it: x's values at `col` of a row with
@@ -93,20 +95,27 @@ __device__ __forceinline__ void store_part(uint8_t* q, uint8_t* qs, const float 
 // 2^e of a scale byte; infinite for 255, so that its q = 0 reads as NaN
 __device__ __forceinline__ float unit(uint32_t byte) { return __uint_as_float(byte << 23); }
 
+// N bytes as they lie in memory, and their values: q + 128 as an unsigned byte, less 128, times the unit
+// (both exact; 128 units may be infinite, so the unit comes last)
+template <int N> using Word = std::conditional_t<N == 8, uint2, uint16_t>;
+__device__ __forceinline__ float value(uint32_t biased, int byte, float u) {
+    return ((float)((biased >> (8 * byte)) & 0xffu) - 128.f) * u;
+}
+template <int N>
+__device__ __forceinline__ void values(float (&x)[N], Word<N> q, float u) {
+    if constexpr (N == 8) {
+        const uint32_t w[2] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = value(w[i >> 2], i & 3, u);
+    } else {
+        const uint32_t w = (uint32_t)q ^ 0x8080u;
+        x[0] = value(w, 0, u);
+        x[1] = value(w, 1, u);
+    }
+}
 template <int N>
 __device__ __forceinline__ void values(float (&x)[N], const uint8_t* q, float u) {
-    if constexpr (N == 8) {
-        const uint2 v = *reinterpret_cast<const uint2*>(q);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] = (float)(int)(int8_t)(v.x >> (8 * i)) * u;
-            x[4 + i] = (float)(int)(int8_t)(v.y >> (8 * i)) * u;
-        }
-    } else {
-        const uint32_t v = *reinterpret_cast<const uint16_t*>(q);
-        x[0] = (float)(int)(int8_t)v * u;
-        x[1] = (float)(int)(int8_t)(v >> 8) * u;
-    }
+    values(x, *reinterpret_cast<const Word<N>*>(q), u);
 }
 
 }  // namespace tape8

@@ -136,6 +136,20 @@ def test_values_that_are_not_finite_stay_in_their_rows(dt):
     assert torch.isnan(y[69]).all() and not torch.isfinite(y[73]).any()
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16], ids=IDS.get)
+def test_tape_of_the_largest_values(dt):
+    """Scales at the top of the exponent range, where 128 of their units are infinite."""
+    import stade_hip
+    t, e, i, o, start, x, _, yb, _ = _case(([70, 20], 0, 64, 72), dt, seed=3)
+    x, yb = (x.double() * 2.0 ** 124).to(dt), (yb.double() * 2.0 ** -120).to(dt)
+    tape = new_tape(i, t)
+    stade_hip.tape8_store(x.cuda(), *tape, i, t)
+    wb = torch.empty(e, i, o, device="cuda")
+    stade_hip.expert_mul_b(yb.cuda(), None, None, None, wb, start.cuda(), i, o, t, e, add=False, tape=tape)
+    want, scale = _wb(tape_values(x.double()), yb.double(), start, e)
+    within("wb", wb, want, U * 78 * scale, torch.float32)
+
+
 def test_offsets_that_are_wrong_raise_the_flag():
     import stade_hip
     t, e, i, o = 64, 3, 32, 32

@@ -146,6 +146,26 @@ def test_parts_left_out():
     assert torch.equal(same, xb)
 
 
+@pytest.mark.parametrize("d", [100, 640])
+def test_tape_of_the_largest_values(d):
+    """Scales at the top of the exponent range, where 128 of their units are infinite."""
+    import stade_hip
+    n = 5
+    x, g, _, yb = _inputs(n, d, torch.float32, torch.float32, seed=4)
+    x = (x.double().clamp(-3, 3) * 2.0 ** 124).float()
+    mu, rs = torch.zeros(n), torch.full((n,), 2.0 ** -124)
+    t = new_tape(d, n)
+    stade_hip.tape8_store(x.cuda(), *t, d, n)
+    xb = torch.empty(n, d, device="cuda")
+    gb, bb = torch.empty(d, device="cuda"), torch.empty(d, device="cuda")
+    stade_hip.layernorm_b(yb.cuda(), None, xb, g.cuda(), gb, bb, mu.cuda(), rs.cuda(), d, n, add=False, tape=t)
+    # (rs scales xb into subnormals, which are rounded to their own least)
+    wxb, wgb, wbb, sxb, sgb, sbb = _backward(yb.double(), tape_values(x.double()), g.double(), mu.double()[:, None], rs.double()[:, None])
+    within("gb", gb, wgb, sgb, torch.float32)
+    within("bb", bb, wbb, sbb, torch.float32)
+    within("xb", xb, wxb, sxb + 2.0 ** -126, torch.float32)
+
+
 def test_no_rows():
     import stade_hip
     e, d = torch.empty(0, 6, device="cuda"), 6
