@@ -586,6 +586,9 @@ struct Tile {
     }
 };
 
+// buffers of a tile of 64 x 64
+constexpr int small_buffers(bool tape, bool direct) { return direct && !tape ? 4 : 2; }
+
 // the piece that holds tile `piece` of the pieces of BM rows, and its first row in it
 template <int FORM, int BM>
 __device__ __forceinline__ Rows piece_rows(const Mul& p, const Pieces<BM>* all, int64_t piece, int& m0) {
@@ -599,21 +602,39 @@ __device__ __forceinline__ Rows piece_rows(const Mul& p, const Pieces<BM>* all, 
     }
 }
 
-// one size of tile
-template <class T, class TC, int FORM, bool TAPE, bool DIRECT, int BM, int BN, int WM, int WN, int ST>
-__global__ __launch_bounds__(64 * WM * WN) void product_kernel(Mul p) {
-    using One = Tile<T, TC, FORM, TAPE, DIRECT, BM, BN, WM, WN, ST>;
-    __shared__ char lds[One::LDS];
+// (where results are added to what is there, rows of no expert and experts without rows change nothing: 24 rows that go to
+// 2 of 8 experts, 2048 x 4096, bf16: wb in fp32 36 us, 96 with the others read and written)
+__device__ __forceinline__ bool nothing(const Mul& p, const Rows& r) { return p.add && (r.e < 0 || r.rows == 0); }
+
+// one size of tile: block `block` of the launch
+template <class One, int FORM, int BM, int BN>
+__device__ __forceinline__ void product(const Mul& p, unsigned block, char* lds) {
     const Pieces<BM> all(p.start, FORM == WB ? 0 : p.ne, p.t, FORM == WB ? nullptr : p.flag);
     const int64_t pieces = FORM == WB ? p.pieces : all.count();
     int64_t piece;
     int tn, m0;
     const int64_t all_items = items<FORM>(p, pieces);
-    const int slice = (int)(blockIdx.x / all_items);
-    if (slice >= p.split || !item_place<FORM>(p, blockIdx.x % all_items, pieces, piece, tn)) return;
+    const int slice = (int)(block / all_items);
+    if (slice >= p.split || !item_place<FORM>(p, block % all_items, pieces, piece, tn)) return;
     const Rows r = piece_rows<FORM, BM>(p, &all, piece, m0);
-    if (r.e < 0 && p.add) return;
+    if (nothing(p, r)) return;
     One::run(p, r, m0, tn * BN, lds, slice);
+}
+template <class T, class TC, int FORM, bool TAPE, bool DIRECT, int BM, int BN, int WM, int WN, int ST>
+__global__ __launch_bounds__(64 * WM * WN) void product_kernel(Mul p) {
+    using One = Tile<T, TC, FORM, TAPE, DIRECT, BM, BN, WM, WN, ST>;
+    __shared__ char lds[One::LDS];
+    product<One, FORM, BM, BN>(p, blockIdx.x, lds);
+}
+
+// xb and wb in one launch, where both take tiles of 64 x 64: the first blocks, a multiple of 8, are xb's
+template <class T, class TC, bool TAPE, bool DIRECT>
+__global__ __launch_bounds__(256) void shadows_kernel(Mul px, Mul pw, unsigned first) {
+    using X = Tile<T, T, XB, false, DIRECT, 64, 64, 2, 2, small_buffers(false, DIRECT)>;
+    using W = Tile<T, TC, WB, TAPE, DIRECT, 64, 64, 2, 2, small_buffers(TAPE, DIRECT)>;
+    __shared__ char lds[X::LDS > W::LDS ? X::LDS : W::LDS];
+    if (blockIdx.x < first) product<X, XB, 64, 64>(px, blockIdx.x, lds);
+    else product<W, WB, 64, 64>(pw, blockIdx.x - first, lds);
 }
 
 // Large tiles, 256 x 256, for as many whole rounds as the CUs make of them (one block a CU); the rest,
@@ -637,7 +658,7 @@ __global__ __launch_bounds__(512) void mixed_kernel(Mul p) {
     }
     if (!item_place<FORM>(p, item, pieces, piece, tn)) return;
     const Rows r = piece_rows<FORM, 256>(p, &all, piece, m0);
-    if (r.e < 0 && p.add) return;
+    if (nothing(p, r)) return;
     if (quarter < 0) Large::run(p, r, m0, tn * 256, lds);
     else Quarter::run(p, r, m0 + (quarter >> 1) * 128, tn * 256 + (quarter & 1) * 128, lds);
 }
@@ -667,15 +688,23 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, int slices
     }
 }
 
-template <class T, class TC, int FORM, bool TAPE, bool DIRECT, int BM, int BN, int WM, int WN, int ST = 2>
-int32_t launch(Mul p, hipStream_t stream, const char* name) {
+// the tiles of p, and of its launch; or an error
+template <int FORM, int BM, int BN, int NT>
+int32_t count_tiles(Mul& p, int64_t& tiles, const char* name) {
     p.tiles_n = (p.n + BN - 1) / BN;
     p.pieces = FORM == WB ? (int64_t)p.ne * ((p.m + BM - 1) / BM) : (p.t + BM - 1) / BM + p.ne + 2;
-    const int64_t tiles = FORM == WB ? ((p.m + BM - 1) / BM * p.tiles_n + 7) / 8 * 8 * p.ne : (p.pieces * p.tiles_n + 7) / 8 * 8;
+    tiles = FORM == WB ? ((p.m + BM - 1) / BM * p.tiles_n + 7) / 8 * 8 * p.ne : (p.pieces * p.tiles_n + 7) / 8 * 8;
     // (a launch has less than 2^32 threads)
-    if ((tiles + 4 * (int64_t)p.cus) * p.split >= (1ll << 32) / (64 * WM * WN)) return set_error(STADE_HIP_ERANGE, "%s: too many tiles for a launch", name);
+    if ((tiles + 4 * (int64_t)p.cus) * p.split >= (1ll << 32) / NT) return set_error(STADE_HIP_ERANGE, "%s: too many tiles for a launch", name);
+    return 0;
+}
+
+template <class T, class TC, int FORM, bool TAPE, bool DIRECT, int BM, int BN, int WM, int WN, int ST = 2>
+int32_t launch(Mul p, hipStream_t stream, const char* name) {
+    if (BM == 256) p.split = 1;
+    int64_t tiles;
+    if (int32_t rc = count_tiles<FORM, BM, BN, 64 * WM * WN>(p, tiles, name)) return rc;
     if constexpr (BM == 256) {
-        p.split = 1;
         const unsigned blocks = (unsigned)(tiles + 3 * ((p.cus / 2 + 7) / 8 * 8));
         STADE_TIMED(name, stream, mixed_kernel<T, TC, FORM, TAPE, DIRECT><<<blocks, 512, 0, stream>>>(p));
     } else {
@@ -690,8 +719,16 @@ inline bool whole(const void* p, int64_t ld, int64_t d, int64_t tile, size_t siz
     return (uintptr_t)p % 16 == 0 && ld * size % 16 == 0 && d * size % 16 == 0 && tile * ld * (int64_t)size < (1ll << 31);
 }
 
-template <class T, class TC, int FORM, bool TAPE>
-int32_t run(const Mul& p, hipStream_t stream, const char* name) {
+// How a product is done: by tiles of 64 x 64 (in `slices` of k), of 64 x 128 with three steps in flight, of 128 x 128, or of
+// 256 x 256; `direct`: by straight loads
+enum Size { SMALL, FLAT, MIDDLE, LARGE };
+struct Plan {
+    bool direct;
+    Size size;
+    int slices;
+};
+template <class T, int FORM, bool TAPE>
+Plan plan(const Mul& p) {
     const bool direct = (TAPE || whole(p.a, p.lda, FORM == WB ? p.m : p.k, 256, sizeof(T))) &&
                         whole(p.b, p.ldb, FORM == XB ? p.k : p.n, 256, sizeof(T));
     // the tiles of 256 x 256 that the rows will make, half a tile more an expert
@@ -700,58 +737,81 @@ int32_t run(const Mul& p, hipStream_t stream, const char* name) {
     // (a step takes a microsecond; the launch that adds the slices up takes five).  64 rows, 4 experts, 1672 x 2484, bf16: y
     // 43.4 -> 31.3 us, xb 45.7 -> 25.8; 3584 rows, 2 experts, 128 x 295: wb 37 -> 20; in fp32 137 rows, 4 experts, 1856 x 256: y
     // 71 -> 18.  Saving 8 steps: 1000 rows, 7 experts, 500 x 700, fp32: 18.7 -> 23.7.
-    {
-        const int64_t small = std::max<int64_t>(1, (FORM == WB ? (int64_t)p.ne * ((p.m + 63) / 64) : p.t / 64 + std::min<int64_t>(p.ne, p.t)) * ((p.n + 63) / 64));
-        const int64_t steps = (FORM == WB ? p.t / p.ne : p.k) / kBK<T>, slices = std::min<int64_t>(std::min<int64_t>(2 * p.cus / small, steps / 4), 32);
-        if (small < p.cus && slices >= 2 && steps - steps / slices >= 12) {
-            const int64_t rows = FORM == WB ? (int64_t)p.ne * p.m : p.t;
-            Mul q = p;
-            q.split = (int)slices;
-            q.add = 0;
-            q.ldc = p.n;
-            if (!(q.c = scratch((size_t)slices * rows * p.n * sizeof(float)))) return scratch_error();
-            const int32_t rc = direct ? launch<T, float, FORM, TAPE, true, 64, 64, 2, 2, TAPE ? 2 : 4>(q, stream, name)
-                                      : launch<T, float, FORM, TAPE, false, 64, 64, 2, 2>(q, stream, name);
-            if (rc) return rc;
-            const unsigned grid = (unsigned)std::min<int64_t>((rows * ((p.n + 7) / 8) + 255) / 256, 1 << 14);
-            STADE_TIMED("expert_mul_join", stream,
-                        join_kernel<TC><<<grid, 256, 0, stream>>>((const float*)q.c, q.split, (TC*)p.c, FORM == WB ? p.n : p.ldc, rows, p.n, p.add));
-            STADE_LAUNCHED("expert_mul join_kernel");
-            return STADE_HIP_OK;
-        }
-    }
+    const int64_t small = std::max<int64_t>(1, (FORM == WB ? (int64_t)p.ne * ((p.m + 63) / 64) : p.t / 64 + std::min<int64_t>(p.ne, p.t)) * ((p.n + 63) / 64));
+    const int64_t steps = (FORM == WB ? p.t / p.ne : p.k) / kBK<T>, slices = std::min<int64_t>(std::min<int64_t>(2 * p.cus / small, steps / 4), 32);
+    if (small < p.cus && slices >= 2 && steps - steps / slices >= 12) return Plan{direct, SMALL, (int)slices};
     // Few rows an expert (y and xb: at most 64): bound by reading w, so small tiles, many blocks and three or four
     // steps in flight.  24 rows, 8 experts, 2048 x 4096, bf16: y 26.6 us (128 x 128 tiles 28.7, quarters 27.4), xb 24.8
     // (45, 37).
     const bool few = FORM != WB && p.t <= 64 * (int64_t)p.ne;
-    if constexpr (!TAPE) {
-        if (direct && few) {
-            if constexpr (FORM == Y) return launch<T, TC, FORM, TAPE, true, 64, 128, 1, 4, 3>(p, stream, name);
-            else return launch<T, TC, FORM, TAPE, true, 64, 64, 2, 2, 4>(p, stream, name);
-        }
+    if (direct && few) return Plan{direct, FORM == Y ? FLAT : SMALL, 1};
+    // fp32 is bound by its matrix instructions: the tile that fills the CUs (1000 rows, 7 experts, 500 x 700: 64 x 64
+    // 18 us, 128 x 128 42; 8192 rows, 8 experts, 2048 x 1024: y 378 and 408, wb 302 and 272)
+    if (sizeof(T) == 4) return Plan{direct, est < 2 * p.cus ? SMALL : MIDDLE, 1};
+    // Less than a round of large tiles, more than one of quarters: 128 x 128 tiles of four waves, two
+    // blocks a CU.  4096 rows, 8 experts, 1024 x 1024: 22.8 us, with quarters 29.0; 1024 rows, 4 experts,
+    // 2048 x 2048, one round of quarters: 25.4 us, with these 28.4.
+    if (direct) return Plan{direct, est < p.cus && 4 * est > p.cus ? MIDDLE : LARGE, 1};
+    // Through registers: 1000 rows, 7 experts, 500 x 700 18 us, with large tiles and quarters 20.7; 24 rows, 8 experts,
+    // 2044 x 4100 55 us (113); 8000 rows 377 us, with large tiles 245.
+    return Plan{direct, few || 4 * est <= p.cus ? SMALL : LARGE, 1};
+}
+
+template <class T, class TC, int FORM, bool TAPE>
+int32_t run(const Mul& p, hipStream_t stream, const char* name) {
+    const Plan how = plan<T, FORM, TAPE>(p);
+    if (how.slices > 1) {
+        const int64_t rows = FORM == WB ? (int64_t)p.ne * p.m : p.t;
+        Mul q = p;
+        q.split = how.slices;
+        q.add = 0;
+        q.ldc = p.n;
+        if (!(q.c = scratch((size_t)q.split * rows * p.n * sizeof(float)))) return scratch_error();
+        const int32_t rc = how.direct ? launch<T, float, FORM, TAPE, true, 64, 64, 2, 2, small_buffers(TAPE, true)>(q, stream, name)
+                                      : launch<T, float, FORM, TAPE, false, 64, 64, 2, 2>(q, stream, name);
+        if (rc) return rc;
+        const unsigned grid = (unsigned)std::min<int64_t>((rows * ((p.n + 7) / 8) + 255) / 256, 1 << 14);
+        STADE_TIMED("expert_mul_join", stream,
+                    join_kernel<TC><<<grid, 256, 0, stream>>>((const float*)q.c, q.split, (TC*)p.c, FORM == WB ? p.n : p.ldc, rows, p.n, p.add));
+        STADE_LAUNCHED("expert_mul join_kernel");
+        return STADE_HIP_OK;
     }
+    if constexpr (FORM == Y)
+        if (how.size == FLAT) return launch<T, TC, FORM, TAPE, true, 64, 128, 1, 4, 3>(p, stream, name);
+    if constexpr (sizeof(T) == 4 || FORM != WB)   // (wb of 16-bit types takes no small tiles by straight loads, but in slices)
+        if (how.size == SMALL && how.direct) return launch<T, TC, FORM, TAPE, true, 64, 64, 2, 2, small_buffers(TAPE, true)>(p, stream, name);
+    if (how.size == SMALL) return launch<T, TC, FORM, TAPE, false, 64, 64, 2, 2>(p, stream, name);
     if constexpr (sizeof(T) == 4) {
-        // fp32 is bound by its matrix instructions: the tile that fills the CUs (1000 rows, 7 experts, 500 x 700: 64 x 64
-        // 18 us, 128 x 128 42; 8192 rows, 8 experts, 2048 x 1024: y 378 and 408, wb 302 and 272)
-        if (direct) {
-            if (est < 2 * p.cus) return launch<T, TC, FORM, TAPE, true, 64, 64, 2, 2, TAPE ? 2 : 4>(p, stream, name);
-            return launch<T, TC, FORM, TAPE, true, 128, 128, 2, 2>(p, stream, name);
-        }
-        if (est < 2 * p.cus) return launch<T, TC, FORM, TAPE, false, 64, 64, 2, 2>(p, stream, name);
+        if (how.direct) return launch<T, TC, FORM, TAPE, true, 128, 128, 2, 2>(p, stream, name);
         return launch<T, TC, FORM, TAPE, false, 128, 128, 2, 2>(p, stream, name);
     } else {
-        if (direct) {
-            // Less than a round of large tiles, more than one of quarters: 128 x 128 tiles of four waves, two
-            // blocks a CU.  4096 rows, 8 experts, 1024 x 1024: 22.8 us, with quarters 29.0; 1024 rows, 4 experts,
-            // 2048 x 2048, one round of quarters: 25.4 us, with these 28.4.
-            if (est < p.cus && 4 * est > p.cus) return launch<T, TC, FORM, TAPE, true, 128, 128, 2, 2>(p, stream, name);
-            return launch<T, TC, FORM, TAPE, true, 256, 256, 2, 4>(p, stream, name);
-        }
-        // Through registers: 1000 rows, 7 experts, 500 x 700 18 us, with large tiles and quarters 20.7; 24 rows, 8 experts,
-        // 2044 x 4100 55 us (113); 8000 rows 377 us, with large tiles 245.
-        if (few || 4 * est <= p.cus) return launch<T, TC, FORM, TAPE, false, 64, 64, 2, 2>(p, stream, name);
+        if (how.size == MIDDLE) return launch<T, TC, FORM, TAPE, true, 128, 128, 2, 2>(p, stream, name);
+        if (how.direct) return launch<T, TC, FORM, TAPE, true, 256, 256, 2, 4>(p, stream, name);
         return launch<T, TC, FORM, TAPE, false, 256, 256, 2, 4>(p, stream, name);
     }
+}
+
+// xb and wb.  One launch where both take small tiles: 1000 rows, 7 experts, 500 x 700, f16: 15.4 us, two launches
+// 23.6; 4000 rows, 6 experts, 215 x 331, bf16: 16.9 and 24.5; fp32, 504 x 704: 28.5 and 38.8.
+template <class T, class TC, bool TAPE>
+int32_t run_both(Mul px, Mul pw, hipStream_t stream) {
+    const Plan x = plan<T, XB, false>(px), w = plan<T, WB, TAPE>(pw);
+    if (x.size == SMALL && w.size == SMALL && x.slices == 1 && w.slices == 1 && x.direct == w.direct) {
+        int64_t first, more;
+        if (int32_t rc = count_tiles<XB, 64, 64, 512>(px, first, "expert_mul_b")) return rc;
+        if (int32_t rc = count_tiles<WB, 64, 64, 512>(pw, more, "expert_mul_b")) return rc;
+        const auto go = [&](auto direct) -> int32_t {
+            STADE_TIMED("expert_mul_b", stream,
+                        shadows_kernel<T, TC, TAPE, decltype(direct)::value><<<(unsigned)(first + more), 256, 0, stream>>>(px, pw, (unsigned)first));
+            STADE_LAUNCHED("expert_mul shadows_kernel");
+            return STADE_HIP_OK;
+        };
+        if constexpr (sizeof(T) == 4)   // (as in run)
+            if (x.direct) return go(std::true_type{});
+        return go(std::false_type{});
+    }
+    if (int32_t rc = run<T, T, XB, false>(px, stream, "expert_mul_xb")) return rc;
+    return run<T, TC, WB, TAPE>(pw, stream, "expert_mul_wb");
 }
 
 int32_t check(const char* fn, int64_t tx, const int64_t* start, int64_t i_in, int64_t i_out, int64_t i_t, int64_t i_e) {
@@ -818,21 +878,20 @@ int32_t stade_hip_expert_mul_b(int64_t tx, int64_t twb, const void* yb, int64_t 
     p.start = start; p.ne = (int)i_e; p.t = i_t; p.add = add != 0; p.flag = error_flag(call.ws);
     p.cus = cu_count();
     p.split = 1;
+    Mul px = p, pw = p;
+    px.a = yb; px.lda = ldyb; px.b = w; px.ldb = i_out; px.c = xb; px.ldc = ldxb; px.n = (int)i_in; px.k = (int)i_out;
+    pw.a = x; pw.lda = ldx; pw.q = (const uint8_t*)q; pw.qs = qs; pw.b = yb; pw.ldb = ldyb; pw.c = wb; pw.m = (int)i_in; pw.n = (int)i_out;
+    const bool do_x = xb && i_t > 0, do_w = wb && i_out > 0 && i_e > 0;
     return with_type(tx, [&](auto t) -> int32_t {
         using T = decltype(t);
-        if (xb && i_t > 0) {
-            p.a = yb; p.lda = ldyb; p.b = w; p.ldb = i_out; p.c = xb; p.ldc = ldxb; p.n = (int)i_in; p.k = (int)i_out;
-            if (int32_t rc = run<T, T, XB, false>(p, stream, "expert_mul_xb")) return rc;
-        }
-        if (wb && i_out > 0 && i_e > 0) {
-            p.a = x; p.lda = ldx; p.q = (const uint8_t*)q; p.qs = qs; p.b = yb; p.ldb = ldyb; p.c = wb; p.m = (int)i_in; p.n = (int)i_out;
-            const auto go = [&](auto tape) -> int32_t {
-                if (twb == STADE_HIP_F32) return run<T, float, WB, decltype(tape)::value>(p, stream, "expert_mul_wb");
-                return run<T, T, WB, decltype(tape)::value>(p, stream, "expert_mul_wb");
-            };
-            return q ? go(std::true_type{}) : go(std::false_type{});
-        }
-        return STADE_HIP_OK;
+        if (!do_w) return do_x ? run<T, T, XB, false>(px, stream, "expert_mul_xb") : STADE_HIP_OK;
+        const auto go = [&](auto tw, auto tape) -> int32_t {
+            using TW = decltype(tw);
+            constexpr bool TAPE = decltype(tape)::value;
+            return do_x ? run_both<T, TW, TAPE>(px, pw, stream) : run<T, TW, WB, TAPE>(pw, stream, "expert_mul_wb");
+        };
+        if (twb == STADE_HIP_F32) return q ? go(float{}, std::true_type{}) : go(float{}, std::false_type{});
+        return q ? go(t, std::true_type{}) : go(t, std::false_type{});
     });
 }
 
