@@ -122,10 +122,10 @@ struct Pieces {
 // expert e's rows
 __device__ __forceinline__ Rows expert_rows(const int64_t* start, int ne, int64_t t, int e, int32_t* flag) {
     const int lane = threadIdx.x & 63;
-    int64_t lo = 0, hi = 0;
+    int64_t lo = 0, hi = 0, raw = 0;
     for (int base = 0; base <= e + 1; base += 64) {
         const int i = base + lane;
-        const int64_t raw = i <= e + 1 ? start[i] : 0;
+        raw = i <= e + 1 ? start[i] : 0;
         if (i <= e + 1 && (raw < 0 || raw > t) && flag) *flag = kErrIndex;
         int64_t a = i <= e ? min(max(raw, (int64_t)0), t) : 0, b = i <= e + 1 ? min(max(raw, (int64_t)0), t) : 0;
 #pragma unroll
@@ -136,6 +136,7 @@ __device__ __forceinline__ Rows expert_rows(const int64_t* start, int ne, int64_
         lo = max(lo, a);
         hi = max(hi, b);
     }
+    if (lane == ((e + 1) & 63) && raw < lo && flag) *flag = kErrIndex;
     return Rows{e, lo, (int)(hi - lo)};
 }
 

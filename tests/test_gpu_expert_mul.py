@@ -166,6 +166,20 @@ def test_offsets_that_are_wrong_raise_the_flag():
     assert stade_hip.device_error() == 0
 
 
+def test_decreasing_offsets_raise_the_flag_of_wb_alone():
+    import stade_hip
+    g = gen(2)
+    for e in (3, 70):
+        x, yb, wb = cuda(normal(g, 64, 32)), cuda(normal(g, 64, 32)), torch.empty(e, 32, 32, device="cuda")
+        for at in (2, e):
+            print(f"expert_mul_b wb alone, experts {e}, decreasing at {at}", flush=True)
+            start = torch.full((e + 1,), 40)
+            start[0], start[at] = 0, 20
+            with pytest.raises(stade_hip.StadeHipBoundsError):
+                stade_hip.expert_mul_b(yb, x, None, None, wb, start.cuda(), 32, 32, 64, e, add=False, check=True)
+    assert stade_hip.device_error() == 0
+
+
 def test_nothing():
     import stade_hip
     start = torch.zeros(4, dtype=torch.int64, device="cuda")
