@@ -29,8 +29,11 @@
  *   - Calls on one device share a library workspace (reduction partials, device scalars and
  *     scratch).  Calls are serialised per device: a host thread holds the device's lock while
  *     it enqueues, and a call on a stream other than the previous call's first waits
- *     (hipStreamWaitEvent) for the event that call recorded at its end, so calls on different
- *     streams run one after the other instead of racing.
+ *     (hipStreamWaitEvent) for an event behind that call, so calls on different streams run one
+ *     after the other instead of racing, for the workspace or for the caller's arrays.  A call
+ *     records that event at its end; while a device's calls have all come on the default
+ *     stream they record none, and the first call on another stream waits for what the default stream
+ *     has been given by then.
  *   - Graph capture: a call on a capturing stream takes no dependency outside the capture, and
  *     the workspace does not grow under capture (STADE_HIP_ESTATE): make one eager call of the
  *     largest size first.  Replays are not ordered against eager calls on other streams (the

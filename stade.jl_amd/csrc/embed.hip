@@ -739,8 +739,8 @@ int32_t stade_hip_embed(int64_t ty, int64_t tw, void* y, int64_t ldy, const void
     if (int32_t rc = check_ld(fn, "ldw", ldw, i_d)) return rc;
     if (i_d == 0 || i_t == 0) return STADE_HIP_OK;
     if (!y || !tok || (i_v > 0 && !w)) return bad(fn, "null pointer");
-    Workspace* ws = workspace();
-    if (!ws) return STADE_HIP_ENOMEM;
+    WsCall call(stream);
+    if (!call.ok()) return call.error();
     const int64_t jobs = i_t * ((i_d + kCols - 1) / kCols);
     const unsigned grid = (unsigned)std::min<int64_t>((jobs + NT / 64 - 1) / (NT / 64), 1 << 16);
     return with_type(ty, [&](auto a) -> int32_t {
@@ -749,7 +749,7 @@ int32_t stade_hip_embed(int64_t ty, int64_t tw, void* y, int64_t ldy, const void
             using TW = decltype(b);
             STADE_TIMED("embed", stream,
                         embed_kernel<TY, TW><<<grid, NT, 0, stream>>>((TY*)y, ldy, (const TW*)w, ldw, tok, (float)s, (int)i_d, i_v, i_t,
-                                                                      error_flag(ws)));
+                                                                      error_flag(call.ws)));
             STADE_LAUNCHED("embed embed_kernel");
             return STADE_HIP_OK;
         });
@@ -769,15 +769,15 @@ int32_t stade_hip_embed_b(int64_t ty, int64_t tw, const void* yb, int64_t ldyb, 
     if (i_d == 0 || (i_v == 0 && i_t == 0)) return STADE_HIP_OK;
     if ((i_v > 0 && !wb) || (i_t > 0 && (!yb || !tok))) return bad(fn, "null pointer");
     const int64_t row_bytes = ldwb * type_size(tw), width = i_d * type_size(tw);
+    if (i_t == 0 && add) return STADE_HIP_OK;
+    WsCall call(stream);
+    if (!call.ok()) return call.error();
     if (i_t == 0) {
-        if (add) return STADE_HIP_OK;
         STADE_TIMED("embed_zero", stream,
                     zero_all_kernel<<<(unsigned)std::min<int64_t>(i_v, 1 << 16), NT, 0, stream>>>((char*)wb, i_v, row_bytes, width));
         STADE_LAUNCHED("embed zero_all_kernel");
         return STADE_HIP_OK;
     }
-    WsCall call(stream);
-    if (!call.ok()) return call.error();
     const int64_t strips = (i_d + kCols - 1) / kCols;
     const bool w = i_d >= 8 && (!add || i_d % kCols == 0 || i_d % kCols >= 8);
     if (i_t <= kFewTokens) {

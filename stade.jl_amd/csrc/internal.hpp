@@ -69,10 +69,12 @@ int32_t scratch_error();
 // While the guard lives, the calling thread holds the device's library lock, so calls from
 // other host threads wait (scratch cannot be regrown under a call that is enqueuing into it).
 // If the previous call on the device used another stream, `stream` first waits for an event
-// that call recorded at its end, so calls on different streams that share the workspace run
-// one after the other on the device instead of racing.  The destructor records this call's
-// event on `stream` (a stream that may be destroyed later is never touched again).  A
-// stream under graph capture is neither ordered nor recorded: the caller's graph orders it.
+// behind that call's work, so calls on different streams run one after the other on the device
+// instead of racing, for the workspace or for arrays that they share: every entry point that
+// enqueues has one.  The destructor records this call's event on `stream` (a stream that may be
+// destroyed later is never touched again); on the default stream, only once the device has
+// had calls on a second one: until then the first such call records it there.  A stream
+// under graph capture is neither ordered nor recorded: the caller's graph orders it.
 class WsCall {
   public:
     // with_workspace = false: the lock and the ordering only (the allocation-free entry

@@ -531,6 +531,8 @@ int32_t stade_hip_layernorm(int64_t tx, int64_t tg, void* y, int64_t ldy, const 
     if (!y || !x) return bad(fn, "null pointer");
     if (!q != !qs) return bad(fn, "q and qs go together");
     if ((uintptr_t)q % 8) return bad(fn, "q is not aligned to 8 bytes");
+    WsCall call(stream, false);
+    if (!call.ok()) return call.error();
     const Fwd p{y, ldy, x, ldx, g, b, mu, rs, (uint8_t*)q, qs, (int)i_d, i_n, (float)eps};
     return with_types(tx, tg, [&](auto t, auto w) -> int32_t {
         STADE_TIMED("layernorm", stream, {
@@ -560,6 +562,8 @@ int32_t stade_hip_layernorm_b(int64_t tx, int64_t tg, const void* yb, int64_t ld
     if ((uintptr_t)q % 8) return bad(fn, "q is not aligned to 8 bytes");
     const bool sums = gb || bb;
     if (!some && (!sums || add)) return STADE_HIP_OK;
+    WsCall call(stream);
+    if (!call.ok()) return call.error();
     // a block's rows: enough blocks for two a CU, and no more (each leaves a row of partial sums)
     const unsigned rpb = back_rows(i_d);
     const int64_t trips = (i_n + rpb - 1) / rpb;
@@ -581,8 +585,6 @@ int32_t stade_hip_layernorm_b(int64_t tx, int64_t tg, const void* yb, int64_t ld
     // (long rows: not over 256 MiB of partial sums, but 16 blocks at least)
     const int64_t most = std::min<int64_t>(kSumParts, std::max<int64_t>(16, ((int64_t)1 << 28) / (8 * i_d)));
     const unsigned grid = (unsigned)std::min<int64_t>(trips, most);
-    WsCall call(stream);
-    if (!call.ok()) return call.error();
     float* part = nullptr;
     if (sums && some && !(part = (float*)scratch((size_t)grid * 2 * (size_t)i_d * sizeof(float)))) return scratch_error();
     p.part = part;

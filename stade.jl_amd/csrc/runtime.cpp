@@ -32,12 +32,17 @@ static std::mutex g_ws_mu;
 static Workspace g_ws[64];
 static bool g_ws_ready[64];
 
-// per device: the lock a library call holds while it enqueues, and the event the last call
-// recorded on its stream at its end
+// per device: the lock a library call holds while it enqueues, the last call's stream, and the
+// event that is behind that call's work.  A call records the event at its end, but not on
+// the default stream while no other stream has been used: an event costs the device as much as a
+// small kernel (a call of 3.2 us takes 6.5 with one), and the default stream, which is
+// never destroyed, can still be given it when a call on another stream comes.
 static std::recursive_mutex g_call_mu[64];
 struct CallOrder {
     hipStream_t last;
     bool has_last;
+    bool several;     // calls have come on more than one stream
+    bool recorded;    // `ev` is behind the last call's work
     hipEvent_t ev;
 };
 static CallOrder g_order[64];
@@ -104,8 +109,17 @@ WsCall::WsCall(hipStream_t stream, bool with_workspace)
     capturing_ = hipStreamIsCapturing(stream, &cs) == hipSuccess && cs != hipStreamCaptureStatusNone;
     tl_capturing = capturing_;
     if (capturing_ && w) w->scratch_captured = true;
-    if (!capturing_ && o.has_last && o.last != stream && o.ev) {
-        if ((e = hipStreamWaitEvent(stream, o.ev, 0)) != hipSuccess) {
+    if (!capturing_ && o.has_last && o.last != stream) {
+        o.several = true;
+        if (!o.recorded && o.last == nullptr) {
+            if ((!o.ev && (e = hipEventCreateWithFlags(&o.ev, hipEventDisableTiming)) != hipSuccess) ||
+                (e = hipEventRecord(o.ev, o.last)) != hipSuccess) {
+                err_ = check_hip(e, "hipEventRecord (ordering after the default stream)");
+                return;
+            }
+            o.recorded = true;
+        }
+        if (o.recorded && (e = hipStreamWaitEvent(stream, o.ev, 0)) != hipSuccess) {
             err_ = check_hip(e, "hipStreamWaitEvent (ordering after the previous call's stream)");
             return;
         }
@@ -131,11 +145,14 @@ WsCall::~WsCall() {
     tl_capturing = false;
     if (ok_ && !capturing_) {
         CallOrder& o = g_order[dev_];
-        hipError_t e = hipSuccess;
-        if (!o.ev) e = hipEventCreateWithFlags(&o.ev, hipEventDisableTiming);
-        // a failure leaves the next call on another stream unordered; it is reported by
-        // that call's own first HIP error, if any
-        if (e == hipSuccess) (void)hipEventRecord(o.ev, stream_);
+        o.recorded = false;
+        if (stream_ != nullptr || o.several) {
+            hipError_t e = hipSuccess;
+            if (!o.ev) e = hipEventCreateWithFlags(&o.ev, hipEventDisableTiming);
+            // a failure leaves the next call on another stream unordered; it is reported by
+            // that call's own first HIP error, if any
+            o.recorded = e == hipSuccess && hipEventRecord(o.ev, stream_) == hipSuccess;
+        }
         o.last = stream_;
         o.has_last = true;
     }

@@ -76,6 +76,8 @@ int32_t stade_hip_tape8_store(int64_t type, const void* x, int64_t ldx, int8_t* 
                               hipStream_t stream) {
     if (int32_t rc = check("stade_hip_tape8_store", type, x, ldx, q, qs, i_d, i_n)) return rc;
     if (i_d == 0 || i_n == 0) return STADE_HIP_OK;
+    WsCall call(stream, false);
+    if (!call.ok()) return call.error();
     return rows::with_type(type, [&](auto t) -> int32_t {
         using T = decltype(t);
         STADE_TIMED("tape8_store", stream,
@@ -89,6 +91,8 @@ int32_t stade_hip_tape8_load(int64_t type, const int8_t* q, const uint8_t* qs, v
                              hipStream_t stream) {
     if (int32_t rc = check("stade_hip_tape8_load", type, x, ldx, q, qs, i_d, i_n)) return rc;
     if (i_d == 0 || i_n == 0) return STADE_HIP_OK;
+    WsCall call(stream, false);
+    if (!call.ok()) return call.error();
     return rows::with_type(type, [&](auto t) -> int32_t {
         using T = decltype(t);
         STADE_TIMED("tape8_load", stream,
