@@ -249,8 +249,9 @@ int32_t stade_hip_token_order(const int64_t* tok, int64_t* order, int64_t* start
 
 /* The 8-bit tape of a matrix (i_d, i_n): q Int8, a column's values at a stride of 32 * ceil(i_d / 32), and qs UInt8,
  * one scale for each 32 of a column (a power of two: exponent + 127).  lengths: of q and of qs.  A value reads back as
- * q * 2^(qs - 127), exactly; it is within max|x| / 127 of the 32 values' largest.  A group with a value that is not
- * finite reads back as NaN.  q aligned to 8 bytes. */
+ * q * 2^(qs - 127), exactly in the type it was stored from; it is within max|x| / 127 of x, max|x| the 32 values' largest, or
+ * within 2^-127 where that is more (the least scale is 2^-126).  A group with a value that is not finite reads back
+ * as NaN.  q aligned to 8 bytes. */
 int32_t stade_hip_tape8_lengths(int64_t i_d, int64_t i_n, int64_t lengths[2]);
 int32_t stade_hip_tape8_store(int64_t type, const void* x, int64_t ldx, int8_t* q, uint8_t* qs, int64_t i_d, int64_t i_n,
                               hipStream_t stream);

@@ -3,11 +3,13 @@
 // A row is cut into groups of 32.  A group has one scale 2^e, the least power of two with
 // max|x| <= 127 * 2^e, held as the byte e + 127, and each value is the whole number
 // q = rint(x / 2^e) (to nearest even) in an int8.  x / 2^e is exact, so q is a function of x alone,
-// and q * 2^e has 7 bits: it is exact in fp32, bf16 and f16, so a product may take it as a 16-bit
-// operand without a further rounding.  |x - q 2^e| <= 2^(e-1) <= max|x| / 127.
-//   - a group of zeros has byte 1 (2^-126, the least scale; smaller values flush to q = 0);
-//   - a group with an infinity or a NaN has byte 255 and reads back as NaN (0 * inf);
-//   - |q| stops at 63 where 64 * 2^e would be the element type's infinity.
+// and q * 2^e has 7 bits: it is exact in fp32, bf16 and f16 (the type that x had), so a product may
+// take it as a 16-bit operand without a further rounding.  |x - q 2^e| <= 2^(e-1) <= max|x| / 127.
+//   - e is at least -126 (byte 1; also of a group of zeros): there |x - q 2^e| <= 2^-127, and values
+//     of at most 2^-127 become 0;
+//   - where 64 * 2^e would be the element type's infinity, e is one less, and |q| stops at 127: the
+//     largest values are below 128 of that scale, so they too are within max|x| / 127;
+//   - a group with an infinity or a NaN has byte 255 and reads back as NaN (0 * inf).
 // Rows are held at a stride of 32 * ceil(d / 32) bytes, the places past d zero, so that every
 // group's 32 bytes are aligned whatever d is.
 #pragma once
@@ -28,20 +30,19 @@ template <> constexpr uint32_t top_exponent<rows::f16>() { return 142; }
 
 struct Scale {
     uint32_t byte;   // e + 127
-    float inv, lim;  // 2^-e, and the largest |q|
+    float inv;       // 2^-e
 };
 
 // `big`: the largest |x| of the group as bits (bit order is size order, with NaN above infinity)
 template <class T>
 __device__ __forceinline__ Scale scale_of(uint32_t big) {
     const uint32_t k = big >> 23;
-    // max|x| = m 2^(k-127): m 2^6 <= 127 for m up to 127/64, else one binade more
-    const bool up = (big & 0x7fffffu) > 0x7e0000u;
+    // max|x| = m 2^(k-127): m 2^6 <= 127 for m up to 127/64, else one binade more, if there is one
+    const bool up = (big & 0x7fffffu) > 0x7e0000u && k != top_exponent<T>();
     Scale s;
     const int b = (int)k - 6 + (up ? 1 : 0);
     s.byte = k == 255u ? 255u : (uint32_t)(b < 1 ? 1 : b);
     s.inv = k == 255u ? 0.f : __uint_as_float((254u - s.byte) << 23);
-    s.lim = up && k == top_exponent<T>() ? 63.f : 127.f;
     return s;
 }
 
@@ -67,7 +68,7 @@ template <int N>
 __device__ __forceinline__ void put(uint8_t* q, const float (&x)[N], const Scale& s) {
     uint32_t w[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = __float_as_uint(__builtin_amdgcn_fmed3f(x[i] * s.inv, -s.lim, s.lim) + 12582912.f);
+    for (int i = 0; i < N; ++i) w[i] = __float_as_uint(__builtin_amdgcn_fmed3f(x[i] * s.inv, -127.f, 127.f) + 12582912.f);
     const uint32_t keep = s.byte == 255u ? 0u : ~0u;
     const auto two = [](uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x0c0c0400u); };
     if constexpr (N == 8) {
