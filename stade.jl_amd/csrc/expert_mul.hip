@@ -739,7 +739,8 @@ Plan plan(const Mul& p) {
     // 43.4 -> 31.3 us, xb 45.7 -> 25.8; 3584 rows, 2 experts, 128 x 295: wb 37 -> 20; in fp32 137 rows, 4 experts, 1856 x 256: y
     // 71 -> 18.  Saving 8 steps: 1000 rows, 7 experts, 500 x 700, fp32: 18.7 -> 23.7.
     const int64_t small = std::max<int64_t>(1, (FORM == WB ? (int64_t)p.ne * ((p.m + 63) / 64) : p.t / 64 + std::min<int64_t>(p.ne, p.t)) * ((p.n + 63) / 64));
-    const int64_t steps = (FORM == WB ? p.t / p.ne : p.k) / kBK<T>, slices = std::min<int64_t>(std::min<int64_t>(2 * p.cus / small, steps / 4), 32);
+    // (no experts, no products: nothing to slice)
+    const int64_t steps = p.ne == 0 ? 0 : (FORM == WB ? p.t / p.ne : p.k) / kBK<T>, slices = std::min<int64_t>(std::min<int64_t>(2 * p.cus / small, steps / 4), 32);
     if (small < p.cus && slices >= 2 && steps - steps / slices >= 12) return Plan{direct, SMALL, (int)slices};
     // Few rows an expert (y and xb: at most 64): bound by reading w, so small tiles, many blocks and three or four
     // steps in flight.  24 rows, 8 experts, 2048 x 4096, bf16: y 26.6 us (128 x 128 tiles 28.7, quarters 27.4), xb 24.8
