@@ -36,7 +36,7 @@
  *     has been given by then.
  *   - Graph capture: a call on a capturing stream takes no dependency outside the capture, and
  *     the workspace does not grow under capture (STADE_HIP_ESTATE): make one eager call of the
- *     largest size first.  Replays are not ordered against eager calls on other streams (the
+ *     function at its largest size first.  Replays are not ordered against eager calls on other streams (the
  *     caller orders them, as any graph); they share the workspace with those calls.  A scratch
  *     buffer that a captured graph may hold is never freed: a later, larger eager call retires
  *     it and allocates another, so earlier graphs stay valid.

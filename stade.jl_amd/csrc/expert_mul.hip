@@ -833,6 +833,15 @@ int cu_count() {
 
 int32_t* error_flag(Workspace* ws) { return (int32_t*)(ws->dscalars + kErrFlagSlot); }
 
+// Small products take scratch where large ones take none (`plan`): every eager call makes sure of what any product in
+// slices needs, so that a smaller one may be captured after it.  There are at most 2 cus tiles of 64 x 64 in fp32: `slices`
+// is 2 cus / small at most, and the result lies in `small` tiles (8 MiB for 256 CUs).
+int32_t reserve(const WsCall& call, int cus) {
+    const size_t bytes = (size_t)2 * cus * 64 * 64 * sizeof(float);
+    if (call.capturing() || call.ws->scratch_bytes >= bytes) return 0;
+    return scratch(bytes) ? 0 : scratch_error();
+}
+
 }  // namespace
 }  // namespace stade
 
@@ -855,6 +864,7 @@ int32_t stade_hip_expert_mul(int64_t tx, void* y, int64_t ldy, const void* x, in
     p.start = start; p.ne = (int)i_e; p.t = i_t; p.n = (int)i_out; p.k = (int)i_in; p.add = add != 0; p.flag = error_flag(call.ws);
     p.cus = cu_count();
     p.split = 1;
+    if (int32_t rc = reserve(call, p.cus)) return rc;
     return with_type(tx, [&](auto t) -> int32_t { return run<decltype(t), decltype(t), Y, false>(p, stream, "expert_mul"); });
 }
 
@@ -880,6 +890,7 @@ int32_t stade_hip_expert_mul_b(int64_t tx, int64_t twb, const void* yb, int64_t 
     p.start = start; p.ne = (int)i_e; p.t = i_t; p.add = add != 0; p.flag = error_flag(call.ws);
     p.cus = cu_count();
     p.split = 1;
+    if (int32_t rc = reserve(call, p.cus)) return rc;
     Mul px = p, pw = p;
     px.a = yb; px.lda = ldyb; px.b = w; px.ldb = i_out; px.c = xb; px.ldc = ldxb; px.n = (int)i_in; px.k = (int)i_out;
     pw.a = x; pw.lda = ldx; pw.q = (const uint8_t*)q; pw.qs = qs; pw.b = yb; pw.ldb = ldyb; pw.c = wb; pw.m = (int)i_in; pw.n = (int)i_out;

@@ -168,7 +168,7 @@ void* scratch(size_t bytes) {
             tl_scratch_code = STADE_HIP_ESTATE;
             set_error(STADE_HIP_ESTATE,
                       "the library workspace cannot grow under graph capture (%zu bytes needed, %zu held): "
-                      "make one eager call of the largest size before capturing", bytes, w->scratch_bytes);
+                      "make one eager call of the function at its largest size before capturing", bytes, w->scratch_bytes);
             return nullptr;
         }
         if (w->scratch) {

@@ -1,0 +1,79 @@
+"""Calls captured in a HIP graph after one eager call of the function at its largest size: smaller ones
+may take scratch where the largest takes none, or more of it, and are captured all the same.
+
+The scratch only grows within a process, so each case runs in one of its own."""
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from lmhelp import gen, normal
+
+pytestmark = pytest.mark.gpu
+
+
+def _expert_mul(t, e, i, o):
+    import stade_hip as hip
+    g = gen(t)
+    x, w = (normal(g, *s, dtype=torch.bfloat16).cuda() for s in ((t, i), (e, i, o)))
+    y = torch.zeros(t, o, dtype=torch.bfloat16, device="cuda")
+    start = (torch.arange(e + 1) * t // e).cuda()
+    return lambda: hip.expert_mul(y, x, w, start, i, o, t, e), [y]
+
+
+def _expert_mul_b(t, e, i, o):
+    import stade_hip as hip
+    g = gen(t)
+    x, w, yb = (normal(g, *s).cuda() for s in ((t, i), (e, i, o), (t, o)))
+    xb, wb = torch.zeros(t, i, device="cuda"), torch.zeros(e, i, o, device="cuda")
+    start = (torch.arange(e + 1) * t // e).cuda()
+    return lambda: hip.expert_mul_b(yb, x, xb, w, wb, start, i, o, t, e, add=False), [xb, wb]
+
+
+# function, the largest call, and smaller ones that take more scratch
+CASES = {
+    "expert_mul": (_expert_mul, (8192, 4, 2048, 2560), [(64, 4, 1672, 2484), (30, 2, 2000, 72)]),
+    "expert_mul_b": (_expert_mul_b, (4096, 4, 2048, 2560), [(64, 4, 1672, 2484), (3584, 2, 128, 295)]),
+}
+
+
+def capture_after_largest(name):
+    import stade_hip
+    make, largest, smaller = CASES[name]
+    print(f"{name}: eager {largest}", flush=True)
+    make(*largest)[0]()
+    torch.cuda.synchronize()
+    for size in smaller:
+        call, outs = make(*size)
+        print(f"{name}: captured {size}, {stade_hip.workspace_info()[0]} bytes held", flush=True)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call()
+        call()
+        torch.cuda.synchronize()
+        eager = [v.clone() for v in outs]
+        for rep in range(3):
+            for v in outs:
+                v.zero_()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(v, w) for v, w in zip(outs, eager)), f"{name} {size}: replay {rep}"
+            _ = torch.randn(1000, device="cuda").sum().item()
+    print("captured", flush=True)
+
+
+def _in_a_process(call):
+    from helpers import ROOT
+    code = (f"import sys; sys.path[:0] = [{str(ROOT / 'tests')!r}, {str(ROOT / 'stade.jl_amd')!r}]; "
+            f"import test_gpu_lm_capture as m; m.{call}")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100, cwd=str(ROOT))
+    assert r.returncode == 0 and "captured" in r.stdout.split(), r.stdout[-2000:] + r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("name", CASES)
+def test_smaller_calls_are_captured_after_the_largest(name):
+    print(f"capture after the largest call: {name}", flush=True)
+    _in_a_process(f"capture_after_largest({name!r})")
