@@ -759,16 +759,26 @@ Plan plan(const Mul& p) {
     return Plan{direct, few || 4 * est <= p.cus ? SMALL : LARGE, 1};
 }
 
+// the rows of a product's result, and the scratch that its slices take
+template <int FORM>
+int64_t result_rows(const Mul& p) {
+    return FORM == WB ? (int64_t)p.ne * p.m : p.t;
+}
+template <int FORM>
+size_t slice_bytes(const Mul& p, const Plan& how) {
+    return how.slices > 1 ? (size_t)how.slices * result_rows<FORM>(p) * p.n * sizeof(float) : 0;
+}
+
 template <class T, class TC, int FORM, bool TAPE>
 int32_t run(const Mul& p, hipStream_t stream, const char* name) {
     const Plan how = plan<T, FORM, TAPE>(p);
     if (how.slices > 1) {
-        const int64_t rows = FORM == WB ? (int64_t)p.ne * p.m : p.t;
+        const int64_t rows = result_rows<FORM>(p);
         Mul q = p;
         q.split = how.slices;
         q.add = 0;
         q.ldc = p.n;
-        if (!(q.c = scratch((size_t)q.split * rows * p.n * sizeof(float)))) return scratch_error();
+        if (!(q.c = scratch(slice_bytes<FORM>(p, how)))) return scratch_error();
         const int32_t rc = how.direct ? launch<T, float, FORM, TAPE, true, 64, 64, 2, 2, small_buffers(TAPE, true)>(q, stream, name)
                                       : launch<T, float, FORM, TAPE, false, 64, 64, 2, 2>(q, stream, name);
         if (rc) return rc;
@@ -812,6 +822,9 @@ int32_t run_both(Mul px, Mul pw, hipStream_t stream) {
             if (x.direct) return go(std::true_type{});
         return go(std::false_type{});
     }
+    // (a call that is refused its scratch enqueues nothing: the larger one's first)
+    const size_t bytes = std::max(slice_bytes<XB>(px, x), slice_bytes<WB>(pw, w));
+    if (bytes > 0 && !scratch(bytes)) return scratch_error();
     if (int32_t rc = run<T, T, XB, false>(px, stream, "expert_mul_xb")) return rc;
     return run<T, TC, WB, TAPE>(pw, stream, "expert_mul_wb");
 }

@@ -65,12 +65,35 @@ def capture_after_largest(name):
     print("captured", flush=True)
 
 
+def refused_call_enqueues_nothing():
+    """Captured with no eager call before: refused, and the graph holds no part of the call."""
+    import stade_hip
+    call, (xb, wb) = _expert_mul_b(3584, 2, 128, 295)   # (wb in slices, xb not)
+    print("expert_mul_b captured first", flush=True)
+    stade_hip.workspace_info()   # (the workspace is there, without scratch)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(stade_hip.StadeHipError, match="cannot grow under graph capture"):
+        with torch.cuda.graph(graph):
+            xb.add_(1.0)
+            call()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert xb.eq(1.0).all() and not wb.any()
+    print("captured", flush=True)
+
+
 def _in_a_process(call):
     from helpers import ROOT
     code = (f"import sys; sys.path[:0] = [{str(ROOT / 'tests')!r}, {str(ROOT / 'stade.jl_amd')!r}]; "
             f"import test_gpu_lm_capture as m; m.{call}")
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100, cwd=str(ROOT))
     assert r.returncode == 0 and "captured" in r.stdout.split(), r.stdout[-2000:] + r.stderr[-2000:]
+
+
+def test_a_refused_call_enqueues_nothing():
+    print("capture without an eager call: expert_mul_b", flush=True)
+    _in_a_process("refused_call_enqueues_nothing()")
 
 
 @pytest.mark.parametrize("name", CASES)
