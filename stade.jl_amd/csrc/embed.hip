@@ -770,7 +770,7 @@ int32_t stade_hip_embed_b(int64_t ty, int64_t tw, const void* yb, int64_t ldyb, 
     if ((i_v > 0 && !wb) || (i_t > 0 && (!yb || !tok))) return bad(fn, "null pointer");
     const int64_t row_bytes = ldwb * type_size(tw), width = i_d * type_size(tw);
     if (i_t == 0 && add) return STADE_HIP_OK;
-    WsCall call(stream);
+    WsCall call(stream, i_t > 0);
     if (!call.ok()) return call.error();
     if (i_t == 0) {
         STADE_TIMED("embed_zero", stream,

@@ -562,15 +562,16 @@ int32_t stade_hip_layernorm_b(int64_t tx, int64_t tg, const void* yb, int64_t ld
     if ((uintptr_t)q % 8) return bad(fn, "q is not aligned to 8 bytes");
     const bool sums = gb || bb;
     if (!some && (!sums || add)) return STADE_HIP_OK;
-    WsCall call(stream);
-    if (!call.ok()) return call.error();
     // a block's rows: enough blocks for two a CU, and no more (each leaves a row of partial sums)
     const unsigned rpb = back_rows(i_d);
     const int64_t trips = (i_n + rpb - 1) / rpb;
+    const bool one = some && trips <= kOneBlock && i_d <= kMostHeldBack, parts = sums && some && !one;
+    WsCall call(stream, parts);   // (the workspace for the partial sums only: without them nothing has to be allocated before a capture)
+    if (!call.ok()) return call.error();
     Bwd p{yb, ldyb, x, ldx, (const uint8_t*)q, qs, xb, ldxb, g, mu, rs, nullptr, nullptr, nullptr, (int)i_d, i_n, add != 0};
     // Few rows: one block, which leaves gb and bb whole (each of its trips takes about a microsecond, the second
     // launch and the scratch five).
-    if (some && trips <= kOneBlock && i_d <= kMostHeldBack) {
+    if (one) {
         p.gb = gb;
         p.bb = bb;
         return with_types(tx, tg, [&](auto t, auto w) -> int32_t {
@@ -586,7 +587,7 @@ int32_t stade_hip_layernorm_b(int64_t tx, int64_t tg, const void* yb, int64_t ld
     const int64_t most = std::min<int64_t>(kSumParts, std::max<int64_t>(16, ((int64_t)1 << 28) / (8 * i_d)));
     const unsigned grid = (unsigned)std::min<int64_t>(trips, most);
     float* part = nullptr;
-    if (sums && some && !(part = (float*)scratch((size_t)grid * 2 * (size_t)i_d * sizeof(float)))) return scratch_error();
+    if (parts && !(part = (float*)scratch((size_t)grid * 2 * (size_t)i_d * sizeof(float)))) return scratch_error();
     p.part = part;
     return with_types(tx, tg, [&](auto t, auto w) -> int32_t {
         if (some) {

@@ -83,6 +83,44 @@ def refused_call_enqueues_nothing():
     print("captured", flush=True)
 
 
+def first_call_without_workspace():
+    """Calls that use nothing of the library's are captured with no call before them."""
+    import stade_hip as hip
+    n, d = 8, 256
+    g = gen(5)
+    x, yb = normal(g, n, d).cuda(), normal(g, n, d).cuda()
+    y, xb, back, wb = (torch.full((n, d), 7.0, device="cuda") for _ in range(4))
+    mu, rs, gb, bb = (torch.zeros(k, device="cuda") for k in (n, n, d, d))
+    q, qs = torch.zeros(n * d, dtype=torch.int8, device="cuda"), torch.zeros(n * d // 32, dtype=torch.uint8, device="cuda")
+    none, no_rows = torch.empty(0, dtype=torch.int64, device="cuda"), torch.empty(0, d, device="cuda")
+
+    def calls():
+        hip.layernorm(y, x, None, None, mu, rs, d, n, tape=(q, qs))
+        hip.tape8_store(x, q, qs, d, n)
+        hip.tape8_load(q, qs, back, d, n)
+        hip.layernorm_b(yb, x, xb, None, gb, bb, mu, rs, d, n, add=False)
+        hip.embed_b(no_rows, wb, none, 1.0, d, n, 0, add=False)
+
+    print("norms and tape captured first", flush=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls()
+    outs = [y, xb, back, wb, mu, rs, gb, bb, q, qs]
+    calls()
+    torch.cuda.synchronize()
+    eager = [v.clone() for v in outs]
+    for rep in range(3):
+        for v in outs:
+            v.fill_(3)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(v, w) for v, w in zip(outs, eager)), f"replay {rep}"
+        _ = torch.randn(1000, device="cuda").sum().item()
+    print("captured", flush=True)
+
+
 def _in_a_process(call):
     from helpers import ROOT
     code = (f"import sys; sys.path[:0] = [{str(ROOT / 'tests')!r}, {str(ROOT / 'stade.jl_amd')!r}]; "
@@ -94,6 +132,11 @@ def _in_a_process(call):
 def test_a_refused_call_enqueues_nothing():
     print("capture without an eager call: expert_mul_b", flush=True)
     _in_a_process("refused_call_enqueues_nothing()")
+
+
+def test_first_calls_that_need_no_workspace():
+    print("capture without an eager call: norms, tape", flush=True)
+    _in_a_process("first_call_without_workspace()")
 
 
 @pytest.mark.parametrize("name", CASES)
