@@ -688,6 +688,15 @@ __global__ __launch_bounds__(NT) void zero_all_kernel(char* wb, int64_t rows, in
     for (int64_t r = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6); r < rows; r += (int64_t)gridDim.x * (NT / 64)) zero_row(wb + r * row_bytes, width);
 }
 
+// Bytes of partial sums, two rows a chunk: enough for any fewer tokens and columns too, so that a call captured after a
+// larger eager one finds its scratch.  Short chunks are for less than 2048 strips (below), whose partial
+// sums take less than 17 MiB: t / 16 * strips < 2048 and d <= 512 strips.
+constexpr size_t kShortMost = (size_t)17 << 20;
+size_t part_bytes(int64_t t, int64_t d) {
+    const size_t whole = (size_t)((t + kChunk - 1) / kChunk) * 2 * (size_t)d * 4, brief = (size_t)((t + kShortChunk - 1) / kShortChunk) * 2 * (size_t)d * 4;
+    return (std::max(whole, std::min(brief, kShortMost)) + 255) / 256 * 256;
+}
+
 constexpr int64_t kMostIds = (int64_t)1 << 30;
 
 }  // namespace
@@ -807,7 +816,7 @@ int32_t stade_hip_embed_b(int64_t ty, int64_t tw, const void* yb, int64_t ldyb, 
         });
     }
     const int64_t chunk = i_t / kChunk * strips < 2048 ? kShortChunk : kChunk, chunks = (i_t + chunk - 1) / chunk;
-    const size_t keys = ((size_t)i_t * 4 + 255) / 256 * 256, parts = ((size_t)chunks * 2 * (size_t)i_d * 4 + 255) / 256 * 256;
+    const size_t keys = ((size_t)i_t * 4 + 255) / 256 * 256, parts = part_bytes(i_t, i_d);
     const bool one = one_block(i_t, i_v);
     char* work = (char*)scratch(2 * keys + parts + (one ? 0 : radix_bytes(i_t)));
     if (!work) return scratch_error();

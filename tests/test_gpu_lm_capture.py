@@ -31,10 +31,18 @@ def _expert_mul_b(t, e, i, o):
     return lambda: hip.expert_mul_b(yb, x, xb, w, wb, start, i, o, t, e, add=False), [xb, wb]
 
 
+def _embed_b(t, d, v):
+    import stade_hip as hip
+    g = gen(t)
+    yb, tok, wb = normal(g, t, d).cuda(), torch.randint(0, v + 1, (t,), generator=g).cuda(), torch.zeros(v, d, device="cuda")
+    return lambda: hip.embed_b(yb, wb, tok, 0.5, d, v, t, add=False), [wb]
+
+
 # function, the largest call, and smaller ones that take more scratch
 CASES = {
     "expert_mul": (_expert_mul, (8192, 4, 2048, 2560), [(64, 4, 1672, 2484), (30, 2, 2000, 72)]),
     "expert_mul_b": (_expert_mul_b, (4096, 4, 2048, 2560), [(64, 4, 1672, 2484), (3584, 2, 128, 295)]),
+    "embed_b": (_embed_b, (40000, 512, 300), [(32000, 512, 300), (32767, 500, 299)]),
 }
 
 
