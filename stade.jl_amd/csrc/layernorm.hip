@@ -587,7 +587,11 @@ int32_t stade_hip_layernorm_b(int64_t tx, int64_t tg, const void* yb, int64_t ld
     const int64_t most = std::min<int64_t>(kSumParts, std::max<int64_t>(16, ((int64_t)1 << 28) / (8 * i_d)));
     const unsigned grid = (unsigned)std::min<int64_t>(trips, most);
     float* part = nullptr;
-    if (parts && !(part = (float*)scratch((size_t)grid * 2 * (size_t)i_d * sizeof(float)))) return scratch_error();
+    // (as much as any fewer rows and columns take, so that a call captured after a larger eager one finds its scratch:
+    // `most` rounds down, and 2^16 columns take all of the 256 MiB where some longer rows take less)
+    const size_t room = std::max<size_t>((size_t)1 << 28, (size_t)16 * 8 * i_d);
+    const size_t bytes = std::min((size_t)std::min<int64_t>(trips, kSumParts) * 8 * (size_t)i_d, room);
+    if (parts && !(part = (float*)scratch(bytes))) return scratch_error();
     p.part = part;
     return with_types(tx, tg, [&](auto t, auto w) -> int32_t {
         if (some) {

@@ -38,11 +38,20 @@ def _embed_b(t, d, v):
     return lambda: hip.embed_b(yb, wb, tok, 0.5, d, v, t, add=False), [wb]
 
 
+def _layernorm_b(n, d):
+    import stade_hip as hip
+    g = gen(n)
+    x, yb, xb = normal(g, n, d).cuda(), normal(g, n, d).cuda(), torch.zeros(n, d, device="cuda")
+    gb, bb, mu, rs = torch.zeros(d, device="cuda"), torch.zeros(d, device="cuda"), torch.zeros(n, device="cuda"), torch.ones(n, device="cuda")
+    return lambda: hip.layernorm_b(yb, x, xb, None, gb, bb, mu, rs, d, n, add=False), [xb, gb, bb]
+
+
 # function, the largest call, and smaller ones that take more scratch
 CASES = {
     "expert_mul": (_expert_mul, (8192, 4, 2048, 2560), [(64, 4, 1672, 2484), (30, 2, 2000, 72)]),
     "expert_mul_b": (_expert_mul_b, (4096, 4, 2048, 2560), [(64, 4, 1672, 2484), (3584, 2, 128, 295)]),
     "embed_b": (_embed_b, (40000, 512, 300), [(32000, 512, 300), (32767, 500, 299)]),
+    "layernorm_b": (_layernorm_b, (520, 70000), [(520, 65536), (512, 65537)]),
 }
 
 
