@@ -20,9 +20,9 @@
 //   3. run_join_kernel: for each run that spans chunks, its partial sums in order.
 // Up to 256 tokens take one launch, few_kernel.  More tokens than one block sorts go through a radix sort over blocks, 8 bits a pass.
 // Bound by HBM: yb read once, wb written once.  Measured on an MI355X: 16384 tokens of 2048 (bf16) into 65536 rows
-// (fp32) 143 us, 85 of them for the zero rows (5.4 TB/s) with the sort hidden behind them; 3001 tokens of 515 into 10007
-// rows (fp32) 23 us, of which 20 are three dependent launches; added to what is there (no zero rows) 16384 tokens
-// take 74 us.
+// (fp32) 139 us, 86 of them for the zero rows (5.4 TB/s) with the sort hidden behind them, 74 added to what is there (no zero
+// rows); 3001 tokens of 515 into 10007 rows (fp32) 20 us, three dependent launches.  Above 16384 tokens nothing hides the
+// zero rows: 65536 tokens of 1024 into 65536 rows 190 us, added 135, of which the order by id takes 65.
 #include "rows.hpp"
 
 #include <algorithm>
@@ -243,8 +243,9 @@ __device__ __forceinline__ void zero_rows(const Sort& p, int part, int parts, ui
 
 // The order of few tokens by counting: an item's place is the number of items before it, those of a
 // smaller key and those of its own key that came first.  Every block holds all the keys in LDS; a
-// wave takes an item at a time.  n^2 comparisons over all the CUs: 2 us for 5000 items, where the sort in
-// one block takes 10.  The same blocks then clear rows.
+// wave takes an item at a time.  n^2 comparisons over all the CUs: the launch takes 3.9, 5.6, 10.3 and 16.3 us for 1000, 3001,
+// 5000 and 8192 items; the sort in one block 18.7, 26.7, 15.6 and 15.9 (of 300, 10007, 60 and 60 ids: it takes more passes
+// for more ids).  The same blocks then clear rows.
 constexpr int kRankMost = 8192;
 __global__ __launch_bounds__(kSortNT) void rank_kernel(Sort p) {
     __shared__ uint32_t keys[kRankMost], marks[kZeroRows];

@@ -11,12 +11,13 @@
 // fp32 and rounded once.  The tape's values are exact in 16 bits, so wb from the tape needs no further rounding.
 //
 // Bound by the matrix cores for many rows, by reading w for few.  On an MI355X in bf16:
-//   one round of 256 x 256 tiles (4096 x 4096, k = 4096): 117 us, 1170 TFLOP/s.  A step of 64 k takes 1.56 us: 1.24
-//     with its loads left out, 1.15 without LDS reads either (the matrix cores at the clock that they hold);
-//     18 us are prologue and epilogue, whatever k is.
-//   16384 rows, 16 experts, 2048 x 4096: y 305 us (903 TFLOP/s), xb 291 (944), wb in fp32 336 (819; its 537 MB alone
-//     take 107 us), wb from the tape 361 (the bytes become 16-bit values between the products).
-//   24 rows, 8 experts, 2048 x 4096: y 26.7 us, xb 24.7 (5.0 and 5.4 TB/s of w).
+//   one round of 256 x 256 tiles (4096 x 4096): 41, 65, 116 and 218 us for k = 1024, 2048, 4096 and 8192 (1190 TFLOP/s at
+//     4096): 1.6 us a step of 64 k and 14 us whatever k is (launch, prologue and epilogue).
+//   16384 rows, 16 experts with as many each, 2048 x 4096: y 252 us (1090 TFLOP/s), xb 248 (1110), wb in fp32 326 (844; its
+//     537 MB alone take 107 us), wb from the tape 347 (the bytes become 16-bit values between the products).  With uneven
+//     shares (a standard deviation of 30 %) xb 289 us, wb from the tape 360.  Added to what is there: y 313 us, xb 278, wb in fp32
+//     469, in bf16 410 (293 set): 16-bit results that add go out straight from the registers.
+//   24 rows, 8 experts, 2048 x 4096: y 23.5 us, xb 21.8 (5.7 and 6.2 TB/s of w, which the last-level cache holds in part).
 #include "tape8.hpp"
 
 #include <algorithm>
@@ -747,8 +748,10 @@ Plan plan(const Mul& p) {
     // (45, 37).
     const bool few = FORM != WB && p.t <= 64 * (int64_t)p.ne;
     if (direct && few) return Plan{direct, FORM == Y ? FLAT : SMALL, 1};
-    // fp32 is bound by its matrix instructions: the tile that fills the CUs (1000 rows, 7 experts, 500 x 700: 64 x 64
-    // 18 us, 128 x 128 42; 8192 rows, 8 experts, 2048 x 1024: y 378 and 408, wb 302 and 272)
+    // fp32 is bound by its matrix instructions: the tile that fills the CUs.  1000 rows, 7 experts, 500 x 700: y 15 us with
+    // 64 x 64 tiles, 39 with 128 x 128 (xb 18 and 51, wb 17 and 18); 16384 rows, 16 experts, 2048 x 2048 (`est` 576):
+    // y 1169 and 1016, xb 1121 and 997, wb 1192 and 1037.  Between these the rule takes the small tiles where the large
+    // ones win: 8192 rows, 8 experts, 2048 x 1024 (`est` 144, of wb 256): y 296 and 258, xb 294 and 257, wb 302 and 262.
     if (sizeof(T) == 4) return Plan{direct, est < 2 * p.cus ? SMALL : MIDDLE, 1};
     // Less than a round of large tiles, more than one of quarters: 128 x 128 tiles of four waves, two
     // blocks a CU.  4096 rows, 8 experts, 1024 x 1024: 22.8 us, with quarters 29.0; 1024 rows, 4 experts,

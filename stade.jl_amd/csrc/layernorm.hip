@@ -13,10 +13,13 @@
 // atomics, the same bits at every call.  Sums are fp32 throughout.
 // Rows longer than the registers hold are read again for each of the sums.
 //
-// Measured on an MI355X (16384 x 4096 bf16, copy 4.7 TB/s): forward 56 us (4.8 TB/s), with the tape 86 (4.0);
-// reverse 86 us (4.7 TB/s), from the tape 84 (4.0; the bytes turn into values by one conversion, one subtraction
-// and one product each).  In the reverse sweep the next row, its statistics and the weights are in registers
-// before the row's sums are waited for: without them 152 us.
+// Measured on an MI355X (16384 x 4096 bf16, calls one after the other: arrays of 134 MB stay in the last-level cache in
+// part; copy 4.7 TB/s): forward 45 us (6.0 TB/s), with the tape 69 (4.9); reverse 79 us (5.1 TB/s), from the tape 71 (4.7;
+// the bytes turn into values by one conversion, one subtraction and one product each).  In the reverse sweep the next
+// row, its statistics and the weights are in registers before the row's sums are waited for: without them 152 us.
+// Longer rows are slower: 4096 x 12288 bf16 forward 50 us (4.0 TB/s), reverse 77 (3.9: the registers do not hold
+// all of two rows and the sums, and some go through scratch memory); 4096 x 24576 reverse 430 us (1.4 TB/s: read twice,
+// and each block adds to its partial sums in memory).
 #include "tape8.hpp"
 
 #include <algorithm>
@@ -465,8 +468,10 @@ void start(const Bwd& p, unsigned grid, hipStream_t stream) {
     else backward_kernel<T, G, VE, NV, WPR, NT, TAPE, false><<<grid, NT, 0, stream>>>(p);
 }
 
-// The form by the row's length.  Forward: the fewest waves a row that hold it in 4 vectors a thread, from
-// 2048 on four waves.
+// The form by the row's length.  Forward: a wave a row up to 1024, then the waves that hold it in at most 4 vectors a
+// thread.  Other splits come close (bf16, and with the tape): 16384 x 2048 four waves of one vector 26.4 us (29.5), one
+// wave of four 24.5 (28.1); 16384 x 4096 two waves of four 43.3 (66.9), four of two 42.4 (65.0); 4096 x 12288 sixteen waves of
+// two 50.4 (62.4), eight of four 36.2 (63.0).
 template <class T, class G, bool TAPE>
 void launch(const Fwd& p, hipStream_t s) {
     const int d = p.d;
