@@ -20,7 +20,7 @@
 //   3. run_join_kernel: for each run that spans chunks, its partial sums in order.
 // Up to 256 tokens take one launch, few_kernel.  More tokens than one block sorts go through a radix sort over blocks, 8 bits a pass.
 // Bound by HBM: yb read once, wb written once.  Measured on an MI355X: 16384 tokens of 2048 (bf16) into 65536 rows
-// (fp32) 139 us, 86 of them for the zero rows (5.4 TB/s) with the sort hidden behind them, 74 added to what is there (no zero
+// (fp32) 139 us, 86 of them for the zero rows (5.4 TB/s) with the sort hidden behind them, 71 added to what is there (no zero
 // rows); 3001 tokens of 515 into 10007 rows (fp32) 20 us, three dependent launches.  Above 16384 tokens nothing hides the
 // zero rows: 65536 tokens of 1024 into 65536 rows 190 us, added 135, of which the order by id takes 65.
 #include "rows.hpp"
@@ -460,12 +460,18 @@ __device__ __forceinline__ void put(const Runs& p, uint32_t key, int col, const 
     if (p.add) load_row<W>(o, out, p.d - col);
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] = p.add ? fmaf(p.s, acc[i], o[i]) : p.s * acc[i];
-    store_row<W>(out, o, p.d - col);
+    if (W && p.add && col % 8 != 0) {   // (moved back: what it shares with the vector before is that lane's to write)
+#pragma unroll
+        for (int i = 1; i < 8; ++i)
+            if (i >= 8 - p.d % 8) out[i] = (TW)o[i];
+    } else {
+        store_row<W>(out, o, p.d - col);
+    }
 }
 
 // W: no tests value by value.  A row's last vector is moved back to end with the row; what it shares with the
-// one before is written twice, the same.  (With `add` that is right within a wave, which reads before
-// it writes, but not where the last vector is a wave's only one: the values before it are another's.)
+// one before is written twice, the same, or with `add` by the one before alone: a lane may read what it shares after the
+// other has written it.
 template <class TY, class TW, bool W>
 __global__ __launch_bounds__(NT) void run_sum_kernel(Runs p) {
     const int strips = (p.d + kCols - 1) / kCols;
@@ -789,7 +795,7 @@ int32_t stade_hip_embed_b(int64_t ty, int64_t tw, const void* yb, int64_t ldyb, 
         return STADE_HIP_OK;
     }
     const int64_t strips = (i_d + kCols - 1) / kCols;
-    const bool w = i_d >= 8 && (!add || i_d % kCols == 0 || i_d % kCols >= 8);
+    const bool w = i_d >= 8;
     if (i_t <= kFewTokens) {
         Sort o{};
         o.tok = tok;
