@@ -17,9 +17,10 @@
 // part; copy 4.7 TB/s): forward 45 us (6.0 TB/s), with the tape 69 (4.9); reverse 79 us (5.1 TB/s), from the tape 71 (4.7;
 // the bytes turn into values by one conversion, one subtraction and one product each).  In the reverse sweep the next
 // row, its statistics and the weights are in registers before the row's sums are waited for: without them 152 us.
-// Longer rows are slower: 4096 x 12288 bf16 forward 50 us (4.0 TB/s), reverse 77 (3.9: the registers do not hold
-// all of two rows and the sums, and some go through scratch memory); 4096 x 24576 reverse 430 us (1.4 TB/s: read twice,
-// and each block adds to its partial sums in memory).
+// Longer rows are slower: 4096 x 12288 bf16 forward 50 us (4.0 TB/s), reverse 77 (3.9), from the tape 67 (3.8), fp32 147
+// (4.1; in fp32 and from the tape the registers do not hold two rows' values and the sums, and some go through scratch
+// memory, as from 16385 columns on in the forward sweep with the tape); 4096 x 24576 reverse 430 us (1.4 TB/s: read
+// twice, and each block adds to its partial sums in memory).
 #include "tape8.hpp"
 
 #include <algorithm>
