@@ -279,6 +279,74 @@ int32_t stade_hip_expert_mul_b(int64_t tx, int64_t twb, const void* yb, int64_t 
                                const uint8_t* qs, void* xb, int64_t ldxb, const void* w, void* wb, const int64_t* start, int64_t i_in,
                                int64_t i_out, int64_t i_t, int64_t i_e, int64_t add, hipStream_t stream);
 
+/* ---- attention and its surroundings, with the rules of the operators above ------------------
+ * Positions and the offsets of sequences count from 0. */
+
+/* Host only: the angles a position turns each of the i_r / 2 pairs by, in radians: base^(-2 j / i_r), divided by `factor` for
+ * contexts `factor` times as long.  length = 0: all pairs.  length > 0 (the context that the model was trained on): pairs
+ * that turn at most `low` times over it, and none that turns `high` times or more; between them a straight ramp. */
+int32_t stade_hip_rotary_freq(int64_t i_r, double base, double factor, double length, double low, double high, double* freq);
+
+/* x (i_d * (i_q + i_k), i_t): i_q heads of queries, then i_k of keys.  norm != 0: each head by itself becomes
+ * x / sqrt(mean(x^2) + eps) * g, g (i_d) = gq for queries and gk for keys, of type tg: Float32 or x's type; null: 1.  Then the pairs of its first
+ * i_r values (even) turn by pos[t] * freq[j] (Float64[i_r / 2]), and are multiplied by s: pair j is (j, i_r / 2 + j) for half != 0,
+ * else (2 j, 2 j + 1).  i_d <= 256.  y may be x. */
+int32_t stade_hip_head_rotary(int64_t tx, int64_t tg, void* y, int64_t ldy, const void* x, int64_t ldx, const void* gq, const void* gk,
+                              const int64_t* pos, const double* freq, int64_t i_d, int64_t i_q, int64_t i_k, int64_t i_r, int64_t i_t,
+                              int64_t half, int64_t norm, double eps, double s, hipStream_t stream);
+/* its adjoint: xb, gqb and gkb (Float32) from yb and x (x is read with the norm only); xb, gqb and gkb may each be null. */
+int32_t stade_hip_head_rotary_b(int64_t tx, int64_t tg, const void* yb, int64_t ldyb, const void* x, int64_t ldx, void* xb, int64_t ldxb,
+                                const void* gq, float* gqb, const void* gk, float* gkb, const int64_t* pos, const double* freq, int64_t i_d,
+                                int64_t i_q, int64_t i_k, int64_t i_r, int64_t i_t, int64_t half, int64_t norm, double eps, double s,
+                                int64_t add, hipStream_t stream);
+
+/* Attention over i_n sequences: sequence n has the queries qstart[n] <= t < qstart[n + 1] of q (i_d * i_q, i_t) and the keys and
+ * values kstart[n] <= t < kstart[n + 1] of k, v (i_d * i_k, i_tk) (Int64[i_n + 1], in increasing order, on the device).  i_q is a
+ * multiple of i_k: query head h goes with key head h / (i_q / i_k).  The last query stands at the last key; a query at key
+ * p sees the keys i <= p with p - i < window (window < 0: all) or i < sinks.  y = sum of softmax(s q . k) v over what it
+ * sees; lse (i_q, i_t) Float32, if not null: the logarithm of the sum of exp(s q . k), which the adjoint takes.  A query that sees nothing,
+ * and a column of no sequence, gets zeros and -Inf.  A product with keys that are not seen is never formed into the result,
+ * whatever they hold.  Offsets that decrease or lie outside the columns raise the device error flag.  i_d <= 128, sinks <= 64. */
+int32_t stade_hip_attention(int64_t tx, void* y, int64_t ldy, float* lse, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
+                            int64_t ldv, const int64_t* qstart, const int64_t* kstart, double s, int64_t i_d, int64_t i_q, int64_t i_k,
+                            int64_t i_t, int64_t i_tk, int64_t i_n, int64_t window, int64_t sinks, hipStream_t stream);
+/* its adjoint: qb, kb, vb from yb and what the forward call took and gave; each may be null. */
+int32_t stade_hip_attention_b(int64_t tx, const void* yb, int64_t ldyb, const void* y, int64_t ldy, const float* lse, const void* q, int64_t ldq,
+                              void* qb, int64_t ldqb, const void* k, int64_t ldk, void* kb, int64_t ldkb, const void* v, int64_t ldv, void* vb,
+                              int64_t ldvb, const int64_t* qstart, const int64_t* kstart, double s, int64_t i_d, int64_t i_q, int64_t i_k,
+                              int64_t i_t, int64_t i_tk, int64_t i_n, int64_t window, int64_t sinks, int64_t add, hipStream_t stream);
+
+/* Tokens with several experts each: ids (i_k, i_t), slot (k, t)'s expert or 0.  order Int64[i_k * i_t]: the slots' numbers
+ * (from 1) in stable order of their experts, those of none last; place (i_k, i_t): where each slot is in that order, 0 for those of none;
+ * start Int64[i_e + 1]: what stade_hip_expert_mul takes.  i_k <= 64, i_e <= 4096. */
+int32_t stade_hip_expert_order(const int64_t* ids, int64_t* order, int64_t* place, int64_t* start, int64_t i_k, int64_t i_e, int64_t i_t,
+                               hipStream_t stream);
+/* xs[:, place[k, t]] = x[:, t], x (i_d, i_t), xs (i_d, i_k * i_t).  Places are different or 0; columns of xs that none names
+ * stay as they are.  A place outside 0..i_k * i_t is taken as 0 and raises the device error flag, here and below. */
+int32_t stade_hip_expert_take(int64_t tx, void* xs, int64_t ldxs, const void* x, int64_t ldx, const int64_t* place, int64_t i_d, int64_t i_k,
+                              int64_t i_t, hipStream_t stream);
+/* its adjoint: xb[:, t] (+)= sum over k of xsb[:, place[k, t]] */
+int32_t stade_hip_expert_take_b(int64_t tx, const void* xsb, int64_t ldxsb, void* xb, int64_t ldxb, const int64_t* place, int64_t i_d,
+                                int64_t i_k, int64_t i_t, int64_t add, hipStream_t stream);
+/* y[:, t] (+)= sum over k of p[k, t] * ys[:, place[k, t]]; p (i_k, i_t) Float32, null: 1 */
+int32_t stade_hip_expert_join(int64_t tx, void* y, int64_t ldy, const void* ys, int64_t ldys, const float* p, const int64_t* place, int64_t i_d,
+                              int64_t i_k, int64_t i_t, int64_t add, hipStream_t stream);
+/* its adjoint: ysb[:, place[k, t]] (+)= p[k, t] * yb[:, t] (other columns stay as they are) and pb[k, t] (+)= yb[:, t] . ys[:, place[k, t]]
+ * (set: 0 without a place).  ysb and pb may each be null; ys is read for pb only. */
+int32_t stade_hip_expert_join_b(int64_t tx, const void* yb, int64_t ldyb, const void* ys, int64_t ldys, void* ysb, int64_t ldysb, const float* p,
+                                float* pb, const int64_t* place, int64_t i_d, int64_t i_k, int64_t i_t, int64_t add, hipStream_t stream);
+
+/* y = r + m x / (1 - p), matrices (i_d, i_n), r null: 0.  m is 1 where 16 bits that the generator gives for (key[0], key[1],
+ * column, row) are at least round(65536 p), and p stands for that multiple of 2^-16 (below 1); it is the same for every
+ * type, stride and call.  key: Int64[2] on the device (a seed, and a number that tells calls apart).  The generator: Philox 4x32 with 10
+ * rounds, key = key[0], counter = (row / 8, column, key[1]) with rows and columns from 0; its words' halves, low first, serve rows 8 j .. 8 j + 7.
+ * y may be x or r. */
+int32_t stade_hip_dropout(int64_t tx, void* y, int64_t ldy, const void* x, int64_t ldx, const void* r, int64_t ldr, const int64_t* key, double p,
+                          int64_t i_d, int64_t i_n, hipStream_t stream);
+/* its adjoint: xb (+)= m yb / (1 - p) (r's shadow is yb itself) */
+int32_t stade_hip_dropout_b(int64_t tx, const void* yb, int64_t ldyb, void* xb, int64_t ldxb, const int64_t* key, double p, int64_t i_d,
+                            int64_t i_n, int64_t add, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

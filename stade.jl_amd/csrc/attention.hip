@@ -1,0 +1,315 @@
+// Attention over ragged sequences with heads in groups, a sliding window and sinks:
+//   y = sum over the seen keys of softmax(s q . k) v,   lse = log sum exp(s q . k)
+// One pass over the keys with the running maximum m and sum l of a row's exponentials: a tile of keys whose scores go
+// up to m' > m scales what was summed before by exp(m - m').  (The sums are scaled only where some row's maximum grows by
+// more than 8 in the exponent of 2; until then exponentials are up to 2^8, which every type holds.)
+//
+// Scores are formed as K Q^T, keys along the registers: a lane has one query and half of a tile's keys, so
+// maxima and sums are lane by lane and one exchange of the half waves.  Exponentials are rounded to the
+// type (to nearest: like v, they are one factor of a product, whose sum is fp32) and are, as they lie in registers, the other operand of
+// V^T P, whose V^T comes from the row-major tile by the transposing LDS read: they never go through LDS.
+//
+// Two forms.  Wide: four waves of 32 rows each share tiles of 64 keys, double-buffered.  Narrow, for few rows a sequence
+// (single tokens): bound by reading k and v.  A block has 32 rows, its four waves take tiles of 32 keys in turn, each with
+// buffers of its own and no barrier, and a sequence's keys go over several blocks, whose parts a
+// second launch joins in order.
+#include "attention.hpp"
+
+#include <algorithm>
+#include <math.h>
+#include <type_traits>
+
+namespace stade {
+namespace {
+
+using namespace attn;
+
+struct Att {
+    void* y; int64_t ldy;
+    float* lse;
+    const void* q; int64_t ldq;
+    const void* k; int64_t ldk;
+    const void* v; int64_t ldv;
+    Seqs seqs;
+    int d, heads;          // of the keys
+    float s;               // the scores' factor, made positive (`negate`: q's sign is turned)
+    int negate;
+    int64_t slots;         // of rows (wide, and narrow for long sequences)
+    // narrow: slots of keys, `chunk` keys each, or (chunk 0) `parts` of each sequence
+    int64_t key_slots;
+    int chunk, parts;
+    float* part;           // a block's rows: 32 x (d values, m, l)
+};
+
+constexpr int kNarrow = 32;      // rows of a narrow block
+constexpr float kGrow = 8.f;     // of the maximum, in the exponent of 2, before sums are scaled
+
+// a lane's query
+struct Row {
+    bool here;
+    int64_t t;      // column
+    int head;
+    int pos;        // its key
+};
+__device__ __forceinline__ Row row_at(const Seq& q, const Seqs& s, int kvh, int r) {
+    Row w;
+    const int j = r / s.group;
+    w.here = j < q.nq;
+    w.t = q.q0 + j;
+    w.head = kvh * s.group + r - j * s.group;
+    w.pos = w.here ? j + q.shift() : -1;
+    return w;
+}
+
+// The running softmax and the sums of a wave's 32 rows
+template <class T, int DT>
+struct Sums {
+    static constexpr int DP = DT > 2 ? 128 : 64, FR = DT * 32 / (2 * kCE<T>);
+    float m, l;          // of the lane's row: the maximum (raw scores), the lane's share of the sum
+    floatx16 o[DT];      // values 32 i + .. of the head by rows of registers, the row by lane
+    v4u q[FR];
+
+    __device__ __forceinline__ void clear() {
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
+    }
+
+    // a tile of 32 NB keys from `key` on; c = s log2(e)
+    template <int NB>
+    __device__ __forceinline__ void tile(const char* kt, const char* vt, int key, const Seqs& s, int pos, int p0, int p1, float c) {
+        const int lane = threadIdx.x & 63, h = lane >> 5;
+        floatx16 x[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[b][j] = 0.f;
+#pragma unroll
+            for (int f = 0; f < FR; ++f) x[b] = multiply<T>(along_head<T, DP>(kt, 32 * b, f), q[f], x[b]);
+        }
+        // (tiles that every row sees whole need no tests)
+        if (key + 32 * NB - 1 > p0 || (p1 - key >= s.window && key + 32 * NB > s.sinks)) {
+            const int high = pos - key - 4 * h, low = high - s.window, sink = s.sinks - key - 4 * h;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int e = 32 * b + 8 * (j >> 2) + (j & 3);
+                    if (!(e <= high && (e > low || e < sink))) x[b][j] = -INFINITY;
+                }
+        }
+        float top = x[0][0];
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) top = fmaxf(top, x[b][j]);
+        top = fmaxf(top, other_half(top));
+        if (__any((top - m) * c > kGrow)) {   // (m = -Inf, of rows that saw nothing so far, too; NaN: no)
+            const float to = fmaxf(m, top), f = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - to) * c);
+            m = to;
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < DT; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[i][j] *= f;
+        }
+        const float base = m == -INFINITY ? 0.f : -m * c;
+        float sum = 0.f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                x[b][j] = __builtin_amdgcn_exp2f(fmaf(x[b][j], c, base));
+                sum += x[b][j];
+            }
+#pragma unroll
+            for (int u = 0; u < kParts<T>; ++u) {
+                const v4u p = part_of<T>(x[b], u);
+#pragma unroll
+                for (int i = 0; i < DT; ++i) o[i] = multiply<T>(along_rows<T, DP>(vt, 32 * b + u * 2 * kCE<T>, 32 * i), p, o[i]);
+            }
+        }
+        l += sum;
+    }
+};
+
+template <class T>
+__device__ __forceinline__ void negate_all(v4u* f, int n) {
+    const uint32_t bits = sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+    for (int i = 0; i < n; ++i) f[i] ^= bits;
+}
+
+// four consecutive values of the head
+template <class T>
+__device__ __forceinline__ void store4(T* p, float a, float b, float c, float e, int left) {
+    const float v[4] = {a, b, c, e};
+    store_row(p, v, left);
+}
+
+// a wave's finished rows: y and lse
+template <class T, int DT>
+__device__ __forceinline__ void store_rows(const Att& p, const floatx16 (&o)[DT], const Row& w, float m, float l) {
+    if (!w.here) return;
+    const int h = (threadIdx.x & 63) >> 5;
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    T* y = (T*)p.y + w.t * p.ldy + (int64_t)w.head * p.d;
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int col = 32 * i + 8 * g + 4 * h;
+            store4(y + col, o[i][4 * g] * inv, o[i][4 * g + 1] * inv, o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv, p.d - col);
+        }
+    if (p.lse && h == 0) p.lse[w.t * (p.heads * p.seqs.group) + w.head] = l > 0.f || l != l ? m * p.s + kLn2 * __builtin_amdgcn_logf(l) : -INFINITY;
+}
+
+// columns of no sequence: zeros and -Inf
+template <class T>
+__device__ __forceinline__ void store_nothing(const Att& p, const Seq& q, int kvh, int r0, int rows) {
+    for (int r = r0 + threadIdx.x; r < r0 + rows; r += blockDim.x) {
+        const Row w = row_at(q, p.seqs, kvh, r);
+        if (!w.here) continue;
+        for (int i = 0; i < p.d; ++i) ((T*)p.y)[w.t * p.ldy + (int64_t)w.head * p.d + i] = (T)0.f;
+        if (p.lse) p.lse[w.t * (p.heads * p.seqs.group) + w.head] = -INFINITY;
+    }
+}
+
+// a block's place: blocks go round the 8 XCDs, each with an L2 of its own; blocks of one key head
+// go to one XCD, or a key head's blocks go round the XCDs that have it
+__device__ __forceinline__ void place_of(int64_t block, int64_t slots, int heads, int64_t& slot, int& kvh) {
+    if (heads % 8 == 0) {
+        const int64_t in = block >> 3;
+        kvh = (int)(block & 7) + 8 * (int)(in / slots);
+        slot = in % slots;
+    } else if (8 % heads == 0) {
+        kvh = (int)(block % heads);
+        slot = block / heads;
+    } else {
+        kvh = (int)(block / slots);
+        slot = block % slots;
+    }
+}
+
+constexpr int kWideRows = 128, kWideKeys = 64;
+
+template <class T, int DT, bool DIRECT>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void wide_kernel(Att p) {
+    constexpr int DP = DT > 2 ? 128 : 64, BN = kWideKeys, TILE = BN * kRow<T, DP>;
+    using S = Stage<T, DP, BN, 256, DIRECT>;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
+    const Seqs& s = p.seqs;
+    check_offsets(s, blockIdx.x, gridDim.x);
+    int64_t slot, tile;
+    int kvh;
+    place_of(blockIdx.x, p.slots, p.heads, slot, kvh);
+    // (the last tiles of a sequence, which see the most, first)
+    const int j = find_range(s.qstart, s.t, s.group, kWideRows, s.n + 1, slot, tile);
+    const Seq q = sequence(s, j - 1);
+    const int rows = q.nq * s.group;
+    const int tiles = (rows + kWideRows - 1) / kWideRows;
+    if (tile >= tiles) return;
+    const int r0 = uniform((int)(tiles - 1 - tile) * kWideRows);
+    if (!q.real) {
+        store_nothing<T>(p, q, kvh, r0, kWideRows);
+        return;
+    }
+    const int wave = uniform((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    const Row w = row_at(q, s, kvh, r0 + 32 * wave + (lane & 31));
+    const int p0 = r0 / s.group + q.shift(), p1 = min(r0 + kWideRows - 1, rows - 1) / s.group + q.shift();
+    // this wave's rows
+    const int w0 = uniform((r0 + 32 * wave) / s.group + q.shift()), w1 = uniform(min(r0 + 32 * wave + 31, rows - 1) / s.group + q.shift());
+    const bool working = r0 + 32 * wave < rows;
+    Sums<T, DT> sums;
+    sums.clear();
+    row_fragments<T, DT, DIRECT>(sums.q, (const T*)p.q + w.t * p.ldq + (int64_t)w.head * p.d, w.here, p.d);
+    if (p.negate) negate_all<T>(sums.q, sums.FR);
+    const Range range = seen_by(s, p0, p1), mine = seen_by(s, w0, w1);
+    const KeyTiles<BN> keys(range);
+    const T* k = (const T*)p.k + q.k0 * p.ldk + (int64_t)kvh * p.d;
+    const T* v = (const T*)p.v + q.k0 * p.ldv + (int64_t)kvh * p.d;
+    const float c = p.s * kLog2e;
+    typename S::Held hk, hv;
+    auto load = [&](int i, char* at) {
+        const int key = keys.key(i);
+        int from, to;
+        tile_rows<BN>(range, key, from, to);
+        S::load(hk, k + key * p.ldk, p.ldk, p.d, from, to, at, threadIdx.x);
+        S::load(hv, v + key * p.ldv, p.ldv, p.d, from, to, at + TILE, threadIdx.x);
+    };
+    if (keys.count > 0) {
+        load(0, lds);
+        S::store(hk, lds, threadIdx.x);
+        S::store(hv, lds + TILE, threadIdx.x);
+        if constexpr (DIRECT) wait_loads<0>();
+    }
+    __syncthreads();
+    for (int i = 0; i < keys.count; ++i) {
+        char* now = lds + (i & 1) * 2 * TILE;
+        char* next = lds + (~i & 1) * 2 * TILE;
+        if (i + 1 < keys.count) load(i + 1, next);
+        const int key = keys.key(i);
+        // (a wave whose rows see none of the tile leaves it out)
+        if (working && ((key < mine.high && key + BN > mine.low) || key < mine.sinks)) sums.template tile<BN / 32>(now, now + TILE, key, s, w.pos, w0, w1, c);
+        if (i + 1 < keys.count) {
+            S::store(hk, next, threadIdx.x);
+            S::store(hv, next + TILE, threadIdx.x);
+            if constexpr (DIRECT) wait_loads<0>();
+        }
+        __syncthreads();
+    }
+    store_rows<T, DT>(p, sums.o, w, sums.m, sums.l + other_half(sums.l));
+}
+
+int32_t* error_flag(Workspace* ws) { return (int32_t*)(ws->dscalars + kErrFlagSlot); }
+
+template <class F>
+int32_t with_width(int64_t d, F&& f) {
+    if (d <= 64) return f(std::integral_constant<int, 2>{});
+    if (d <= 96) return f(std::integral_constant<int, 3>{});
+    return f(std::integral_constant<int, 4>{});
+}
+
+}  // namespace
+}  // namespace stade
+
+using namespace stade;
+
+extern "C" {
+
+int32_t stade_hip_attention(int64_t tx, void* y, int64_t ldy, float* lse, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
+                            int64_t ldv, const int64_t* qstart, const int64_t* kstart, double s, int64_t i_d, int64_t i_q, int64_t i_k,
+                            int64_t i_t, int64_t i_tk, int64_t i_n, int64_t window, int64_t sinks, hipStream_t stream) {
+    const char* fn = "stade_hip_attention";
+    Seqs seqs;
+    if (int32_t rc = check_attention(fn, tx, s, i_d, i_q, i_k, i_t, i_tk, i_n, window, sinks, qstart, kstart, seqs)) return rc;
+    if (int32_t rc = check_ld(fn, "ldy", ldy, i_d * i_q)) return rc;
+    if (int32_t rc = check_ld(fn, "ldq", ldq, i_d * i_q)) return rc;
+    if (int32_t rc = check_ld(fn, "ldk", ldk, i_d * i_k)) return rc;
+    if (int32_t rc = check_ld(fn, "ldv", ldv, i_d * i_k)) return rc;
+    if (i_d == 0 || i_q == 0 || i_t == 0) return STADE_HIP_OK;
+    if (!y || !q || (i_tk > 0 && (!k || !v))) return bad(fn, "null pointer");
+    WsCall call(stream);
+    if (!call.ok()) return call.error();
+    Att p{y, ldy, lse, q, ldq, k, ldk, v, ldv, seqs, (int)i_d, (int)i_k, (float)fabs(s), s < 0.0};
+    p.seqs.flag = error_flag(call.ws);
+    p.slots = slots_of(i_t, p.seqs.group, kWideRows, i_n + 1);
+    return with_type(tx, [&](auto t) -> int32_t {
+        return with_width(i_d, [&](auto dt) -> int32_t {
+            using T = decltype(t);
+            constexpr int DT = decltype(dt)::value;
+            const int64_t size = sizeof(T);
+            const bool direct = straight(q, ldq, i_d, size) && straight(k, ldk, i_d, size) && straight(v, ldv, i_d, size);
+            STADE_TIMED("attention", stream, {
+                if (direct) wide_kernel<T, DT, true><<<(unsigned)(p.slots * i_k), 256, 0, stream>>>(p);
+                else wide_kernel<T, DT, false><<<(unsigned)(p.slots * i_k), 256, 0, stream>>>(p);
+            });
+            STADE_LAUNCHED("attention wide_kernel");
+            return STADE_HIP_OK;
+        });
+    });
+}
+
+}  // extern "C"

@@ -13,8 +13,8 @@ Julia function it stands for (`<k>_b`, `<k>_d`, `<k>_hv` of stade.jl_amd/corpus/
   the scalar shadows, bare if one, a tuple otherwise; the HVP returns (xb, xbd) pairs);
 * work is enqueued on torch's current stream of the tensors' device.
 
-The operators of language models (`embed`, `token_order`, `tape8_*`, `layernorm`, `expert_mul` and
-their adjoints `<k>_b`) have no generated counterpart.  They follow the same rules, with the
+The operators of language models (`embed`, `token_order`, `tape8_*`, `layernorm`, `expert_mul`,
+`head_rotary`, `attention`, `expert_order`, `expert_take`, `expert_join`, `dropout` and their adjoints `<k>_b`) have no generated counterpart.  They follow the same rules, with the
 primal function and the adjoint as two calls, matrices whose rows may lie apart, the element
 types float32, bfloat16 and float16, and `add=False` to set shadows instead of accumulating.
 
@@ -37,6 +37,8 @@ from .api import (  # noqa: F401
     conv3x3_b, conv3x3_d, conv3x3_hv,
     embed, embed_b, token_order, tape8_lengths, tape8_store, tape8_load,
     layernorm, layernorm_b, expert_mul, expert_mul_b,
+    rotary_freq, head_rotary, head_rotary_b, attention, attention_b,
+    expert_order, expert_take, expert_take_b, expert_join, expert_join_b, dropout, dropout_b,
     rng_normal, rng_uniform, rng_int_range, stable_seed,
 )
 from .emit import stade_hip_file  # noqa: F401

@@ -66,6 +66,17 @@ ENTRY_POINTS: dict[str, str] = {
     "stade_hip_layernorm_b": "ii" + "aiaiaaai" + "aaaaa" + "iii",
     "stade_hip_expert_mul": "i" + "aiaiaa" + "iiiii",
     "stade_hip_expert_mul_b": "ii" + "aiaiaaaiaaa" + "iiiii",
+    "stade_hip_head_rotary": "ii" + "aiaiaaaa" + "iiiiiii" + "ff",
+    "stade_hip_head_rotary_b": "ii" + "aiaiaiaaaaaa" + "iiiiiii" + "ff" + "i",
+    "stade_hip_attention": "i" + "aia" + "aiaiai" + "aa" + "f" + "iiiiiiii",
+    "stade_hip_attention_b": "i" + "aiaia" + "aiaiaiaiaiai" + "aa" + "f" + "iiiiiiiii",
+    "stade_hip_expert_order": "aaaaiii",
+    "stade_hip_expert_take": "i" + "aiaia" + "iii",
+    "stade_hip_expert_take_b": "i" + "aiaia" + "iiii",
+    "stade_hip_expert_join": "i" + "aiaiaa" + "iiii",
+    "stade_hip_expert_join_b": "i" + "aiaiaiaaa" + "iiii",
+    "stade_hip_dropout": "i" + "aiaiaia" + "f" + "ii",
+    "stade_hip_dropout_b": "i" + "aiaia" + "f" + "iii",
 }
 
 _CT = {"a": P, "i": I64, "f": F64, "r": F64P}
@@ -766,3 +777,199 @@ def expert_mul_b(yb, x, xb, w, wb, start, i_in, i_out, i_t, i_e, add=True, tape=
     _call("stade_hip_expert_mul_b", a, _stream_of(yb))
     if check:
         _flag("expert_mul_b", "start decreases or lies outside 0..i_t")
+
+
+# ------------------------------------------------------------------------------------------
+# attention and its surroundings: positions, ragged attention, several experts a token, dropout
+# ------------------------------------------------------------------------------------------
+
+def rotary_freq(i_r, base=10000.0, factor=1.0, length=0.0, low=1.0, high=32.0) -> np.ndarray:
+    """The angles (radians, Float64[i_r / 2], on the host) that a position turns head_rotary's pairs by: base^(-2 j / i_r), divided by
+    `factor` for contexts `factor` times as long.  With `length`, the context that the model was trained on, only pairs that turn at
+    most `low` times over it are divided, none that turns `high` times or more, and those between by a straight ramp."""
+    r = _nat("i_r", i_r)
+    out = np.empty(r // 2, dtype=np.float64)
+    L = lib()
+    L.stade_hip_rotary_freq.argtypes = [I64] + [F64] * 5 + [P]
+    L.stade_hip_rotary_freq.restype = ctypes.c_int32
+    _check("stade_hip_rotary_freq", L.stade_hip_rotary_freq(r, float(base), float(factor), float(length), float(low), float(high), out.ctypes.data))
+    return out
+
+
+def _head_weights(gq, gk, x, d: int):
+    """(type code, gq pointer, gk pointer): both Float32, or both of x's type."""
+    some = gq if gq is not None else gk
+    if some is None:
+        return 0, None, None
+    return _code("g", some), _opt("gq", gq, some.dtype, d), _opt("gk", gk, some.dtype, d)
+
+
+def head_rotary(y, x, gq, gk, pos, freq, i_d, i_q, i_k, i_r, i_t, norm=True, eps=1e-6, half=True, s=1.0):
+    """x (i_d * (i_q + i_k), i_t), i_q heads of queries and then i_k of keys.  Each head by itself: divided by sqrt(mean(x^2) + eps)
+    and multiplied by gq (gk for keys; Float32 or x's type; None: 1), without norm as it is; then the pairs of its first i_r values turned by
+    pos[t] * freq[j] (Int64[i_t], Float64[i_r / 2], see rotary_freq) and multiplied by s.  half: pair j is values j and i_r / 2 + j, else
+    2 j and 2 j + 1 (from 0).  y may be x."""
+    import torch
+    d, hq, hk, r, t = _nat("i_d", i_d), _nat("i_q", i_q), _nat("i_k", i_k), _nat("i_r", i_r), _nat("i_t", i_t)
+    w = d * (hq + hk)
+    tx = _code("x", x)
+    (yp, ldy), (xp, ldx) = _mat("y", y, w, t, x.dtype), _mat("x", x, w, t)
+    tg, gqp, gkp = _head_weights(gq, gk, x, d)
+    a = [tx, tg, yp, ldy, xp, ldx, gqp, gkp, _arr("pos", pos, torch.int64, t) if r else None, _arr("freq", freq, torch.float64, r // 2) if r else None,
+         d, hq, hk, r, t, int(bool(half)), int(bool(norm)), float(eps), float(s)]
+    _one_device(y, x, gq, gk, *((pos, freq) if r else ()))
+    _call("stade_hip_head_rotary", a, _stream_of(x))
+
+
+def head_rotary_b(yb, x, xb, gq, gqb, gk, gkb, pos, freq, i_d, i_q, i_k, i_r, i_t, norm=True, eps=1e-6, half=True, s=1.0, add=True):
+    """Adjoint of head_rotary from its output's shadow yb and, with the norm, its input x (else None): xb, gqb and gkb are
+    accumulated (add=False: set).  gqb, gkb Float32; xb, gqb and gkb may be None."""
+    import torch
+    d, hq, hk, r, t = _nat("i_d", i_d), _nat("i_q", i_q), _nat("i_k", i_k), _nat("i_r", i_r), _nat("i_t", i_t)
+    w = d * (hq + hk)
+    tx = _code("yb", yb)
+    yp, ldy = _mat("yb", yb, w, t)
+    xp, ldx = _mat("x", x, w, t, yb.dtype) if x is not None else (None, w)
+    xbp, ldxb = _mat("xb", xb, w, t, yb.dtype) if xb is not None else (None, w)
+    tg, gqp, gkp = _head_weights(gq, gk, yb, d)
+    a = [tx, tg, yp, ldy, xp, ldx, xbp, ldxb, gqp, _opt("gqb", gqb, torch.float32, d), gkp, _opt("gkb", gkb, torch.float32, d),
+         _arr("pos", pos, torch.int64, t) if r else None, _arr("freq", freq, torch.float64, r // 2) if r else None,
+         d, hq, hk, r, t, int(bool(half)), int(bool(norm)), float(eps), float(s), int(bool(add))]
+    _one_device(yb, x, xb, gq, gqb, gk, gkb, *((pos, freq) if r else ()))
+    _call("stade_hip_head_rotary_b", a, _stream_of(yb))
+
+
+def _attention_sizes(i_d, i_q, i_k, i_t, i_tk, i_n, window, sinks):
+    sizes = [_nat(n, v) for n, v in (("i_d", i_d), ("i_q", i_q), ("i_k", i_k), ("i_t", i_t), ("i_tk", i_tk), ("i_n", i_n))]
+    return sizes + [-1 if window is None else _nat("window", window), _nat("sinks", sinks)]
+
+
+def attention(y, lse, q, k, v, qstart, kstart, s, i_d, i_q, i_k, i_t, i_tk, i_n, window=None, sinks=0, check=False):
+    """y = softmax(s q . k) v over i_n sequences, with the queries qstart[n] <= t < qstart[n + 1] of q (i_d * i_q, i_t) and the keys
+    kstart[n] <= t < kstart[n + 1] of k, v (i_d * i_k, i_tk) (Int64[i_n + 1], increasing).  Query head h goes with key head h // (i_q / i_k).  A
+    sequence's last query stands at its last key; a query at key p sees the keys i <= p with p - i < window (None: all) or
+    i < sinks.  lse (i_q, i_t) Float32: the logarithms of the sums, for the adjoint (None: not kept).  A query that sees nothing
+    and a column of no sequence get 0 and -Inf.  check=True raises StadeHipBoundsError for offsets that decrease or lie outside
+    the columns (one synchronisation)."""
+    import torch
+    d, hq, hk, t, tk, n, w, sk = sizes = _attention_sizes(i_d, i_q, i_k, i_t, i_tk, i_n, window, sinks)
+    tx = _code("q", q)
+    (yp, ldy), (qp, ldq) = _mat("y", y, d * hq, t, q.dtype), _mat("q", q, d * hq, t)
+    (kp, ldk), (vp, ldv) = _mat("k", k, d * hk, tk, q.dtype), _mat("v", v, d * hk, tk, q.dtype)
+    a = [tx, yp, ldy, _opt("lse", lse, torch.float32, hq * t), qp, ldq, kp, ldk, vp, ldv, _arr("qstart", qstart, torch.int64, n + 1),
+         _arr("kstart", kstart, torch.int64, n + 1), float(s), *sizes]
+    _one_device(y, lse, q, k, v, qstart, kstart)
+    _call("stade_hip_attention", a, _stream_of(q))
+    if check:
+        _flag("attention", "offsets of the sequences decrease or lie outside the columns")
+
+
+def attention_b(yb, y, lse, q, qb, k, kb, v, vb, qstart, kstart, s, i_d, i_q, i_k, i_t, i_tk, i_n, window=None, sinks=0, add=True, check=False):
+    """Adjoint of attention: qb, kb and vb from yb and what the forward call took and gave (y, lse); accumulated (add=False: set).
+    Each may be None.  By sums in fixed order: the same call gives the same bits."""
+    import torch
+    d, hq, hk, t, tk, n, w, sk = sizes = _attention_sizes(i_d, i_q, i_k, i_t, i_tk, i_n, window, sinks)
+    tx = _code("yb", yb)
+
+    def mat(name, m, heads, cols):
+        return _mat(name, m, d * heads, cols, yb.dtype) if m is not None else (None, d * heads)
+
+    a = [tx, *mat("yb", yb, hq, t), *mat("y", y, hq, t), _arr("lse", lse, torch.float32, hq * t), *mat("q", q, hq, t), *mat("qb", qb, hq, t),
+         *mat("k", k, hk, tk), *mat("kb", kb, hk, tk), *mat("v", v, hk, tk), *mat("vb", vb, hk, tk), _arr("qstart", qstart, torch.int64, n + 1),
+         _arr("kstart", kstart, torch.int64, n + 1), float(s), *sizes, int(bool(add))]
+    _one_device(yb, y, lse, q, qb, k, kb, v, vb, qstart, kstart)
+    _call("stade_hip_attention_b", a, _stream_of(yb))
+    if check:
+        _flag("attention_b", "offsets of the sequences decrease or lie outside the columns")
+
+
+def expert_order(ids, order, place, start, i_k, i_e, i_t, check=False):
+    """ids (i_k, i_t) Int64, the experts 1..i_e of each token's i_k slots (0: none).  order (Int64[i_k * i_t]): the slots' numbers (from 1) in
+    stable order of their experts, those of none last; place (i_k, i_t): where each slot is in that order, 0 for those of none; start (Int64[i_e + 1]):
+    the `start` of expert_mul.  check=True raises StadeHipBoundsError for any other id, which is taken as 0 (one synchronisation)."""
+    import torch
+    k, e, t = _nat("i_k", i_k), _nat("i_e", i_e), _nat("i_t", i_t)
+    a = [_arr("ids", ids, torch.int64, k * t), _arr("order", order, torch.int64, k * t), _arr("place", place, torch.int64, k * t),
+         _arr("start", start, torch.int64, e + 1), k, e, t]
+    _one_device(ids, order, place, start)
+    _call("stade_hip_expert_order", a, _stream_of(ids))
+    if check:
+        _flag("expert_order", "an id is outside 0..i_e")
+
+
+def expert_take(xs, x, place, i_d, i_k, i_t, check=False):
+    """xs[:, place[k, t]] = x[:, t] for x (i_d, i_t) and xs (i_d, i_k * i_t): the rows that expert_mul takes.  Columns of xs that no
+    place names stay as they are.  check=True raises StadeHipBoundsError for a place outside 0..i_k * i_t (one synchronisation)."""
+    import torch
+    d, k, t = _nat("i_d", i_d), _nat("i_k", i_k), _nat("i_t", i_t)
+    tx = _code("x", x)
+    a = [tx, *_mat("xs", xs, d, k * t, x.dtype), *_mat("x", x, d, t), _arr("place", place, torch.int64, k * t), d, k, t]
+    _one_device(xs, x, place)
+    _call("stade_hip_expert_take", a, _stream_of(x))
+    if check:
+        _flag("expert_take", "a place is outside 0..i_k * i_t")
+
+
+def expert_take_b(xsb, xb, place, i_d, i_k, i_t, add=True, check=False):
+    """Adjoint of expert_take: xb[:, t] += the sum over k of xsb[:, place[k, t]] (add=False: set)."""
+    import torch
+    d, k, t = _nat("i_d", i_d), _nat("i_k", i_k), _nat("i_t", i_t)
+    tx = _code("xsb", xsb)
+    a = [tx, *_mat("xsb", xsb, d, k * t), *_mat("xb", xb, d, t, xsb.dtype), _arr("place", place, torch.int64, k * t), d, k, t, int(bool(add))]
+    _one_device(xsb, xb, place)
+    _call("stade_hip_expert_take_b", a, _stream_of(xsb))
+    if check:
+        _flag("expert_take_b", "a place is outside 0..i_k * i_t")
+
+
+def expert_join(y, ys, p, place, i_d, i_k, i_t, add=False, check=False):
+    """y[:, t] = the sum over k of p[k, t] * ys[:, place[k, t]] (add=True: accumulated) for ys (i_d, i_k * i_t), what expert_mul gave, and
+    the weights p (i_k, i_t) Float32 (None: 1)."""
+    import torch
+    d, k, t = _nat("i_d", i_d), _nat("i_k", i_k), _nat("i_t", i_t)
+    tx = _code("ys", ys)
+    a = [tx, *_mat("y", y, d, t, ys.dtype), *_mat("ys", ys, d, k * t), _opt("p", p, torch.float32, k * t), _arr("place", place, torch.int64, k * t),
+         d, k, t, int(bool(add))]
+    _one_device(y, ys, p, place)
+    _call("stade_hip_expert_join", a, _stream_of(ys))
+    if check:
+        _flag("expert_join", "a place is outside 0..i_k * i_t")
+
+
+def expert_join_b(yb, ys, ysb, p, pb, place, i_d, i_k, i_t, add=True, check=False):
+    """Adjoint of expert_join: ysb[:, place[k, t]] += p[k, t] * yb[:, t] and pb[k, t] += yb[:, t] . ys[:, place[k, t]] (add=False: set;
+    columns of ysb that no place names stay as they are).  ysb and pb may be None; ys is read for pb only."""
+    import torch
+    d, k, t = _nat("i_d", i_d), _nat("i_k", i_k), _nat("i_t", i_t)
+    tx = _code("yb", yb)
+    ysp, ldys = _mat("ys", ys, d, k * t, yb.dtype) if ys is not None else (None, d)
+    ysbp, ldysb = _mat("ysb", ysb, d, k * t, yb.dtype) if ysb is not None else (None, d)
+    a = [tx, *_mat("yb", yb, d, t), ysp, ldys, ysbp, ldysb, _opt("p", p, torch.float32, k * t), _opt("pb", pb, torch.float32, k * t),
+         _arr("place", place, torch.int64, k * t), d, k, t, int(bool(add))]
+    _one_device(yb, ys, ysb, p, pb, place)
+    _call("stade_hip_expert_join_b", a, _stream_of(yb))
+    if check:
+        _flag("expert_join_b", "a place is outside 0..i_k * i_t")
+
+
+def dropout(y, x, r, key, p, i_d, i_n):
+    """y = r + m x / (1 - p) for matrices (i_d, i_n) (r None: 0), with the mask m a function of key (Int64[2] on the device: a seed, and
+    a number that tells calls apart) and of the value's row and column alone: the adjoint forms it again.  p counts in steps of
+    2^-16.  y may be x or r."""
+    import torch
+    d, n = _nat("i_d", i_d), _nat("i_n", i_n)
+    tx = _code("x", x)
+    rp, ldr = _mat("r", r, d, n, x.dtype) if r is not None else (None, d)
+    a = [tx, *_mat("y", y, d, n, x.dtype), *_mat("x", x, d, n), rp, ldr, _arr("key", key, torch.int64, 2), float(p), d, n]
+    _one_device(y, x, r, key)
+    _call("stade_hip_dropout", a, _stream_of(x))
+
+
+def dropout_b(yb, xb, key, p, i_d, i_n, add=True):
+    """Adjoint of dropout: xb += m yb / (1 - p) (add=False: set).  The shadow of r is yb itself."""
+    import torch
+    d, n = _nat("i_d", i_d), _nat("i_n", i_n)
+    tx = _code("yb", yb)
+    a = [tx, *_mat("yb", yb, d, n), *_mat("xb", xb, d, n, yb.dtype), _arr("key", key, torch.int64, 2), float(p), d, n, int(bool(add))]
+    _one_device(yb, xb, key)
+    _call("stade_hip_dropout_b", a, _stream_of(yb))
