@@ -154,7 +154,7 @@ template <class T, int DT>
 __device__ __forceinline__ void store_rows(const Att& p, const floatx16 (&o)[DT], const Row& w, float m, float l) {
     if (!w.here) return;
     const int h = (threadIdx.x & 63) >> 5;
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    const float inv = l > 0.f ? 1.f / l : 0.f;
     T* y = (T*)p.y + w.t * p.ldy + (int64_t)w.head * p.d;
 #pragma unroll
     for (int i = 0; i < DT; ++i)
@@ -163,7 +163,36 @@ __device__ __forceinline__ void store_rows(const Att& p, const floatx16 (&o)[DT]
             const int col = 32 * i + 8 * g + 4 * h;
             store4(y + col, o[i][4 * g] * inv, o[i][4 * g + 1] * inv, o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv, p.d - col);
         }
-    if (p.lse && h == 0) p.lse[w.t * (p.heads * p.seqs.group) + w.head] = l > 0.f || l != l ? m * p.s + kLn2 * __builtin_amdgcn_logf(l) : -INFINITY;
+    if (p.lse && h == 0) p.lse[w.t * (p.heads * p.seqs.group) + w.head] = l > 0.f ? m * p.s + kLn2 * __builtin_amdgcn_logf(l) : -INFINITY;
+}
+
+// One row after the other, from the keys of [from, to) that it sees: done(row, m, l, its two values of the sum).
+template <class T, class F>
+__device__ __forceinline__ void exact_rows(const Att& p, const Seq& q, int kvh, int r0, int from, int to, F&& done) {
+    const float s = p.negate ? -p.s : p.s;
+    for (int r = r0; r < r0 + 32; ++r) {
+        const Row w = row_at(q, p.seqs, kvh, r);
+        if (!w.here) break;
+        const Range range = seen_by(p.seqs, w.pos, w.pos);
+        const Two x = load_two((const T*)p.q + w.t * p.ldq + (int64_t)w.head * p.d, p.d);
+        float m = -INFINITY, l = 0.f;
+        Two o{0.f, 0.f};
+        for (int part = 0; part < 2; ++part) {
+            const int end = min(part ? range.high : range.sinks, to);
+            for (int i = max(part ? range.low : 0, from); i < end; ++i) {
+                const Two k = load_two((const T*)p.k + (q.k0 + i) * p.ldk + (int64_t)kvh * p.d, p.d);
+                const Two v = load_two((const T*)p.v + (q.k0 + i) * p.ldv + (int64_t)kvh * p.d, p.d);
+                const float score = dot(x, k) * s;
+                if (score == -INFINITY) continue;
+                const float top = fmaxf(m, score), f = m == -INFINITY ? 0.f : exp2f((m - top) * kLog2e), e = exp2f((score - top) * kLog2e);
+                m = top;
+                l = fmaf(l, f, e);
+                o.a = fmaf(o.a, f, e * v.a);
+                o.b = fmaf(o.b, f, e * v.b);
+            }
+        }
+        done(w, m, l, o);
+    }
 }
 
 // columns of no sequence: zeros and -Inf
@@ -260,7 +289,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void wide_kernel(Att p
         }
         __syncthreads();
     }
-    store_rows<T, DT>(p, sums.o, w, sums.m, sums.l + other_half(sums.l));
+    const float l = sums.l + other_half(sums.l);
+    if (any_not_finite<DT>(sums.o)) {
+        exact_rows<T>(p, q, kvh, r0 + 32 * wave, 0, q.nk, [&](const Row& x, float m, float sum, Two o) {
+            const float inv = 1.f / sum;
+            store_two((T*)p.y + x.t * p.ldy + (int64_t)x.head * p.d, o.a * inv, o.b * inv, p.d, false);
+            if (p.lse && lane == 0) p.lse[x.t * (p.heads * s.group) + x.head] = m + logf(sum);
+        });
+        return;
+    }
+    store_rows<T, DT>(p, sums.o, w, sums.m, l);
 }
 
 int32_t* error_flag(Workspace* ws) { return (int32_t*)(ws->dscalars + kErrFlagSlot); }

@@ -284,6 +284,37 @@ __device__ __forceinline__ v4u part_of(const floatx16& v, int u) {
     return __builtin_bit_cast(v4u, p);
 }
 
+// ------------------------------------------------------------------------------------------
+// values that are not finite
+// ------------------------------------------------------------------------------------------
+// A tile's product multiplies what a row does not see by zero, which infinities and NaN do not mind.  So a wave whose sums
+// are not all finite forms them again one row (or key) after the other, from what is seen alone: a lane has two
+// values of the head.  That is slow (some 500 cycles a pair) and costs nothing where all values are finite but the look at the sums.
+template <int DT>
+__device__ __forceinline__ bool any_not_finite(const floatx16 (&o)[DT]) {
+    float z = 0.f;
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) z = fmaf(o[i][j], 0.f, z);
+    return __any(z != 0.f);
+}
+struct Two {
+    float a, b;
+};
+template <class T>
+__device__ __forceinline__ Two load_two(const T* row, int d) {
+    const int lane = threadIdx.x & 63;
+    return Two{lane < d ? (float)row[lane] : 0.f, lane + 64 < d ? (float)row[lane + 64] : 0.f};
+}
+__device__ __forceinline__ float dot(Two x, Two y) { return wave_sum(fmaf(x.a, y.a, x.b * y.b)); }
+template <class T>
+__device__ __forceinline__ void store_two(T* row, float a, float b, int d, bool add) {
+    const int lane = threadIdx.x & 63;
+    if (lane < d) row[lane] = (T)(add ? (float)row[lane] + a : a);
+    if (lane + 64 < d) row[lane + 64] = (T)(add ? (float)row[lane + 64] + b : b);
+}
+
 // a row's fragments along the head from memory: one row a lane (its half's chunks), zeros past d
 template <class T, int DT, bool DIRECT>
 __device__ __forceinline__ void row_fragments(v4u (&f)[DT * 32 / (2 * kCE<T>)], const T* row, bool here, int d) {

@@ -182,6 +182,28 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void rows_kernel(Back 
         }
         __syncthreads();
     }
+    if (any_not_finite<DT>(acc)) {
+        for (int i = 0; i < 32; ++i) {
+            const int ri = r0 + 32 * wave + i, ji = ri / s.group, hi = kvh * s.group + ri - ji * s.group;
+            if (ji >= q.nq) break;
+            const Range seen = seen_by(s, ji + q.shift(), ji + q.shift());
+            const int64_t ti = q.q0 + ji, ci = (int64_t)hi * p.d, at = ti * (p.heads * s.group) + hi;
+            const Two x = load_two((const T*)p.q + ti * p.ldq + ci, p.d), g = load_two((const T*)p.yb + ti * p.ldyb + ci, p.d);
+            const float li = p.lse[at], di = dot(g, load_two((const T*)p.y + ti * p.ldy + ci, p.d));
+            float a = 0.f, b = 0.f;
+            for (int part = 0; part < 2; ++part) {
+                const int end = part ? seen.high : seen.sinks;
+                for (int n = part ? seen.low : 0; n < end; ++n) {
+                    const Two kn = load_two(k + n * p.ldk, p.d), vn = load_two(v + n * p.ldv, p.d);
+                    const float w = exp2f((dot(x, kn) * p.s - li) * kLog2e) * (dot(g, vn) - di);
+                    a = fmaf(w, kn.a, a);
+                    b = fmaf(w, kn.b, b);
+                }
+            }
+            store_two((T*)p.qb + ti * p.ldqb + ci, a * p.s, b * p.s, p.d, p.add);
+        }
+        return;
+    }
     if (!here) return;
     T* out = (T*)p.qb + t * p.ldqb + col;
 #pragma unroll
@@ -338,7 +360,7 @@ __global__ __launch_bounds__(256 * kHalves<T>, kHalves<T>) void keys_kernel(Back
                 for (int e = 0; e < 16; ++e) {
                     const uint32_t xo = rem + 8 * (e >> 2) + (e & 3), jo = s.group == 1 ? xo : __umulhi(xo, p.magic);
                     const int pos = jq + (int)jo + shift;
-                    if (!(key <= pos && (pos - key < s.window || key < s.sinks))) x[e] = 0.f;
+                    if (!(key <= pos && (pos - key < s.window || key < s.sinks))) x[e] = g[e] = 0.f;
                 }
             }
 #pragma unroll
@@ -362,6 +384,36 @@ __global__ __launch_bounds__(256 * kHalves<T>, kHalves<T>) void keys_kernel(Back
         }
         if (i + 1 < tiles) keep(i + 1, next);
         __syncthreads();
+    }
+    if (working && (any_not_finite<DT>(ka) || any_not_finite<DT>(va))) {
+        for (int n = 0; n < 32 && own + n < keys; ++n) {
+            const int key = own + n;
+            const Two kn = load_two((const T*)p.k + (k_first + key) * p.ldk + hcol, p.d), vn = load_two((const T*)p.v + (k_first + key) * p.ldv + hcol, p.d);
+            Two a{0.f, 0.f}, b{0.f, 0.f};
+            for (int r = r_first + 32 * half; r < r_end; r += (r - r_first) % 32 == 31 ? BM - 31 : 1) {
+                const int ji = r / s.group, hi = kvh * s.group + r - ji * s.group, pos = ji + shift;
+                if (!(key <= pos && (pos - key < s.window || key < s.sinks))) continue;
+                const int64_t ti = q.q0 + ji, ci = (int64_t)hi * p.d, at = ti * heads + hi;
+                const Two x = load_two((const T*)p.q + ti * p.ldq + ci, p.d), g = load_two((const T*)p.yb + ti * p.ldyb + ci, p.d);
+                const float w = exp2f((dot(x, kn) * p.s - p.lse[at]) * kLog2e), ds = w * (dot(g, vn) - p.delta[at]);
+                a.a = fmaf(ds, x.a, a.a);
+                a.b = fmaf(ds, x.b, a.b);
+                b.a = fmaf(w, g.a, b.a);
+                b.b = fmaf(w, g.b, b.b);
+            }
+            // to where the sums of products have them
+#pragma unroll
+            for (int m = 0; m < DT; ++m)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int from = (32 * m + 8 * (e >> 2) + 4 * h + (e & 3)) & 63;
+                    const float x = __shfl(m < 2 ? a.a : a.b, from, 64), y = __shfl(m < 2 ? b.a : b.b, from, 64);
+                    if ((lane & 31) == n) {
+                        ka[m][e] = x;
+                        va[m][e] = y;
+                    }
+                }
+        }
     }
     if constexpr (HALVES > 1) {   // the second half's sums, one array after the other
         static_assert(4 * DT * 4096 <= 2 * BUF, "the sums fit the tiles' memory");
