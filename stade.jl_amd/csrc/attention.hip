@@ -51,7 +51,7 @@ struct Row {
     int head;
     int pos;        // its key
 };
-__device__ __forceinline__ Row row_at(const Seq& q, const Seqs& s, int kvh, int r) {
+__device__ __forceinline__ Row head_row(const Seq& q, const Seqs& s, int kvh, int r) {
     Row w;
     const int j = r / s.group;
     w.here = j < q.nq;
@@ -62,9 +62,10 @@ __device__ __forceinline__ Row row_at(const Seq& q, const Seqs& s, int kvh, int 
 }
 
 // The running softmax and the sums of a wave's 32 rows
-template <class T, int DT>
+template <class T, int DT, int NB>
 struct Sums {
     static constexpr int DP = DT > 2 ? 128 : 64, FR = DT * 32 / (2 * kCE<T>);
+    struct Scores { floatx16 x[NB]; };   // of 32 NB keys
     float m, l;          // of the lane's row: the maximum (raw scores), the lane's share of the sum
     floatx16 o[DT];      // values 32 i + .. of the head by rows of registers, the row by lane
     v4u q[FR];
@@ -78,34 +79,37 @@ struct Sums {
             for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
     }
 
-    // a tile of 32 NB keys from `key` on; c = s log2(e)
-    template <int NB>
-    __device__ __forceinline__ void tile(const char* kt, const char* vt, int key, const Seqs& s, int pos, int p0, int p1, float c) {
-        const int lane = threadIdx.x & 63, h = lane >> 5;
-        floatx16 x[NB];
+    __device__ __forceinline__ void scores(Scores& s, const char* kt) const {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) x[b][j] = 0.f;
+            for (int j = 0; j < 16; ++j) s.x[b][j] = 0.f;
 #pragma unroll
-            for (int f = 0; f < FR; ++f) x[b] = multiply<T>(along_head<T, DP>(kt, 32 * b, f), q[f], x[b]);
+            for (int f = 0; f < FR; ++f) s.x[b] = multiply<T>(along_head<T, DP>(kt, 32 * b, f), q[f], s.x[b]);
         }
-        // (tiles that every row sees whole need no tests)
-        if (key + 32 * NB - 1 > p0 || (p1 - key >= s.window && key + 32 * NB > s.sinks)) {
-            const int high = pos - key - 4 * h, low = high - s.window, sink = s.sinks - key - 4 * h;
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int e = 32 * b + 8 * (j >> 2) + (j & 3);
-                    if (!(e <= high && (e > low || e < sink))) x[b][j] = -INFINITY;
-                }
-        }
-        float top = x[0][0];
+    }
+
+    // what the row at `pos` does not see of the keys from `key` on; p0, p1: the positions of all rows (tiles that every row
+    // sees whole need no tests)
+    __device__ __forceinline__ void hide(Scores& v, int key, const Seqs& s, int pos, int p0, int p1) const {
+        if (!(key + 32 * NB - 1 > p0 || (p1 - key >= s.window && key + 32 * NB > s.sinks))) return;
+        const int h = (threadIdx.x & 63) >> 5, high = pos - key - 4 * h, low = high - s.window, sink = s.sinks - key - 4 * h;
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) top = fmaxf(top, x[b][j]);
+            for (int j = 0; j < 16; ++j) {
+                const int e = 32 * b + 8 * (j >> 2) + (j & 3);
+                if (!(e <= high && (e > low || e < sink))) v.x[b][j] = -INFINITY;
+            }
+    }
+
+    // the maximum with these scores; c = s log2(e)
+    __device__ __forceinline__ void raise(const Scores& s, float c) {
+        float top = s.x[0][0];
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) top = fmaxf(top, s.x[b][j]);
         top = fmaxf(top, other_half(top));
         if (__any((top - m) * c > kGrow)) {   // (m = -Inf, of rows that saw nothing so far, too; NaN: no)
             const float to = fmaxf(m, top), f = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - to) * c);
@@ -116,18 +120,41 @@ struct Sums {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) o[i][j] *= f;
         }
+    }
+
+    // the order of scores() and add() together, as the compiler is to issue them
+    static __device__ __forceinline__ void order() {
+        ORDER(kRead, 4);
+        ORDER(kValu, 6);
+        ORDER(kTrans, 2);
+        static_for<NB * FR>([&](auto i) INLINE {
+            ORDER(kMfma, 1);
+            ORDER(kRead, decltype(i)::value + 4 < NB * FR ? 1 : 2);
+            ORDER(kValu, 3);
+            ORDER(kTrans, 2);
+            ORDER(kValu, 2);
+        });
+        static_for<NB * kParts<T> * DT>([&](auto) INLINE {
+            ORDER(kMfma, 1);
+            ORDER(kRead, 2);
+            ORDER(kValu, 2);
+        });
+    }
+
+    // the scores' weights, and the values by them
+    __device__ __forceinline__ void add(Scores& s, const char* vt, float c) {
         const float base = m == -INFINITY ? 0.f : -m * c;
         float sum = 0.f;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-                x[b][j] = __builtin_amdgcn_exp2f(fmaf(x[b][j], c, base));
-                sum += x[b][j];
+                s.x[b][j] = __builtin_amdgcn_exp2f(fmaf(s.x[b][j], c, base));
+                sum += s.x[b][j];
             }
 #pragma unroll
             for (int u = 0; u < kParts<T>; ++u) {
-                const v4u p = part_of<T>(x[b], u);
+                const v4u p = part_of<T>(s.x[b], u);
 #pragma unroll
                 for (int i = 0; i < DT; ++i) o[i] = multiply<T>(along_rows<T, DP>(vt, 32 * b + u * 2 * kCE<T>, 32 * i), p, o[i]);
             }
@@ -171,7 +198,7 @@ template <class T, class F>
 __device__ __forceinline__ void exact_rows(const Att& p, const Seq& q, int kvh, int r0, int from, int to, F&& done) {
     const float s = p.negate ? -p.s : p.s;
     for (int r = r0; r < r0 + 32; ++r) {
-        const Row w = row_at(q, p.seqs, kvh, r);
+        const Row w = head_row(q, p.seqs, kvh, r);
         if (!w.here) break;
         const Range range = seen_by(p.seqs, w.pos, w.pos);
         const Two x = load_two((const T*)p.q + w.t * p.ldq + (int64_t)w.head * p.d, p.d);
@@ -199,7 +226,7 @@ __device__ __forceinline__ void exact_rows(const Att& p, const Seq& q, int kvh, 
 template <class T>
 __device__ __forceinline__ void store_nothing(const Att& p, const Seq& q, int kvh, int r0, int rows) {
     for (int r = r0 + threadIdx.x; r < r0 + rows; r += blockDim.x) {
-        const Row w = row_at(q, p.seqs, kvh, r);
+        const Row w = head_row(q, p.seqs, kvh, r);
         if (!w.here) continue;
         for (int i = 0; i < p.d; ++i) ((T*)p.y)[w.t * p.ldy + (int64_t)w.head * p.d + i] = (T)0.f;
         if (p.lse) p.lse[w.t * (p.heads * p.seqs.group) + w.head] = -INFINITY;
@@ -226,9 +253,10 @@ constexpr int kWideRows = 128, kWideKeys = 64;
 
 template <class T, int DT, bool DIRECT>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void wide_kernel(Att p) {
-    constexpr int DP = DT > 2 ? 128 : 64, BN = kWideKeys, TILE = BN * kRow<T, DP>;
+    constexpr int DP = DT > 2 ? 128 : 64, BN = kWideKeys, TILE = kTile<T, DP, BN>;
     using S = Stage<T, DP, BN, 256, DIRECT>;
-    __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
+    using R = Sums<T, DT, BN / 32>;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];   // two tiles of keys, two of values
     const Seqs& s = p.seqs;
     check_offsets(s, blockIdx.x, gridDim.x);
     int64_t slot, tile;
@@ -246,52 +274,70 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void wide_kernel(Att p
         return;
     }
     const int wave = uniform((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
-    const Row w = row_at(q, s, kvh, r0 + 32 * wave + (lane & 31));
+    const Row w = head_row(q, s, kvh, r0 + 32 * wave + (lane & 31));
     const int p0 = r0 / s.group + q.shift(), p1 = min(r0 + kWideRows - 1, rows - 1) / s.group + q.shift();
     // this wave's rows
     const int w0 = uniform((r0 + 32 * wave) / s.group + q.shift()), w1 = uniform(min(r0 + 32 * wave + 31, rows - 1) / s.group + q.shift());
     const bool working = r0 + 32 * wave < rows;
-    Sums<T, DT> sums;
+    R sums;
     sums.clear();
     row_fragments<T, DT, DIRECT>(sums.q, (const T*)p.q + w.t * p.ldq + (int64_t)w.head * p.d, w.here, p.d);
     if (p.negate) negate_all<T>(sums.q, sums.FR);
-    const Range range = seen_by(s, p0, p1), mine = seen_by(s, w0, w1);
+    const Range range = seen_by(s, p0, p1);
     const KeyTiles<BN> keys(range);
     const T* k = (const T*)p.k + q.k0 * p.ldk + (int64_t)kvh * p.d;
     const T* v = (const T*)p.v + q.k0 * p.ldv + (int64_t)kvh * p.d;
     const float c = p.s * kLog2e;
-    typename S::Held hk, hv;
-    auto load = [&](int i, char* at) {
+    S sk(p.ldk, p.d, threadIdx.x), sv(p.ldv, p.d, threadIdx.x);
+    auto load = [&](S& st, const T* from_row, int64_t ld, int i, char* at) INLINE {
         const int key = keys.key(i);
         int from, to;
         tile_rows<BN>(range, key, from, to);
-        S::load(hk, k + key * p.ldk, p.ldk, p.d, from, to, at, threadIdx.x);
-        S::load(hv, v + key * p.ldv, p.ldv, p.d, from, to, at + TILE, threadIdx.x);
+        st.load(from_row + key * ld, from, to, at);
     };
+    // Tile i's weights are formed while the matrix cores form tile i + 1's scores (two waves of a SIMD alone do not fill them):
+    // keys lie two tiles ahead of the values' sums, values one.
+    char* const kt[2] = {lds, lds + TILE};
+    char* const vt[2] = {lds + 2 * TILE, lds + 3 * TILE};
     if (keys.count > 0) {
-        load(0, lds);
-        S::store(hk, lds, threadIdx.x);
-        S::store(hv, lds + TILE, threadIdx.x);
+        load(sk, k, p.ldk, 0, kt[0]);
+        load(sv, v, p.ldv, 0, vt[0]);
+        sk.store(kt[0]);
+        sv.store(vt[0]);
+        if (keys.count > 1) {
+            load(sk, k, p.ldk, 1, kt[1]);
+            sk.store(kt[1]);
+        }
         if constexpr (DIRECT) wait_loads<0>();
     }
+    settle_loads();
     __syncthreads();
-    for (int i = 0; i < keys.count; ++i) {
-        char* now = lds + (i & 1) * 2 * TILE;
-        char* next = lds + (~i & 1) * 2 * TILE;
-        if (i + 1 < keys.count) load(i + 1, next);
-        const int key = keys.key(i);
-        // (a wave whose rows see none of the tile leaves it out)
-        if (working && ((key < mine.high && key + BN > mine.low) || key < mine.sinks)) sums.template tile<BN / 32>(now, now + TILE, key, s, w.pos, w0, w1, c);
-        if (i + 1 < keys.count) {
-            S::store(hk, next, threadIdx.x);
-            S::store(hv, next + TILE, threadIdx.x);
-            if constexpr (DIRECT) wait_loads<0>();
+    typename R::Scores a, b;
+    if (keys.count > 0 && working) sums.scores(a, kt[0]);
+    __syncthreads();
+    auto step = [&](auto parity, typename R::Scores& now, typename R::Scores& next, int i) INLINE {
+        constexpr int P = decltype(parity)::value;
+        if (i + 2 < keys.count) load(sk, k, p.ldk, i + 2, kt[P]);
+        if (i + 1 < keys.count) load(sv, v, p.ldv, i + 1, vt[1 - P]);
+        if (working) {
+            sums.hide(now, keys.key(i), s, w.pos, w0, w1);
+            sums.raise(now, c);
+            sums.scores(next, kt[1 - P]);      // (behind the last tile: of what lies there, for nothing)
+            sums.add(now, vt[P], c);
+            if constexpr (sizeof(T) == 2) R::order();
         }
+        if (i + 2 < keys.count) sk.store(kt[P]);
+        if (i + 1 < keys.count) sv.store(vt[1 - P]);
+        if constexpr (DIRECT) wait_loads<0>();
         __syncthreads();
+    };
+    for (int i = 0; i < keys.count; i += 2) {
+        step(std::integral_constant<int, 0>{}, a, b, i);
+        if (i + 1 < keys.count) step(std::integral_constant<int, 1>{}, b, a, i + 1);
     }
     const float l = sums.l + other_half(sums.l);
     if (any_not_finite<DT>(sums.o)) {
-        exact_rows<T>(p, q, kvh, r0 + 32 * wave, 0, q.nk, [&](const Row& x, float m, float sum, Two o) {
+        exact_rows<T>(p, q, kvh, r0 + 32 * wave, 0, q.nk, [&](const Row& x, float m, float sum, Two o) INLINE {
             const float inv = 1.f / sum;
             store_two((T*)p.y + x.t * p.ldy + (int64_t)x.head * p.d, o.a * inv, o.b * inv, p.d, false);
             if (p.lse && lane == 0) p.lse[x.t * (p.heads * s.group) + x.head] = m + logf(sum);

@@ -9,6 +9,8 @@
 
 #include "rows.hpp"
 
+#include <type_traits>
+
 namespace stade {
 namespace attn {
 
@@ -24,6 +26,9 @@ typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef short v8s __attribute__((ext_vector_type(8)));
+
+// of a lambda in a kernel: what it captures stays in registers only where it is inlined
+#define INLINE __attribute__((always_inline))
 
 // the same value in every lane, in scalar registers
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -139,28 +144,38 @@ __device__ __forceinline__ void tile_rows(const Range& r, int key, int& from, in
 // ------------------------------------------------------------------------------------------
 // operand tiles in LDS
 // ------------------------------------------------------------------------------------------
-// A tile holds rows of DP values (64 or 128: the head's values and zeros), in 16-byte chunks; row r has its chunk c at place
-// c ^ turn(r).  It is read in two ways: sixteen rows' chunk c (fragments along the head), and, by the transposing read for
-// 16-bit types, four rows' 64 bytes (fragments along the rows).  The turn's bits are those of r in reverse, so
-// that both meet all the banks: sixteen rows turn a chunk to sixteen places, and rows 0 .. 3 turn 64 bytes to four.
+// A tile holds rows of DP values (64 or 128: the head's values and zeros), in 16-byte chunks, 1024 bytes (what a wave loads
+// straight to LDS at a time) one after the other, each kPad further.  Row r has its chunk c at place c ^ turn(r).  It is read in two
+// ways: sixteen rows' chunk c (fragments along the head), and, by the transposing read for 16-bit types, four rows' 64
+// bytes (fragments along the rows); turn and pad together let both meet all the banks.  For 16-bit types the turn
+// moves whole 64 bytes (two rows a pass over the banks: and 32), so that few addresses serve all fragments, the rest being constants.
 template <class T> constexpr int kCE = 16 / (int)sizeof(T);
 template <class T, int DP> constexpr int kRow = DP * (int)sizeof(T);
+template <class T> constexpr int kPad = sizeof(T) == 2 ? 16 : 0;
+template <class T, int DP, int ROWS> constexpr int kTile = ROWS * kRow<T, DP> / 1024 * (1024 + kPad<T>);
 
 template <class T, int DP>
 __device__ __forceinline__ int turn(int r) {
     if constexpr (sizeof(T) == 4) return (r >> 2 & 1) << 3 | (r & 3) << 1 | (r >> 3 & 1);   // (its rows are read 128 bytes at a time, two rows four apart)
-    else if constexpr (DP == 128) return (r & 3) << 2 | (r >> 2 & 1) << 1 | (r >> 3 & 1);
-    else return (r >> 1 & 1) << 2 | (r >> 2 & 1) << 1 | (r >> 3 & 1);                       // (two rows a pass over the banks)
+    else if constexpr (DP == 128) return (r & 3) << 2;
+    else return (r >> 1 & 1) << 2 | (r >> 2 & 1) << 1;
+}
+// the start of a row
+template <class T, int DP>
+__device__ __forceinline__ int row_at(int r) {
+    constexpr int PER = 1024 / kRow<T, DP>;
+    return r / PER * (1024 + kPad<T>) + r % PER * kRow<T, DP>;
 }
 template <class T, int DP>
 __device__ __forceinline__ int chunk_at(int r, int c) {
-    return r * kRow<T, DP> + ((c ^ turn<T, DP>(r)) << 4);
+    return row_at<T, DP>(r) + ((c ^ turn<T, DP>(r)) << 4);
 }
 
 // 16 bytes a lane from the buffer `r` at `off` to LDS, the wave's lanes from `at` on.  In assembly because
 // of the waits: for the builtin the compiler waits for all loads before the next LDS read of any kind, as it
 // cannot tell the buffers apart.  It has no output register; wait_loads counts it.
 __device__ __forceinline__ void load_to_lds(v4u r, uint32_t off, uint32_t at) {
+    at = (uint32_t)uniform((int)at);
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(r), "s"(at) : "memory");
 }
 template <int N>
@@ -170,6 +185,10 @@ __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
     __builtin_amdgcn_sched_barrier(0);
 }
+// Before a loop that counts its own loads: what the compiler's loads brought into registers is there, in a form that the
+// compiler sees.  Without it the compiler waits for them at their first use inside the loop, in every round, and with them
+// for all that is under way to LDS (the forward sweep at 16500 tokens: 390 us for ...).
+__device__ __forceinline__ void settle_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }   // vmcnt(0)
 // before a buffer is written again: this wave's reads of it are through
 __device__ __forceinline__ void wait_reads() {
     __builtin_amdgcn_sched_barrier(0);
@@ -192,40 +211,55 @@ __device__ __forceinline__ v4u load_chunk(const T* p, int left) {
     return __builtin_bit_cast(v4u, v);
 }
 
+// where the chunk that is the place'th of a tile lies
+template <class T>
+__device__ __forceinline__ int place_at(int place) {
+    return (place >> 6) * (1024 + kPad<T>) + (place & 63) * 16;
+}
+
 // Staging of a tile of ROWS rows by NT threads (`tid`: this thread's number among them): straight to LDS (DIRECT:
 // 16-byte aligned rows and whole chunks), or through registers.  Rows outside [from, to) become zeros.
 template <class T, int DP, int ROWS, int NT, bool DIRECT>
 struct Stage {
     static constexpr int CPR = kRow<T, DP> / 16, PER = ROWS * CPR / NT;
     static_assert(ROWS * CPR % NT == 0, "whole chunks a thread");
-    struct Held { v4u v[DIRECT ? 1 : PER]; };
+    uint32_t off[DIRECT ? PER : 1];   // a thread's chunks from the first row's start (past any buffer: none)
+    v4u held[DIRECT ? 1 : PER];
+    int64_t ld;
+    int d, tid;
 
-    // (`p`: the tile's first row)
-    static __device__ __forceinline__ void load(Held& h, const T* p, int64_t ld, int d, int from, int to, const char* lds, int tid) {
+    __device__ __forceinline__ Stage(int64_t ld_, int d_, int tid_) : ld(ld_), d(d_), tid(tid_) {
         if constexpr (DIRECT) {
-            const uint64_t base = (uint64_t)(p + (int64_t)from * ld);
-            const uint32_t row = (uint32_t)ld * sizeof(T), bytes = to > from ? (uint32_t)(to - from - 1) * row + (uint32_t)d * sizeof(T) : 0;
-            // (rows before `from` have offsets past the buffer too: they wrap)
-            const v4u r = {(uint32_t)uniform((int)(uint32_t)base), (uint32_t)uniform((int)((uint32_t)(base >> 32) & 0xffffu)), (uint32_t)uniform((int)bytes),
-                           0x00020000u};
-            const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)lds + uniform(tid >> 6) * 1024;
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
                 const int place = i * NT + tid, o = place / CPR, c = (place % CPR) ^ turn<T, DP>(o);
-                load_to_lds(r, c * kCE<T> < d ? (uint32_t)(o - from) * row + c * 16 : 0x80000000u, at + i * NT * 16);
+                off[i] = c * kCE<T> < d ? (uint32_t)o * ((uint32_t)ld * sizeof(T)) + c * 16 : 0x80000000u;
             }
+        }
+    }
+    // (`p`: the tile's first row)
+    __device__ __forceinline__ void load(const T* p, int from, int to, const char* lds) {
+        if constexpr (DIRECT) {
+            const uint64_t base = (uint64_t)(p + (int64_t)from * ld);
+            const uint32_t row = (uint32_t)ld * sizeof(T), bytes = to > from ? (uint32_t)(to - from - 1) * row + (uint32_t)d * sizeof(T) : 0;
+            const uint32_t less = (uint32_t)uniform((int)(from * row));   // (rows before `from` have offsets past the buffer too: they wrap)
+            const v4u r = {(uint32_t)uniform((int)(uint32_t)base), (uint32_t)uniform((int)((uint32_t)(base >> 32) & 0xffffu)), (uint32_t)uniform((int)bytes),
+                           0x00020000u};
+            const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)lds + uniform(tid >> 6) * (1024 + kPad<T>);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) load_to_lds(r, off[i] - less, at + i * (NT / 64) * (1024 + kPad<T>));
         } else {
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
                 const int place = i * NT + tid, o = place / CPR, c = (place % CPR) ^ turn<T, DP>(o);
-                h.v[i] = load_chunk(p + (int64_t)o * ld + c * kCE<T>, o >= from && o < to ? d - c * kCE<T> : 0);
+                held[i] = load_chunk(p + (int64_t)o * ld + c * kCE<T>, o >= from && o < to ? d - c * kCE<T> : 0);
             }
         }
     }
-    static __device__ __forceinline__ void store(const Held& h, char* lds, int tid) {
+    __device__ __forceinline__ void store(char* lds) const {
         if constexpr (!DIRECT) {
 #pragma unroll
-            for (int i = 0; i < PER; ++i) *reinterpret_cast<v4u*>(lds + (i * NT + tid) * 16) = h.v[i];
+            for (int i = 0; i < PER; ++i) *reinterpret_cast<v4u*>(lds + place_at<T>(i * NT + tid)) = held[i];
         }
     }
 };
@@ -237,8 +271,13 @@ struct Stage {
 // of the head for 16-bit types, 8 for fp32).
 template <class T, int DP>
 __device__ __forceinline__ v4u along_head(const char* lds, int row0, int s) {
-    const int lane = threadIdx.x & 63;
-    return *reinterpret_cast<const v4u*>(lds + chunk_at<T, DP>(row0 + (lane & 31), 2 * s + (lane >> 5)));
+    const int lane = threadIdx.x & 63, h = lane >> 5, r = lane & 31, t = turn<T, DP>(r);
+    // (row0 is a multiple of 32, which the turn does not see)
+    if constexpr (sizeof(T) == 2 && DP == 128) {
+        return *reinterpret_cast<const v4u*>(lds + (row_at<T, DP>(r) + h * 16 + ((4 * (s >> 1) ^ t) << 4)) + (row_at<T, DP>(row0) + 32 * (s & 1)));
+    } else {
+        return *reinterpret_cast<const v4u*>(lds + (row_at<T, DP>(r) + (((2 * s + h) ^ t) << 4)) + row_at<T, DP>(row0));
+    }
 }
 // Along the rows: 32 values of the head from `col` on, for as many rows from row0 on as a fragment has (16, fp32: 8).
 // The rows come in the order in which a 32 x 32 result holds its rows in registers (lane half h, register i: row
@@ -247,10 +286,12 @@ template <class T, int DP>
 __device__ __forceinline__ v4u along_rows(const char* lds, int row0, int col) {
     const int lane = threadIdx.x & 63, h = lane >> 5;
     if constexpr (sizeof(T) == 2) {
-        const int i = lane & 15, r = row0 + 4 * h + (i >> 2), c = (col >> 3) + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+        // (row0 is a multiple of 16, col of 32: of a chunk's number the turn moves the fours, and the two where it does, by lane)
+        const int i = lane & 15, r = 4 * h + (i >> 2), c = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1), t = turn<T, DP>(r);
+        const char* at = lds + (row_at<T, DP>(r) + (((c ^ (t & 3)) + (col / 8 ^ (t & ~3))) << 4) + (i & 1) * 8) + row_at<T, DP>(row0);
         typedef __attribute__((address_space(3))) v4s* lp;
-        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(lds + chunk_at<T, DP>(r, c) + (i & 1) * 8));
-        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(lds + chunk_at<T, DP>(r + 8, c) + (i & 1) * 8));
+        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(at));
+        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(at + row_at<T, DP>(8)));
         return __builtin_bit_cast(v4u, (v8s){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
     } else {
         const int x = col + (lane & 31);
@@ -282,6 +323,29 @@ __device__ __forceinline__ v4u part_of(const floatx16& v, int u) {
 #pragma unroll
     for (int i = 0; i < kCE<T>; ++i) p[i] = (T)v[u * kCE<T> + i];
     return __builtin_bit_cast(v4u, p);
+}
+
+// The order in which the compiler is to issue a stretch of code: so many instructions of a kind next.  (Left alone it reads a
+// fragment just before its product and waits for LDS each time.)
+constexpr int kValu = 2, kMfma = 8, kRead = 0x100, kTrans = 0x400;
+#define ORDER(kind, n) __builtin_amdgcn_sched_group_barrier(kind, n, 0)
+
+// N products one after the other, in the order written, each step fenced off: product(i, fragment i), the read of the
+// fragment AHEAD products later (so that LDS is never waited for), and what else there is to do meanwhile, rest(i).
+template <int N, int AHEAD, class L, class M, class F>
+__device__ __forceinline__ void products(L&& fragment, M&& product, F&& rest) {
+    decltype(fragment(std::integral_constant<int, 0>{})) r[AHEAD];
+    static_for<AHEAD>([&](auto i) INLINE {
+        if constexpr (decltype(i)::value < N) r[decltype(i)::value] = fragment(i);
+    });
+    __builtin_amdgcn_sched_barrier(0);
+    static_for<N>([&](auto i) INLINE {
+        constexpr int I = decltype(i)::value;
+        product(i, r[I % AHEAD]);
+        if constexpr (I + AHEAD < N) r[I % AHEAD] = fragment(std::integral_constant<int, I + AHEAD>{});
+        rest(i);
+        __builtin_amdgcn_sched_barrier(0);
+    });
 }
 
 // ------------------------------------------------------------------------------------------

@@ -38,12 +38,16 @@ struct Back {
     float s;
     int add;
     int64_t slots;
-    uint32_t magic;        // ceil(2^32 / group)
+    uint32_t magic;        // ceil(2^31 / group)
     float* far;            // partial sums of the sinks; null: none
     int far_parts;
+    int64_t whole;         // tiles of keys that a block has alone; the others go over `splits` blocks each
+    int splits;
+    float* part;           // those blocks' sums
 };
 
 constexpr int kRows = 128, kKeys = 128;
+
 
 template <class T>
 __device__ __forceinline__ void store4(T* p, float a, float b, float c, float e, int left, bool add) {
@@ -77,7 +81,7 @@ __device__ __forceinline__ void place_of(int64_t block, int64_t slots, int heads
 // ------------------------------------------------------------------------------------------
 template <class T, int DT, bool DIRECT>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void rows_kernel(Back p) {
-    constexpr int DP = DT > 2 ? 128 : 64, BN = sizeof(T) == 2 ? 64 : 32, NB = BN / 32, TILE = BN * kRow<T, DP>, FR = DT * 32 / (2 * kCE<T>);
+    constexpr int DP = DT > 2 ? 128 : 64, BN = sizeof(T) == 2 ? 64 : 32, NB = BN / 32, TILE = kTile<T, DP, BN>, FR = DT * 32 / (2 * kCE<T>);
     using S = Stage<T, DP, BN, 256, DIRECT>;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];
     const Seqs& s = p.seqs;
@@ -126,20 +130,21 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void rows_kernel(Back 
     for (int i = 0; i < DT; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
-    typename S::Held hk, hv;
-    auto load = [&](int i, char* at) {
+    S sk(p.ldk, p.d, threadIdx.x), sv(p.ldv, p.d, threadIdx.x);
+    auto load = [&](int i, char* at) INLINE {
         const int key = keys.key(i);
         int from, to;
         tile_rows<BN>(range, key, from, to);
-        S::load(hk, k + key * p.ldk, p.ldk, p.d, from, to, at, threadIdx.x);
-        S::load(hv, v + key * p.ldv, p.ldv, p.d, from, to, at + TILE, threadIdx.x);
+        sk.load(k + key * p.ldk, from, to, at);
+        sv.load(v + key * p.ldv, from, to, at + TILE);
     };
     if (keys.count > 0) {
         load(0, lds);
-        S::store(hk, lds, threadIdx.x);
-        S::store(hv, lds + TILE, threadIdx.x);
+        sk.store(lds);
+        sv.store(lds + TILE);
         if constexpr (DIRECT) wait_loads<0>();
     }
+    settle_loads();
     __syncthreads();
     for (int i = 0; i < keys.count; ++i) {
         char* now = lds + (i & 1) * 2 * TILE;
@@ -176,8 +181,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void rows_kernel(Back 
             }
         }
         if (i + 1 < keys.count) {
-            S::store(hk, next, threadIdx.x);
-            S::store(hv, next + TILE, threadIdx.x);
+            sk.store(next);
+            sv.store(next + TILE);
             if constexpr (DIRECT) wait_loads<0>();
         }
         __syncthreads();
@@ -218,80 +223,159 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void rows_kernel(Back 
 // ------------------------------------------------------------------------------------------
 // kb and vb
 // ------------------------------------------------------------------------------------------
-// The block's waves: four of 32 keys each; for 16-bit types twice, for the two halves of a tile's rows (two waves a SIMD:
-// one's exponentials beside the other's products), whose sums are joined at the end.
-template <class T> constexpr int kHalves = sizeof(T) == 2 ? 2 : 1;
+// A block's waves: kGroups of 32 keys by kRowWaves, each with kBlocks of 32 rows of a tile.  16-bit types: four by one with two
+// blocks side by side, one wave a SIMD, whose 512 registers hold its keys and values, the sums and both blocks' scores; one
+// block's exponentials lie between the other's products.  (Two waves a SIMD, one block each, have no room for the values, and read LDS half
+// as often again.)  fp32: four by one, a block.  FAR: one by four (fp32 two), a block, see below.
+template <class T, bool FAR> constexpr int kGroups = FAR ? 1 : 4;
+template <class T, bool FAR> constexpr int kRowWaves = FAR ? (sizeof(T) == 2 ? 4 : 2) : 1;
+template <class T, bool FAR> constexpr int kBlocks = FAR ? 1 : sizeof(T) == 2 ? 2 : 1;
+template <class T, bool FAR> constexpr int kTileRows = 32 * kRowWaves<T, FAR> * kBlocks<T, FAR>;
 
-// rows r0 .. of a sequence in LDS: a row's q, yb, lse and delta.  A row's column and head by a product with the
-// group's reciprocal (exact for less than 2^32 / group).
+// x / group for small x, by the reciprocal (off by less than x 2^-31: exact for x below 2^31 / group, and here x is
+// below group + 64)
+__device__ __forceinline__ uint32_t by_group(uint32_t x, uint32_t magic) { return __umulhi(2 * x, magic); }
+
+// Rows of a sequence in LDS: q or yb of the (query, head) pairs from one on, heads side by side.  Which of its values a thread
+// loads depends on the first row's head, and not on that where a tile has whole queries.  Their addresses grow row by
+// row: the rows behind the last lie past the buffer's end, and become zeros.
 template <class T, int DP, int ROWS, int NT, bool DIRECT>
 struct RowStage {
     static constexpr int CPR = kRow<T, DP> / 16, PER = ROWS * CPR / NT;
-    struct Held { v4u v[DIRECT ? 1 : PER]; };
+    static_assert(ROWS * CPR % NT == 0, "whole chunks a thread");
+    uint32_t off[DIRECT ? PER : 1];
+    v4u held[DIRECT ? 1 : PER];
+    const T* p;      // the tile's first row's query, head 0 of the group
+    uint32_t bytes;  // from there to the last row's end
+    int rem, rows;   // the first row's head; rows
 
-    static __device__ __forceinline__ void load(Held& held, const T* p, int64_t ld, int d, int group, uint32_t magic, int rem, int rows, const char* lds) {
-        // (p: the head 0 of the group of row r0's query; rem: r0's head)
-        const uint64_t base = (uint64_t)p;
-        const v4u r = {(uint32_t)uniform((int)(uint32_t)base), (uint32_t)uniform((int)((uint32_t)(base >> 32) & 0xffffu)), 0x7fffffffu, 0x00020000u};
-        const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)lds + uniform((int)(threadIdx.x >> 6)) * 1024;
+    // the chunks' places for a first row of head `rem_`
+    __device__ __forceinline__ void places(int64_t ld, int d, int group, uint32_t magic, int rem_) {
+        rem = rem_;
+        if constexpr (DIRECT) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int place = i * NT + threadIdx.x, o = place / CPR, c = (place % CPR) ^ turn<T, DP>(o);
-            const uint32_t x = rem + o, jq = group == 1 ? x : __umulhi(x, magic), hd = x - jq * group;
-            if constexpr (DIRECT)
-                load_to_lds(r, o < rows && c * kCE<T> < d ? (jq * (uint32_t)ld + hd * d + c * kCE<T>) * (uint32_t)sizeof(T) : 0x80000000u, at + i * NT * 16);
-            else
-                held.v[i] = load_chunk(p + (int64_t)jq * ld + hd * d + c * kCE<T>, o < rows ? d - c * kCE<T> : 0);
+            for (int i = 0; i < PER; ++i) {
+                const int place = i * NT + threadIdx.x, o = place / CPR, c = (place % CPR) ^ turn<T, DP>(o);
+                const uint32_t x = rem + o, jq = by_group(x, magic), hd = x - jq * group;
+                off[i] = c * kCE<T> < d ? (jq * (uint32_t)ld + hd * d + c * kCE<T>) * (uint32_t)sizeof(T) : 0x80000000u;
+            }
         }
     }
-    static __device__ __forceinline__ void store(const Held& held, char* lds) {
+    __device__ __forceinline__ void tile(const T* p_, int64_t ld, int d, int group, uint32_t magic, int rows_) {
+        p = p_;
+        rows = rows_;
+        const uint32_t x = rem + max(rows - 1, 0), jq = by_group(x, magic), hd = x - jq * group;
+        bytes = rows > 0 ? (uint32_t)uniform((int)((jq * (uint32_t)ld + hd * d + d) * (uint32_t)sizeof(T))) : 0;
+    }
+    template <int I>
+    __device__ __forceinline__ void load(int64_t ld, int d, int group, uint32_t magic, const char* lds) {
+        if constexpr (DIRECT) {
+            const uint64_t base = (uint64_t)p;
+            const v4u r = {(uint32_t)uniform((int)(uint32_t)base), (uint32_t)uniform((int)((uint32_t)(base >> 32) & 0xffffu)), bytes, 0x00020000u};
+            const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)lds + uniform((int)(threadIdx.x >> 6)) * (1024 + kPad<T>);
+            load_to_lds(r, off[I], at + I * (NT / 64) * (1024 + kPad<T>));
+        } else {
+            const int place = I * NT + threadIdx.x, o = place / CPR, c = (place % CPR) ^ turn<T, DP>(o);
+            const uint32_t x = rem + o, jq = by_group(x, magic), hd = x - jq * group;
+            held[I] = load_chunk(p + (int64_t)jq * ld + hd * d + c * kCE<T>, o < rows ? d - c * kCE<T> : 0);
+        }
+    }
+    __device__ __forceinline__ void store(char* lds) const {
         if constexpr (!DIRECT) {
 #pragma unroll
-            for (int i = 0; i < PER; ++i) *reinterpret_cast<v4u*>(lds + (i * NT + threadIdx.x) * 16) = held.v[i];
+            for (int i = 0; i < PER; ++i) *reinterpret_cast<v4u*>(lds + place_at<T>(i * NT + threadIdx.x)) = held[i];
         }
     }
 };
 
-// FAR: rows past the first tile's window, which see its sinks only; block (part, sequence, head)
+// What a block of keys_kernel works on, and where the rows' range is cut
+struct KeyTile {
+    Seq q;
+    int64_t first;       // of the sequence's (or of no sequence's) key columns
+    int keys, key0;      // how many they are; the tile's first
+    int r_first, r_end;  // the rows that see it, without those past the window of a first tile
+    int far_rows;        // those
+};
+__device__ __forceinline__ KeyTile key_tile(const Seqs& s, int j, int64_t tile) {
+    KeyTile k;
+    k.first = j == 0 ? 0 : clamped(s.kstart[j - 1], s.tk);
+    k.keys = (int)max((j > s.n ? s.tk : clamped(s.kstart[j], s.tk)) - k.first, (int64_t)0);
+    k.key0 = (int)min(tile * kKeys, (int64_t)k.keys);
+    k.q = sequence(s, j - 1);
+    const int64_t last = (int64_t)k.key0 + kKeys - 1 + s.window - 1;    // the last position whose window has a key of the tile
+    const int j0 = max(k.key0 - k.q.shift(), 0), j1 = k.q.real ? (int)min((int64_t)k.q.nq, max(last + 1 - k.q.shift(), (int64_t)0)) : 0;
+    k.r_first = j0 * s.group;
+    k.r_end = max(j1, j0) * s.group;
+    k.far_rows = k.q.real ? (k.q.nq - j1) * s.group : 0;
+    return k;
+}
+// rows of a part, of `parts` that a range is cut into: whole tiles of BM
+__device__ __forceinline__ int part_rows(int rows, int parts, int BM) { return (rows / parts / BM + 1) * BM; }
+
+// A split block's sums, and a far block's: (kb, vb) of its keys, d values each, one key after the other
+template <int DT>
+__device__ __forceinline__ void store_part(float* out, int d, const floatx16 (&a)[DT]) {
+    const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int m = 0; m < DT; ++m)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int at = 32 * m + 8 * g + 4 * h;
+            const float v[4] = {a[m][4 * g], a[m][4 * g + 1], a[m][4 * g + 2], a[m][4 * g + 3]};
+            store_row(out + at, v, d - at);
+        }
+}
+
+// FAR: rows past the first tile's window, which see its sinks only; block (part, sequence, head, 32 of the sinks).  Its waves have
+// the same keys and other rows.
 template <class T, int DT, bool DIRECT, bool FAR>
-__global__ __launch_bounds__(256 * kHalves<T>, kHalves<T>) void keys_kernel(Back p) {
-    constexpr int DP = DT > 2 ? 128 : 64, HALVES = kHalves<T>, NT = 256 * HALVES, BM = 32 * HALVES, TILE = BM * kRow<T, DP>;
-    constexpr int FR = DT * 32 / (2 * kCE<T>), STATS = 2 * BM * 4, BUF = 2 * TILE;
+__global__ __launch_bounds__((64 * kGroups<T, FAR> * kRowWaves<T, FAR>), (sizeof(T) == 2 && DT == 2 && !FAR ? 2 : 1)) void keys_kernel(Back p) {
+    constexpr int DP = DT > 2 ? 128 : 64, KG = kGroups<T, FAR>, RG = kRowWaves<T, FAR>, RB = kBlocks<T, FAR>, NT = 64 * KG * RG, BM = kTileRows<T, FAR>;
+    constexpr int TILE = kTile<T, DP, BM>, FR = DT * 32 / (2 * kCE<T>), STATS = 2 * BM * 4, BUF = 2 * TILE;
+    static_assert(FAR || KG * 32 == kKeys, "the waves' keys make a tile");
     using S = RowStage<T, DP, BM, NT, DIRECT>;
+    // two tiles of rows of q and of yb, and the rows' lse and delta
     __shared__ __attribute__((aligned(1024))) char lds[2 * BUF + 2 * STATS];
+    char* const st = lds + 2 * BUF;
     const Seqs& s = p.seqs;
     int64_t slot, tile;
-    int kvh, j;
+    int kvh, j, split = -1, far32 = 0;
     if constexpr (FAR) {
         const int64_t b = blockIdx.x / p.far_parts;
         tile = blockIdx.x % p.far_parts;
         kvh = (int)(b % p.heads);
         j = (int)(b / p.heads) + 1;
+        far32 = 32 * blockIdx.y;
     } else {
-        place_of(blockIdx.x, p.slots, p.heads, slot, kvh);
+        int64_t unit = blockIdx.x;
+        if (unit >= p.whole) {
+            split = (int)((unit - p.whole) % p.splits);
+            unit = p.whole + (unit - p.whole) / p.splits;
+        }
+        place_of(unit, p.slots, p.heads, slot, kvh);
         j = find_range(s.kstart, s.tk, 1, kKeys, s.n + 1, slot, tile);
     }
-    const int wave = uniform((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, h = lane >> 5, part = wave & 3, half = wave >> 2;
-    const int64_t k_first = j == 0 ? 0 : clamped(s.kstart[j - 1], s.tk);
-    const int keys = (int)max((j > s.n ? s.tk : clamped(s.kstart[j], s.tk)) - k_first, (int64_t)0);
-    const int key0 = FAR ? 0 : (int)min(tile * kKeys, (int64_t)keys);
+    const int wave = uniform((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, h = lane >> 5;
+    const KeyTile kt = key_tile(s, j, FAR ? 0 : tile);
+    const Seq& q = kt.q;
+    const int keys = kt.keys, key0 = kt.key0, shift = q.shift();
     if (key0 >= keys) return;
-    const Seq q = sequence(s, j - 1);
-    // the rows that see the tile's keys, without what the far blocks do
-    const int shift = q.shift();
-    const int64_t last = (int64_t)key0 + kKeys - 1 + s.window - 1;    // the last position whose window has a key of the tile
-    const int j0 = max(key0 - shift, 0), j1 = q.real ? (int)min((int64_t)q.nq, max(last + 1 - shift, (int64_t)0)) : 0;
-    int r_first = j0 * s.group, r_end = j1 * s.group;
-    const int far_rows = max(q.nq - max(j1, 0), 0) * s.group;         // (of the first tile)
-    const int far_step = p.far_parts ? (far_rows / p.far_parts / BM + 1) * BM : 0;
+    int r_first = kt.r_first, r_end = kt.r_end;
+    const int far_step = p.far_parts ? part_rows(kt.far_rows, p.far_parts, BM) : 0;
     if constexpr (FAR) {
         r_first = r_end + (int)tile * far_step;
         r_end = min(r_first + far_step, q.nq * s.group);
         if (!q.real || r_first >= r_end) return;
+    } else if (split >= 0) {
+        const int step = part_rows(r_end - r_first, p.splits, BM);
+        r_first += split * step;
+        r_end = min(r_first + step, r_end);
+        if (r_first >= r_end) return;
     }
-    const int own = key0 + 32 * part;      // this wave's keys
-    const int64_t kcol = k_first + own + (lane & 31), hcol = (int64_t)kvh * p.d;
-    const bool here = own + (lane & 31) < keys, working = own < keys && (!FAR || own < s.sinks);
+    const int group = wave % KG, first_row = 32 * RB * (wave / KG);                     // the wave's rows of a tile
+    const int own = FAR ? far32 : key0 + 32 * group, key = own + (lane & 31);      // its keys, and the lane's
+    const int64_t kcol = kt.first + key, hcol = (int64_t)kvh * p.d;
+    const bool here = key < keys, working = own < keys && (!FAR || own < s.sinks);
     v4u kf[FR], vf[FR];
     row_fragments<T, DT, DIRECT>(kf, (const T*)p.k + kcol * p.ldk + hcol, here, p.d);
     row_fragments<T, DT, DIRECT>(vf, (const T*)p.v + kcol * p.ldv + hcol, here, p.d);
@@ -302,100 +386,165 @@ __global__ __launch_bounds__(256 * kHalves<T>, kHalves<T>) void keys_kernel(Back
         for (int e = 0; e < 16; ++e) ka[i][e] = va[i][e] = 0.f;
     const float c = p.s * kLog2e;
     const int heads = p.heads * s.group, tiles = r_end > r_first ? (r_end - r_first + BM - 1) / BM : 0;
-    typename S::Held hq, ho;
+    // (the query and the head in its group of a tile's first row: of the one at work and of the one on its way)
+    int now_j = uniform(r_first / s.group), now_h = uniform(r_first - now_j * s.group), next_j = now_j, next_h = now_h;
+    S sq, so;
     float stat = 0.f;
-    auto load = [&](int i, char* at) {
-        const int r0 = r_first + i * BM, jq = r0 / s.group, rem = r0 - jq * s.group, rows = min(BM, r_end - r0);
-        const int64_t t = q.q0 + jq, head = (int64_t)kvh * s.group;
-        S::load(hq, (const T*)p.q + t * p.ldq + head * p.d, p.ldq, p.d, s.group, p.magic, rem, rows, at);
-        S::load(ho, (const T*)p.yb + t * p.ldyb + head * p.d, p.ldyb, p.d, s.group, p.magic, rem, rows, at + TILE);
-        if (threadIdx.x < 2 * BM) {     // lse and delta, one a thread (rows that are not: no weight)
+    sq.places(p.ldq, p.d, s.group, p.magic, now_h);
+    so.places(p.ldyb, p.d, s.group, p.magic, now_h);
+    const bool fixed = BM % s.group == 0;      // (tiles of whole queries)
+    const float per_s = -1.f / p.s;
+    auto aim = [&](int i) INLINE {             // at tile i (behind the last: no rows)
+        const int64_t t = q.q0 + next_j, head = (int64_t)kvh * s.group;
+        const int rows = min(BM, r_end - (r_first + i * BM));
+        if (!fixed) {
+            sq.places(p.ldq, p.d, s.group, p.magic, next_h);
+            so.places(p.ldyb, p.d, s.group, p.magic, next_h);
+        }
+        sq.tile((const T*)p.q + t * p.ldq + head * p.d, p.ldq, p.d, s.group, p.magic, rows);
+        so.tile((const T*)p.yb + t * p.ldyb + head * p.d, p.ldyb, p.d, s.group, p.magic, rows);
+        if (threadIdx.x < 2 * BM) {            // lse and delta, one a thread (rows that are not: no weight)
             const int o = threadIdx.x % BM;
-            const uint32_t x = rem + o, jo = s.group == 1 ? x : __umulhi(x, p.magic);
-            const int64_t at1 = (t + jo) * heads + head + (x - jo * s.group);
+            const uint32_t x = next_h + o, jo = by_group(x, p.magic);
+            const int64_t at = (t + jo) * heads + head + (x - jo * s.group);
             const bool first = threadIdx.x < BM;
             stat = first ? INFINITY : 0.f;
-            if (o < rows) stat = first ? p.lse[at1] : p.delta[at1];
-            if (first) stat *= -kLog2e;
+            if (o < rows) stat = first ? p.lse[at] : p.delta[at];
         }
     };
-    auto keep = [&](int i, char* at) {
-        S::store(hq, at);
-        S::store(ho, at + TILE);
-        if (threadIdx.x < 2 * BM) reinterpret_cast<float*>(lds + 2 * BUF + (i & 1) * STATS)[threadIdx.x] = stat;
+    constexpr int CHUNKS = 2 * S::PER;         // of a thread, q's and yb's
+    auto load = [&](auto piece, char* at) INLINE {
+        constexpr int N = decltype(piece)::value;
+        if constexpr (N < S::PER) sq.template load<N>(p.ldq, p.d, s.group, p.magic, at);
+        else so.template load<N - S::PER>(p.ldyb, p.d, s.group, p.magic, at + TILE);
+    };
+    auto load_all = [&](char* at) INLINE { static_for<CHUNKS>([&](auto n) INLINE { load(n, at); }); };
+    // The products start from what belongs to a row: scores from -lse / s, yb v^T from -delta.
+    auto keep = [&](int i, char* at) INLINE {
+        sq.store(at);
+        so.store(at + TILE);
+        if (threadIdx.x < 2 * BM) reinterpret_cast<float*>(st + (i & 1) * STATS)[threadIdx.x] = threadIdx.x < BM ? stat * per_s : -stat;
         if constexpr (DIRECT) wait_loads<0>();
     };
     if (tiles > 0) {
-        load(0, lds);
+        aim(0);
+        load_all(lds);
         keep(0, lds);
     }
+    settle_loads();
     __syncthreads();
     for (int i = 0; i < tiles; ++i) {
         const char* now = lds + (i & 1) * BUF;
         char* next = lds + (~i & 1) * BUF;
-        if (i + 1 < tiles) load(i + 1, next);
-        const int r0 = r_first + i * BM + 32 * half, end = min(r0 + 31, r_end - 1);
-        const int pa = uniform(r0 / s.group + shift), pb = uniform(end / s.group + shift);
-        const int own_to = own + 31;
-        if (working && r0 < r_end && pb >= own && (pa - own_to < s.window || own < s.sinks)) {
-            const float* stats = reinterpret_cast<const float*>(lds + 2 * BUF + (i & 1) * STATS) + 32 * half;
-            floatx16 x, g;
+        const int step = (int)by_group(now_h + BM, p.magic);
+        next_j = now_j + step;
+        next_h = now_h + BM - step * s.group;
+        aim(i + 1);
+        const int end = min(first_row + 32 * RB, r_end - (r_first + i * BM)) - 1;
+        const int pa = uniform(now_j + (int)by_group(now_h + first_row, p.magic) + shift), pb = uniform(now_j + (int)by_group(now_h + max(end, 0), p.magic) + shift);
+        const bool whole = (own + 31 <= pa) & ((pb - own < s.window) | (own + 31 < s.sinks));
+        if (working && end >= first_row && pb >= own && (pa - (own + 31) < s.window || own < s.sinks)) {
+            const float* stats = reinterpret_cast<const float*>(st + (i & 1) * STATS) + first_row;
+            const char* qt = now + row_at<T, DP>(first_row);
+            const char* yt = qt + TILE;
+            constexpr int PU = kParts<T>, PER = PU * DT;      // parts of a result; products by them
+            floatx16 x[RB], g[RB];
+            auto start = [&](floatx16& v, int at) INLINE {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = g[e] = 0.f;
+                for (int m = 0; m < 4; ++m) {
+                    const v4f a = *reinterpret_cast<const v4f*>(stats + at + 8 * m + 4 * h);
 #pragma unroll
-            for (int f = 0; f < FR; ++f) x = multiply<T>(along_head<T, DP>(now, 32 * half, f), kf[f], x);
-#pragma unroll
-            for (int f = 0; f < FR; ++f) g = multiply<T>(along_head<T, DP>(now + TILE, 32 * half, f), vf[f], g);
-            const bool whole = own_to <= pa && (pb - own < s.window || own_to < s.sinks);
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const v4f l = *reinterpret_cast<const v4f*>(stats + 8 * m + 4 * h);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[4 * m + e] = __builtin_amdgcn_exp2f(fmaf(x[4 * m + e], c, l[e]));
-            }
-            if (!whole) {
-                const int key = own + (lane & 31), rr = r0 + 4 * h;
-                const int rem = rr % s.group, jq = rr / s.group;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const uint32_t xo = rem + 8 * (e >> 2) + (e & 3), jo = s.group == 1 ? xo : __umulhi(xo, p.magic);
-                    const int pos = jq + (int)jo + shift;
-                    if (!(key <= pos && (pos - key < s.window || key < s.sinks))) x[e] = g[e] = 0.f;
+                    for (int e = 0; e < 4; ++e) v[4 * m + e] = a[e];
                 }
+            };
+            // The scores block by block, then yb v^T.  Between the first block's products go the loads of the next tile, between all that
+            // follow the exponentials, none before its scores are there.
+            start(x[0], 0);
+            products<2 * RB * FR, 6>(
+                [&](auto n) INLINE {
+                    constexpr int N = decltype(n)::value, PH = N / FR;
+                    return along_head<T, DP>(PH < RB ? qt : yt, 32 * (PH % RB), N % FR);
+                },
+                [&](auto n, const v4u& f) INLINE {
+                    constexpr int N = decltype(n)::value, PH = N / FR;
+                    if constexpr (PH < RB) x[PH] = multiply<T>(f, kf[N % FR], x[PH]);
+                    else g[PH - RB] = multiply<T>(f, vf[N % FR], g[PH - RB]);
+                },
+                [&](auto n) INLINE {
+                    constexpr int N = decltype(n)::value, PH = N / FR, F = N % FR;
+                    if constexpr (PH == 0) {
+                        constexpr int FROM = F * CHUNKS / FR;
+                        static_for<(F + 1) * CHUNKS / FR - FROM>([&](auto k) INLINE { load(std::integral_constant<int, FROM + decltype(k)::value>{}, next); });
+                    }
+                    if constexpr (F == FR - 3 && PH + 1 < 2 * RB) {
+                        if constexpr (PH + 1 < RB) start(x[PH + 1], 32 * (PH + 1));
+                        else start(g[PH + 1 - RB], BM + 32 * (PH + 1 - RB));
+                    }
+                    if constexpr (N > FR) {
+                        constexpr int STEPS = (2 * RB - 1) * FR - 1, FROM = (N - FR - 1) * 16 * RB / STEPS;
+                        static_for<(N - FR) * 16 * RB / STEPS - FROM>([&](auto k) INLINE {
+                            constexpr int E = FROM + decltype(k)::value;
+                            x[E / 16][E % 16] = __builtin_amdgcn_exp2f(x[E / 16][E % 16] * c);
+                        });
+                    }
+                });
+            if (!whole) {
+#pragma unroll
+                for (int b = 0; b < RB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int pos = now_j + (int)by_group(now_h + first_row + 32 * b + 4 * h + 8 * (e >> 2) + (e & 3), p.magic) + shift;
+                        if (!((key <= pos) & ((pos - key < s.window) | (key < s.sinks)))) x[b][e] = g[b][e] = 0.f;
+                    }
             }
+            // vb's products block by block, and between them S = P (yb v^T - delta); then kb's
+            v4u w[RB * PU];
 #pragma unroll
-            for (int u = 0; u < kParts<T>; ++u) {
-                const v4u w = part_of<T>(x, u);
+            for (int b = 0; b < RB; ++b)
 #pragma unroll
-                for (int m = 0; m < DT; ++m) va[m] = multiply<T>(along_rows<T, DP>(now + TILE, 32 * half + u * 2 * kCE<T>, 32 * m), w, va[m]);
-            }
+                for (int u = 0; u < PU; ++u) w[b * PU + u] = part_of<T>(x[b], u);
+            products<2 * RB * PER, 4>(
+                [&](auto n) INLINE {
+                    constexpr int N = decltype(n)::value, PH = N / PER, U = N % PER / DT, M = N % DT;
+                    return along_rows<T, DP>(PH < RB ? yt : qt, 32 * (PH % RB) + U * 2 * kCE<T>, 32 * M);
+                },
+                [&](auto n, const v4u& f) INLINE {
+                    constexpr int N = decltype(n)::value, PH = N / PER, U = N % PER / DT, M = N % DT;
+                    if constexpr (PH < RB) va[M] = multiply<T>(f, w[PH * PU + U], va[M]);
+                    else ka[M] = multiply<T>(f, w[(PH - RB) * PU + U], ka[M]);
+                },
+                [&](auto n) INLINE {
+                    constexpr int N = decltype(n)::value, PH = N / PER, F = N % PER, FROM = F * 16 / PER;
+                    if constexpr (PH < RB) {
+                        static_for<(F + 1) * 16 / PER - FROM>([&](auto k) INLINE {
+                            constexpr int E = FROM + decltype(k)::value;
+                            x[PH][E] *= g[PH][E];
+                        });
+                        if constexpr (F == PER - 1) {
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const v4f dl = *reinterpret_cast<const v4f*>(stats + BM + 8 * m + 4 * h);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[4 * m + e] *= g[4 * m + e] - dl[e];
-            }
-#pragma unroll
-            for (int u = 0; u < kParts<T>; ++u) {
-                const v4u w = part_of<T>(x, u);
-#pragma unroll
-                for (int m = 0; m < DT; ++m) ka[m] = multiply<T>(along_rows<T, DP>(now, 32 * half + u * 2 * kCE<T>, 32 * m), w, ka[m]);
-            }
+                            for (int u = 0; u < PU; ++u) w[PH * PU + u] = part_of<T>(x[PH], u);
+                        }
+                    }
+                });
+        } else {
+            load_all(next);
         }
-        if (i + 1 < tiles) keep(i + 1, next);
+        keep(i + 1, next);
+        now_j = next_j;
+        now_h = next_h;
         __syncthreads();
     }
     if (working && (any_not_finite<DT>(ka) || any_not_finite<DT>(va))) {
         for (int n = 0; n < 32 && own + n < keys; ++n) {
-            const int key = own + n;
-            const Two kn = load_two((const T*)p.k + (k_first + key) * p.ldk + hcol, p.d), vn = load_two((const T*)p.v + (k_first + key) * p.ldv + hcol, p.d);
+            const int kn = own + n;
+            const Two kv = load_two((const T*)p.k + (kt.first + kn) * p.ldk + hcol, p.d), vv = load_two((const T*)p.v + (kt.first + kn) * p.ldv + hcol, p.d);
             Two a{0.f, 0.f}, b{0.f, 0.f};
-            for (int r = r_first + 32 * half; r < r_end; r += (r - r_first) % 32 == 31 ? BM - 31 : 1) {
+            for (int r = r_first + first_row; r < r_end; r += (r - r_first) % (32 * RB) == 32 * RB - 1 ? BM - 32 * RB + 1 : 1) {
                 const int ji = r / s.group, hi = kvh * s.group + r - ji * s.group, pos = ji + shift;
-                if (!(key <= pos && (pos - key < s.window || key < s.sinks))) continue;
+                if (!(kn <= pos && (pos - kn < s.window || kn < s.sinks))) continue;
                 const int64_t ti = q.q0 + ji, ci = (int64_t)hi * p.d, at = ti * heads + hi;
                 const Two x = load_two((const T*)p.q + ti * p.ldq + ci, p.d), g = load_two((const T*)p.yb + ti * p.ldyb + ci, p.d);
-                const float w = exp2f((dot(x, kn) * p.s - p.lse[at]) * kLog2e), ds = w * (dot(g, vn) - p.delta[at]);
+                const float w = exp2f((dot(x, kv) * p.s - p.lse[at]) * kLog2e), ds = w * (dot(g, vv) - p.delta[at]);
                 a.a = fmaf(ds, x.a, a.a);
                 a.b = fmaf(ds, x.b, a.b);
                 b.a = fmaf(w, g.a, b.a);
@@ -415,63 +564,63 @@ __global__ __launch_bounds__(256 * kHalves<T>, kHalves<T>) void keys_kernel(Back
                 }
         }
     }
-    if constexpr (HALVES > 1) {   // the second half's sums, one array after the other
-        static_assert(4 * DT * 4096 <= 2 * BUF, "the sums fit the tiles' memory");
-        float* sums = reinterpret_cast<float*>(lds) + part * DT * 1024 + lane;
-        for (int a = 0; a < 2; ++a) {
-            __syncthreads();
-            if (half == 1) {
+    if constexpr (RG > 1) {     // the sums of the waves with the same keys, one after the other
+        static_assert(KG * DT * 4096 <= 2 * BUF, "the sums fit the tiles' memory");
+        float* sums = reinterpret_cast<float*>(lds) + group * DT * 1024 + lane;
+        auto join = [&](floatx16 (&v)[DT]) INLINE {
+            for (int n = 1; n < RG; ++n) {
+                __syncthreads();
+                if (first_row == 32 * RB * n) {
 #pragma unroll
-                for (int m = 0; m < DT; ++m)
+                    for (int m = 0; m < DT; ++m)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) sums[(m * 16 + e) * 64] = a ? va[m][e] : ka[m][e];
+                        for (int e = 0; e < 16; ++e) sums[(m * 16 + e) * 64] = v[m][e];
+                }
+                __syncthreads();
+                if (first_row == 0) {
+#pragma unroll
+                    for (int m = 0; m < DT; ++m)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) v[m][e] += sums[(m * 16 + e) * 64];
+                }
             }
-            __syncthreads();
-            if (half == 0) {
-#pragma unroll
-                for (int m = 0; m < DT; ++m)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        if (a) va[m][e] += sums[(m * 16 + e) * 64];
-                        else ka[m][e] += sums[(m * 16 + e) * 64];
-                    }
-            }
-        }
-        if (half == 1) return;
+        };
+        join(ka);
+        join(va);
+        if (first_row != 0) return;
     }
     if (!here) return;
-    const int key = own + (lane & 31);
     // partial sums of the sinks: (sequence, head), part, sink, kb and vb, the head's values
-    const int64_t far_at = (((int64_t)(j - 1) * p.heads + kvh) * p.far_parts * s.sinks + key) * 2 * p.d, far_next = (int64_t)s.sinks * 2 * p.d;
+    const int64_t far_at = ((int64_t)(j - 1) * p.heads + kvh) * p.far_parts * s.sinks * 2 * p.d, far_next = (int64_t)s.sinks * 2 * p.d;
     if constexpr (FAR) {
         if (key >= s.sinks) return;
-        float* out = p.far + far_at + tile * far_next;
+        float* out = p.far + far_at + tile * far_next + (int64_t)key * 2 * p.d;
+        store_part<DT>(out, p.d, ka);
+        store_part<DT>(out + p.d, p.d, va);
+        return;
+    }
+    if (split >= 0) {
+        float* out = p.part + ((int64_t)(blockIdx.x - p.whole) * kKeys + key - key0) * 2 * p.d;
+        store_part<DT>(out, p.d, ka);
+        store_part<DT>(out + p.d, p.d, va);
+        return;
+    }
+    if (p.far && q.real && key0 == 0 && key < s.sinks && kt.far_rows > 0) {
+        const float* in = p.far + far_at + (int64_t)key * 2 * p.d;   // (far_kernel has added the parts to the first)
 #pragma unroll
         for (int m = 0; m < DT; ++m)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int at = 32 * m + 8 * (e >> 2) + 4 * h + (e & 3);
-                if (at < p.d) {
-                    out[at] = ka[m][e];
-                    out[p.d + at] = va[m][e];
+            for (int g = 0; g < 4; ++g) {
+                const int at = 32 * m + 8 * g + 4 * h;
+                float a[4], b[4];
+                load_row(a, in + at, p.d - at);
+                load_row(b, in + p.d + at, p.d - at);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    ka[m][4 * g + e] += a[e];
+                    va[m][4 * g + e] += b[e];
                 }
             }
-        return;
-    }
-    if (p.far && q.real && key < s.sinks && key0 == 0) {
-        for (int f = 0; f < p.far_parts && f * far_step < far_rows; ++f) {
-            const float* in = p.far + far_at + f * far_next;
-#pragma unroll
-            for (int m = 0; m < DT; ++m)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int at = 32 * m + 8 * (e >> 2) + 4 * h + (e & 3);
-                    if (at < p.d) {
-                        ka[m][e] += in[at];
-                        va[m][e] += in[p.d + at];
-                    }
-                }
-        }
     }
     T* kb = p.kb ? (T*)p.kb + kcol * p.ldkb + hcol : nullptr;
     T* vb = p.vb ? (T*)p.vb + kcol * p.ldvb + hcol : nullptr;
@@ -485,6 +634,69 @@ __global__ __launch_bounds__(256 * kHalves<T>, kHalves<T>) void keys_kernel(Back
         }
 }
 
+// The far parts' sums of a sequence's sinks added to the first, in order: a block has a strip of (kb, vb) of a (sequence, head)
+__global__ __launch_bounds__(256) void far_kernel(Back p, int BM) {
+    const int strips = (p.seqs.sinks * 2 * p.d + 255) / 256, at = (blockIdx.x % strips) * 256 + threadIdx.x;
+    const int64_t pair = blockIdx.x / strips, next = (int64_t)p.seqs.sinks * 2 * p.d;
+    const KeyTile kt = key_tile(p.seqs, (int)(pair / p.heads) + 1, 0);
+    const int key = at / (2 * p.d), step = part_rows(kt.far_rows, p.far_parts, BM), parts = min(p.far_parts, (kt.far_rows + step - 1) / step);
+    if (key >= p.seqs.sinks || key >= kt.keys || !kt.q.real) return;
+    float* out = p.far + pair * p.far_parts * next + at;
+    float sum = 0.f;
+#pragma unroll 8
+    for (int f = 0; f < parts; ++f) sum += out[f * next];
+    if (parts > 1) *out = sum;
+}
+
+// The split tiles' sums added in order, and the sinks': a block has four of a tile's keys
+template <class T>
+__global__ __launch_bounds__(256) void join_kernel(Back p, int BM) {
+    const Seqs& s = p.seqs;
+    int64_t slot, tile;
+    int kvh;
+    const int64_t nth = blockIdx.x >> 5;
+    place_of(p.whole + nth, p.slots, p.heads, slot, kvh);
+    const int j = find_range(s.kstart, s.tk, 1, kKeys, s.n + 1, slot, tile);
+    const KeyTile kt = key_tile(s, j, tile);
+    const int rows = kt.r_end - kt.r_first, step = part_rows(rows, p.splits, BM);
+    const int64_t next = (int64_t)kKeys * 2 * p.d;
+    const int vecs = (2 * p.d + 3) / 4;
+    for (int i = threadIdx.x; i < 4 * vecs; i += 256) {
+        const int in_tile = (blockIdx.x & 31) * 4 + i / vecs, at = (i % vecs) * 4, key = kt.key0 + in_tile;
+        if (key >= kt.keys) continue;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f}, v[4];
+        const float* in = p.part + nth * p.splits * next + (int64_t)in_tile * 2 * p.d + at;
+        const int parts = min(p.splits, (rows + step - 1) / step);
+#pragma unroll 8
+        for (int n = 0; n < parts; ++n) {
+            load_row(v, in + n * next, 2 * p.d - at);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] += v[e];
+        }
+        if (p.far && kt.q.real && kt.key0 == 0 && key < s.sinks && kt.far_rows > 0) {
+            load_row(v, p.far + (((int64_t)(j - 1) * p.heads + kvh) * p.far_parts * s.sinks + key) * 2 * p.d + at, 2 * p.d - at);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] += v[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int x = at + e;
+            if (x >= 2 * p.d) break;
+            T* out = (T*)(x < p.d ? p.kb : p.vb);
+            if (!out) continue;
+            out += (kt.first + key) * (x < p.d ? p.ldkb : p.ldvb) + (int64_t)kvh * p.d + (x < p.d ? x : x - p.d);
+            const float w = x < p.d ? sum[e] * p.s : sum[e];
+            *out = (T)(p.add ? (float)*out + w : w);
+        }
+    }
+}
+
+int cu_count() {
+    int dev = 0, cus = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 256;
+    return cus > 0 ? cus : 256;
+}
+
 int32_t* error_flag(Workspace* ws) { return (int32_t*)(ws->dscalars + kErrFlagSlot); }
 
 template <class F>
@@ -494,8 +706,8 @@ int32_t with_width(int64_t d, F&& f) {
     return f(std::integral_constant<int, 4>{});
 }
 
-// blocks of far rows for each key head of a sequence: about two a CU in all
-constexpr int64_t kFarBlocks = 512;
+// blocks of far rows for each key head of a sequence: about one a CU in all
+constexpr int64_t kFarBlocks = 256;
 
 }  // namespace
 }  // namespace stade
@@ -528,17 +740,27 @@ int32_t stade_hip_attention_b(int64_t tx, const void* yb, int64_t ldyb, const vo
     if (!call.ok()) return call.error();
     Back p{yb, ldyb, y, ldy, lse, q, ldq, qb, ldqb, k, ldk, kb, ldkb, v, ldv, vb, ldvb, nullptr, seqs, (int)i_d, (int)i_k, (float)s, add != 0};
     p.seqs.flag = error_flag(call.ws);
-    p.magic = seqs.group > 1 ? (uint32_t)(((uint64_t)1 << 32) / seqs.group + 1) : 0;
+    p.magic = (uint32_t)((((uint64_t)1 << 31) + seqs.group - 1) / seqs.group);
     const bool far = sinks > 0 && window >= 0 && window < i_tk && (kb || vb);
     const size_t deltas = ((size_t)i_t * i_q * 4 + 256) / 256 * 256;
     const int64_t pairs = i_n * i_k, sink_bytes = (int64_t)std::max<int64_t>(sinks, 1) * 2 * i_d * 4;
-    char* work = (char*)scratch(deltas + (far ? (size_t)(std::max(pairs, kFarBlocks) * sink_bytes) : 0));
+    const size_t fars = far ? (size_t)(std::max(pairs, kFarBlocks) * sink_bytes) : 0;
+    // Tiles of keys that fill no whole round of the CUs go over as many blocks as make two rounds (a block has a CU to
+    // itself), or as have six tiles of rows each.
+    const int64_t cus = cu_count(), slots = slots_of(i_tk, 1, kKeys, i_n + 1), units = slots * i_k;
+    p.whole = units / cus * cus;
+    const int64_t rest = units - p.whole, longest = std::min<int64_t>(i_t, (int64_t)seqs.window + kKeys) * seqs.group;
+    p.splits = rest ? (int)std::min<int64_t>(2 * cus / rest, std::max<int64_t>(1, longest / (6 * 32 * 2))) : 1;
+    if (p.splits <= 1) p.whole = units;
+    const size_t parts = (kb || vb) && i_t > 0 ? (size_t)(2 * cus) * kKeys * 2 * kMostHead * 4 : 0;
+    char* work = (char*)scratch(deltas + fars + parts);
     if (!work) return scratch_error();
     p.delta = (float*)work;
     if (far) {
         p.far = (float*)(work + deltas);
         p.far_parts = (int)std::max<int64_t>(1, kFarBlocks / std::max<int64_t>(pairs, 1));
     }
+    p.part = (float*)(work + deltas + fars);
     return with_type(tx, [&](auto t) -> int32_t {
         return with_width(i_d, [&](auto dt) -> int32_t {
             using T = decltype(t);
@@ -556,20 +778,27 @@ int32_t stade_hip_attention_b(int64_t tx, const void* yb, int64_t ldyb, const vo
                 STADE_LAUNCHED("attention rows_kernel");
             }
             if ((kb || vb) && i_tk > 0) {
-                constexpr unsigned NT = 256 * kHalves<T>;
+                constexpr unsigned NT = 64 * kGroups<T, false> * kRowWaves<T, false>, NTF = 64 * kGroups<T, true> * kRowWaves<T, true>;
                 if (far) {
                     STADE_TIMED("attention_b_sinks", stream, {
-                        if (direct) keys_kernel<T, DT, true, true><<<(unsigned)(pairs * p.far_parts), NT, 0, stream>>>(p);
-                        else keys_kernel<T, DT, false, true><<<(unsigned)(pairs * p.far_parts), NT, 0, stream>>>(p);
+                        if (direct) keys_kernel<T, DT, true, true><<<dim3((unsigned)(pairs * p.far_parts), sinks > 32 ? 2 : 1), NTF, 0, stream>>>(p);
+                        else keys_kernel<T, DT, false, true><<<dim3((unsigned)(pairs * p.far_parts), sinks > 32 ? 2 : 1), NTF, 0, stream>>>(p);
                     });
                     STADE_LAUNCHED("attention keys_kernel (sinks)");
+                    STADE_TIMED("attention_b_sinks", stream, far_kernel<<<(unsigned)(pairs * ((sinks * 2 * i_d + 255) / 256)), 256, 0, stream>>>(p, (kTileRows<T, true>)));
+                    STADE_LAUNCHED("attention far_kernel");
                 }
-                p.slots = slots_of(i_tk, 1, kKeys, i_n + 1);
+                p.slots = slots;
+                const unsigned grid = (unsigned)(p.whole + (units - p.whole) * p.splits);
                 STADE_TIMED("attention_b_keys", stream, {
-                    if (direct) keys_kernel<T, DT, true, false><<<(unsigned)(p.slots * i_k), NT, 0, stream>>>(p);
-                    else keys_kernel<T, DT, false, false><<<(unsigned)(p.slots * i_k), NT, 0, stream>>>(p);
+                    if (direct) keys_kernel<T, DT, true, false><<<grid, NT, 0, stream>>>(p);
+                    else keys_kernel<T, DT, false, false><<<grid, NT, 0, stream>>>(p);
                 });
                 STADE_LAUNCHED("attention keys_kernel");
+                if (p.whole < units) {
+                    STADE_TIMED("attention_b_join", stream, join_kernel<T><<<(unsigned)(32 * (units - p.whole)), 256, 0, stream>>>(p, (kTileRows<T, false>)));
+                    STADE_LAUNCHED("attention join_kernel");
+                }
             }
             return STADE_HIP_OK;
         });
