@@ -9,9 +9,8 @@
 // type (to nearest: like v, they are one factor of a product, whose sum is fp32) and are, as they lie in registers, the other operand of
 // V^T P, whose V^T comes from the row-major tile by the transposing LDS read: they never go through LDS.
 //
-// Two forms.  Wide: four waves of 32 rows each share tiles of 64 keys, double-buffered.  Narrow, for few rows a sequence
-// (single tokens): bound by reading k and v.  A block has 32 rows, its four waves take tiles of 32 keys in turn, each with
-// buffers of its own and no barrier, and a sequence's keys go over several blocks, whose parts a
+// A block has 128 rows, four waves of 32, which share tiles of 64 keys and values in two buffers.  Where the rows do not make two
+// blocks a CU (single tokens, chunks behind a long context) the keys of each go over several blocks, whose maxima, sums and values a
 // second launch joins in order.
 #include "attention.hpp"
 
@@ -34,14 +33,11 @@ struct Att {
     int d, heads;          // of the keys
     float s;               // the scores' factor, made positive (`negate`: q's sign is turned)
     int negate;
-    int64_t slots;         // of rows (wide, and narrow for long sequences)
-    // narrow: slots of keys, `chunk` keys each, or (chunk 0) `parts` of each sequence
-    int64_t key_slots;
-    int chunk, parts;
-    float* part;           // a block's rows: 32 x (d values, m, l)
+    int64_t slots;         // tiles of rows
+    int splits;            // blocks that share a tile's keys
+    float* part;           // their sums, where there are several: by block and row, d values, the maximum and the sum
 };
 
-constexpr int kNarrow = 32;      // rows of a narrow block
 constexpr float kGrow = 8.f;     // of the maximum, in the exponent of 2, before sums are scaled
 
 // a lane's query
@@ -250,6 +246,7 @@ __device__ __forceinline__ void place_of(int64_t block, int64_t slots, int heads
 }
 
 constexpr int kWideRows = 128, kWideKeys = 64;
+constexpr int64_t kSplitBlocks = 1024;
 
 template <class T, int DT, bool DIRECT>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void wide_kernel(Att p) {
@@ -258,7 +255,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void wide_kernel(Att p
     using R = Sums<T, DT, BN / 32>;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TILE];   // two tiles of keys, two of values
     const Seqs& s = p.seqs;
-    check_offsets(s, blockIdx.x, gridDim.x);
+    if (blockIdx.y == 0) check_offsets(s, blockIdx.x, gridDim.x);
     int64_t slot, tile;
     int kvh;
     place_of(blockIdx.x, p.slots, p.heads, slot, kvh);
@@ -270,7 +267,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void wide_kernel(Att p
     if (tile >= tiles) return;
     const int r0 = uniform((int)(tiles - 1 - tile) * kWideRows);
     if (!q.real) {
-        store_nothing<T>(p, q, kvh, r0, kWideRows);
+        if (blockIdx.y == 0) store_nothing<T>(p, q, kvh, r0, kWideRows);
         return;
     }
     const int wave = uniform((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
@@ -284,13 +281,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void wide_kernel(Att p
     row_fragments<T, DT, DIRECT>(sums.q, (const T*)p.q + w.t * p.ldq + (int64_t)w.head * p.d, w.here, p.d);
     if (p.negate) negate_all<T>(sums.q, sums.FR);
     const Range range = seen_by(s, p0, p1);
-    const KeyTiles<BN> keys(range);
+    const KeyTiles<BN> all(range);
+    // this block's share of the tiles of keys
+    const int share = (all.count + p.splits - 1) / p.splits, i_first = min((int)blockIdx.y * share, all.count), count = min(share, all.count - i_first);
+    if (blockIdx.y > 0 && count <= 0) return;
     const T* k = (const T*)p.k + q.k0 * p.ldk + (int64_t)kvh * p.d;
     const T* v = (const T*)p.v + q.k0 * p.ldv + (int64_t)kvh * p.d;
     const float c = p.s * kLog2e;
     S sk(p.ldk, p.d, threadIdx.x), sv(p.ldv, p.d, threadIdx.x);
     auto load = [&](S& st, const T* from_row, int64_t ld, int i, char* at) INLINE {
-        const int key = keys.key(i);
+        const int key = all.key(i_first + i);
         int from, to;
         tile_rows<BN>(range, key, from, to);
         st.load(from_row + key * ld, from, to, at);
@@ -299,12 +299,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void wide_kernel(Att p
     // keys lie two tiles ahead of the values' sums, values one.
     char* const kt[2] = {lds, lds + TILE};
     char* const vt[2] = {lds + 2 * TILE, lds + 3 * TILE};
-    if (keys.count > 0) {
+    if (count > 0) {
         load(sk, k, p.ldk, 0, kt[0]);
         load(sv, v, p.ldv, 0, vt[0]);
         sk.store(kt[0]);
         sv.store(vt[0]);
-        if (keys.count > 1) {
+        if (count > 1) {
             load(sk, k, p.ldk, 1, kt[1]);
             sk.store(kt[1]);
         }
@@ -313,30 +313,61 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void wide_kernel(Att p
     settle_loads();
     __syncthreads();
     typename R::Scores a, b;
-    if (keys.count > 0 && working) sums.scores(a, kt[0]);
+    if (count > 0 && working) sums.scores(a, kt[0]);
     __syncthreads();
     auto step = [&](auto parity, typename R::Scores& now, typename R::Scores& next, int i) INLINE {
         constexpr int P = decltype(parity)::value;
-        if (i + 2 < keys.count) load(sk, k, p.ldk, i + 2, kt[P]);
-        if (i + 1 < keys.count) load(sv, v, p.ldv, i + 1, vt[1 - P]);
+        if (i + 2 < count) load(sk, k, p.ldk, i + 2, kt[P]);
+        if (i + 1 < count) load(sv, v, p.ldv, i + 1, vt[1 - P]);
         if (working) {
-            sums.hide(now, keys.key(i), s, w.pos, w0, w1);
+            sums.hide(now, all.key(i_first + i), s, w.pos, w0, w1);
             sums.raise(now, c);
             sums.scores(next, kt[1 - P]);      // (behind the last tile: of what lies there, for nothing)
             sums.add(now, vt[P], c);
             if constexpr (sizeof(T) == 2) R::order();
         }
-        if (i + 2 < keys.count) sk.store(kt[P]);
-        if (i + 1 < keys.count) sv.store(vt[1 - P]);
+        if (i + 2 < count) sk.store(kt[P]);
+        if (i + 1 < count) sv.store(vt[1 - P]);
         if constexpr (DIRECT) wait_loads<0>();
         __syncthreads();
     };
-    for (int i = 0; i < keys.count; i += 2) {
+    for (int i = 0; i < count; i += 2) {
         step(std::integral_constant<int, 0>{}, a, b, i);
-        if (i + 1 < keys.count) step(std::integral_constant<int, 1>{}, b, a, i + 1);
+        if (i + 1 < count) step(std::integral_constant<int, 1>{}, b, a, i + 1);
     }
     const float l = sums.l + other_half(sums.l);
-    if (any_not_finite<DT>(sums.o)) {
+    const bool odd = any_not_finite<DT>(sums.o);
+    if (p.splits > 1) {
+        float* part = p.part + (((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kWideRows + 32 * wave) * (p.d + 2);
+        if (odd) {   // (no row sees a key between the tiles of sinks and those of the window)
+            const int from = all.key(i_first), to = all.key(i_first + count - 1) + BN;
+            exact_rows<T>(p, q, kvh, r0 + 32 * wave, from, to, [&](const Row& x, float m, float sum, Two o) INLINE {
+                float* at = part + (int64_t)((int)(x.t - q.q0) * s.group + x.head - kvh * s.group - (r0 + 32 * wave)) * (p.d + 2);
+                store_two(at, o.a, o.b, p.d, false);
+                if (lane == 0) {
+                    at[p.d] = m;
+                    at[p.d + 1] = sum;
+                }
+            });
+            return;
+        }
+        if (!w.here) return;
+        const int h = lane >> 5;
+        part += (lane & 31) * (p.d + 2);
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int col = 32 * i + 8 * g + 4 * h;
+                store4(part + col, sums.o[i][4 * g], sums.o[i][4 * g + 1], sums.o[i][4 * g + 2], sums.o[i][4 * g + 3], p.d - col);
+            }
+        if (h == 0) {
+            part[p.d] = sums.m == -INFINITY ? sums.m : sums.m * p.s;
+            part[p.d + 1] = l;
+        }
+        return;
+    }
+    if (odd) {
         exact_rows<T>(p, q, kvh, r0 + 32 * wave, 0, q.nk, [&](const Row& x, float m, float sum, Two o) INLINE {
             const float inv = 1.f / sum;
             store_two((T*)p.y + x.t * p.ldy + (int64_t)x.head * p.d, o.a * inv, o.b * inv, p.d, false);
@@ -345,6 +376,49 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void wide_kernel(Att p
         return;
     }
     store_rows<T, DT>(p, sums.o, w, sums.m, l);
+}
+
+// The blocks' sums of a row joined in order: a wave has eight rows, one after the other
+constexpr int kJoinRows = 32;
+template <class T>
+__global__ __launch_bounds__(256) void join_kernel(Att p, int64_t blocks) {
+    const Seqs& s = p.seqs;
+    const int lane = threadIdx.x & 63, wave = uniform((int)(threadIdx.x >> 6));
+    const int64_t block = blockIdx.x / (kWideRows / kJoinRows);
+    const int first = (int)(blockIdx.x % (kWideRows / kJoinRows)) * kJoinRows + wave;
+    int64_t slot, tile;
+    int kvh;
+    place_of(block, p.slots, p.heads, slot, kvh);
+    const int j = find_range(s.qstart, s.t, s.group, kWideRows, s.n + 1, slot, tile);
+    const Seq q = sequence(s, j - 1);
+    const int rows = q.nq * s.group, tiles = (rows + kWideRows - 1) / kWideRows;
+    if (tile >= tiles || !q.real) return;
+    const int r0 = (int)(tiles - 1 - tile) * kWideRows;
+    // (as the blocks counted them)
+    const KeyTiles<kWideKeys> keys(seen_by(s, r0 / s.group + q.shift(), min(r0 + kWideRows - 1, rows - 1) / s.group + q.shift()));
+    const int share = (keys.count + p.splits - 1) / p.splits, parts = max(1, share ? (keys.count + share - 1) / share : 1);
+    const int64_t next = blocks * kWideRows * (p.d + 2);
+    for (int in = first; in < first + kJoinRows; in += 4) {
+        const Row w = head_row(q, s, kvh, r0 + in);
+        if (!w.here) return;
+        const float* part = p.part + (block * kWideRows + in) * (p.d + 2);
+        float m = -INFINITY, l = 0.f;
+        Two o{0.f, 0.f};
+#pragma unroll 4
+        for (int n = 0; n < parts; ++n) {
+            const float* at = part + n * next;
+            const Two v = load_two(at, p.d);
+            const float mn = at[p.d], ln = at[p.d + 1], top = fmaxf(m, mn);
+            const float f = m == -INFINITY ? 0.f : exp2f((m - top) * kLog2e), e = mn == -INFINITY ? 0.f : exp2f((mn - top) * kLog2e);
+            m = top;
+            l = fmaf(l, f, ln * e);
+            o.a = fmaf(o.a, f, v.a * e);
+            o.b = fmaf(o.b, f, v.b * e);
+        }
+        const float inv = l != 0.f ? 1.f / l : 0.f;     // (a NaN stays one)
+        store_two((T*)p.y + w.t * p.ldy + (int64_t)w.head * p.d, o.a * inv, o.b * inv, p.d, false);
+        if (p.lse && lane == 0) p.lse[w.t * (p.heads * s.group) + w.head] = l != 0.f ? m + logf(l) : -INFINITY;
+    }
 }
 
 int32_t* error_flag(Workspace* ws) { return (int32_t*)(ws->dscalars + kErrFlagSlot); }
@@ -380,6 +454,16 @@ int32_t stade_hip_attention(int64_t tx, void* y, int64_t ldy, float* lse, const 
     Att p{y, ldy, lse, q, ldq, k, ldk, v, ldv, seqs, (int)i_d, (int)i_k, (float)fabs(s), s < 0.0};
     p.seqs.flag = error_flag(call.ws);
     p.slots = slots_of(i_t, p.seqs.group, kWideRows, i_n + 1);
+    // Blocks for two rounds of two a CU, eight tiles of keys each (a tile takes a microsecond, the second launch with what it reads some
+    // ten), and no more than 32 (which the second launch reads one after the other).  A sequence is taken to be up to twice as long as the
+    // mean.  One token of 8192 keys, 8 key heads: 135 us alone, 22 by 16 blocks; of 65536: 1167 and 75 by 32; 4 chunks of 512 behind
+    // 8192, 4 key heads: 319 and 229 by three; 2 prompts of 300, 2 key heads: 17, and 25 by two.
+    // (Two slots more than sequences, for columns of none, usually are empty.)
+    const int64_t blocks = p.slots * i_k, full = std::max<int64_t>(1, (p.slots - 2) * i_k);
+    const int64_t longest = std::min({i_tk, 2 * i_tk / std::max<int64_t>(i_n, 1) + 1, (int64_t)seqs.window + kMostSinks + kWideRows});
+    p.splits = (int)std::max<int64_t>(1, std::min({kSplitBlocks / full, 2 * kSplitBlocks / blocks, longest / (8 * kWideKeys), (int64_t)32}));
+    // (as much as any call takes, so that each is captured after an eager one)
+    if (p.splits > 1 && !(p.part = (float*)scratch((size_t)2 * kSplitBlocks * kWideRows * (kMostHead + 2) * 4))) return scratch_error();
     return with_type(tx, [&](auto t) -> int32_t {
         return with_width(i_d, [&](auto dt) -> int32_t {
             using T = decltype(t);
@@ -387,10 +471,14 @@ int32_t stade_hip_attention(int64_t tx, void* y, int64_t ldy, float* lse, const 
             const int64_t size = sizeof(T);
             const bool direct = straight(q, ldq, i_d, size) && straight(k, ldk, i_d, size) && straight(v, ldv, i_d, size);
             STADE_TIMED("attention", stream, {
-                if (direct) wide_kernel<T, DT, true><<<(unsigned)(p.slots * i_k), 256, 0, stream>>>(p);
-                else wide_kernel<T, DT, false><<<(unsigned)(p.slots * i_k), 256, 0, stream>>>(p);
+                if (direct) wide_kernel<T, DT, true><<<dim3((unsigned)blocks, p.splits), 256, 0, stream>>>(p);
+                else wide_kernel<T, DT, false><<<dim3((unsigned)blocks, p.splits), 256, 0, stream>>>(p);
             });
             STADE_LAUNCHED("attention wide_kernel");
+            if (p.splits > 1) {
+                STADE_TIMED("attention_join", stream, join_kernel<T><<<(unsigned)(blocks * (kWideRows / kJoinRows)), 256, 0, stream>>>(p, blocks));
+                STADE_LAUNCHED("attention join_kernel");
+            }
             return STADE_HIP_OK;
         });
     });

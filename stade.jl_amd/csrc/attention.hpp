@@ -187,7 +187,7 @@ __device__ __forceinline__ void wait_loads() {
 }
 // Before a loop that counts its own loads: what the compiler's loads brought into registers is there, in a form that the
 // compiler sees.  Without it the compiler waits for them at their first use inside the loop, in every round, and with them
-// for all that is under way to LDS (the forward sweep at 16500 tokens: 390 us for ...).
+// for all that is under way to LDS.
 __device__ __forceinline__ void settle_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }   // vmcnt(0)
 // before a buffer is written again: this wave's reads of it are through
 __device__ __forceinline__ void wait_reads() {
