@@ -27,7 +27,7 @@ using namespace rows;
 constexpr int NT = 256;
 constexpr int64_t kMostHead = 256, kMostHeads = 4096;
 constexpr int kTable = 2048;      // pairs' cosines and sines in LDS (16 KB)
-constexpr unsigned kSumParts = 1024;   // blocks that leave partial sums, at most
+constexpr int64_t kSumParts = 1024;    // blocks that leave partial sums, at most
 
 struct Rot {
     const void* x; int64_t ldx;
@@ -35,13 +35,14 @@ struct Rot {
     const void* yb; int64_t ldyb;       // (the adjoint)
     const void* gq; const void* gk; int gtype;
     const int64_t* pos; const double* freq;
-    float* part;                        // (the adjoint) a block's sums: gqb and gkb, 2 d values; null without them
+    float* part;                        // (the adjoint) a block's sums of its weights' shadow; null without them
     int d, nq, nk, r;
     int64_t t;
     int tile;                           // tokens of a block at a time
     int log_lanes;                      // lanes of a head
     float eps, s;
     int add;
+    int q_blocks;                       // blocks for queries; the rest are for keys
 };
 
 __device__ __forceinline__ float weight(const void* g, int type, int i) {
@@ -117,96 +118,145 @@ __device__ __forceinline__ void fill_table(const Rot& p, int64_t first, int toke
     }
 }
 
-template <class T, int V>
-__device__ __forceinline__ void load_heads_row(float (&a)[V], float (&b)[V], const void* x, int64_t at, const Cols& c) {
-    load_row(a, (const T*)x + at + c.a, c.na);
-    load_row(b, (const T*)x + at + c.b, c.nb);
+// A lane's two vectors of a head as they come from memory, so that the next head's are on their way while this one's
+// are worked on.  WHOLE: vectors are full or empty.
+template <class T, int V, bool WHOLE>
+struct Raw {
+    typedef typename Pack<T, V>::vec vec;
+    vec a, b;
+    static __device__ __forceinline__ void get(vec& v, const T* at, int left) {
+        v = vec{};
+        if (WHOLE ? left > 0 : left >= V) {
+            v = *reinterpret_cast<const typename Pack<T, V>::loose*>(at);
+        } else if constexpr (!WHOLE) {
+            if (left > 0) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[i] = i < left ? at[i] : (T)0.f;
+            }
+        }
+    }
+    __device__ __forceinline__ void load(const void* x, int64_t at, const Cols& c) {
+        get(a, (const T*)x + at + c.a, c.na);
+        get(b, (const T*)x + at + c.b, c.nb);
+    }
+    __device__ __forceinline__ void values(float (&u)[V], float (&w)[V]) const {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            u[i] = (float)a[i];
+            w[i] = (float)b[i];
+        }
+    }
+};
+
+// What a block works on: queries' heads, or keys' (the last blocks), which have weights of their own
+struct Part {
+    int first, heads;       // of the heads
+    const void* g;
+    int64_t block, blocks;  // among those of its kind
+};
+__device__ __forceinline__ Part my_part(const Rot& p) {
+    if ((int)blockIdx.x < p.q_blocks) return Part{0, p.nq, p.gq, blockIdx.x, p.q_blocks};
+    return Part{p.nq, p.nk, p.gk, blockIdx.x - p.q_blocks, gridDim.x - p.q_blocks};
 }
 
-template <class T, int V, bool HALF, bool NORM>
+template <class T, int V, bool HALF, bool NORM, bool WHOLE>
 __global__ __launch_bounds__(NT) void forward_kernel(Rot p) {
     __shared__ float2 table[kTable];
-    const int log = p.log_lanes, lane = threadIdx.x & ((1 << log) - 1), heads = p.nq + p.nk;
+    const Part part = my_part(p);
+    const int log = p.log_lanes, lane = threadIdx.x & ((1 << log) - 1), heads = part.heads, step = gridDim.y * (NT >> log);
     const Cols c = my_cols<HALF, V>(lane, p.d, p.r);
     const int stride = (p.r / 2 + V - 1) / V * V;
-    float gq[2][V], gk[2][V];
+    float g[2][V];
     if constexpr (NORM) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            gq[0][i] = i < c.na ? weight(p.gq, p.gtype, c.a + i) : 0.f;
-            gq[1][i] = i < c.nb ? weight(p.gq, p.gtype, c.b + i) : 0.f;
-            gk[0][i] = i < c.na ? weight(p.gk, p.gtype, c.a + i) : 0.f;
-            gk[1][i] = i < c.nb ? weight(p.gk, p.gtype, c.b + i) : 0.f;
+            g[0][i] = i < c.na ? weight(part.g, p.gtype, c.a + i) : 0.f;
+            g[1][i] = i < c.nb ? weight(part.g, p.gtype, c.b + i) : 0.f;
         }
     }
-    for (int64_t first = (int64_t)blockIdx.x * p.tile; first < p.t; first += (int64_t)gridDim.x * p.tile) {
+    for (int64_t first = part.block * p.tile; first < p.t; first += part.blocks * p.tile) {
         const int tokens = (int)min((int64_t)p.tile, p.t - first), units = tokens * heads;
+        Raw<T, V, WHOLE> next;
+        auto fetch = [&](int u) __attribute__((always_inline)) {
+            const int k = u / heads, h = u - k * heads;
+            if (u < units) next.load(p.x, (first + k) * p.ldx + (int64_t)(part.first + h) * p.d, c);
+        };
+        int u = (blockIdx.y * NT + threadIdx.x) >> log;
+        fetch(u);
         __syncthreads();
         fill_table(p, first, tokens, stride, table);
         __syncthreads();
-        for (int u = (blockIdx.y * NT + threadIdx.x) >> log; u < units; u += gridDim.y * (NT >> log)) {
+        for (; u < units; u += step) {
             const int k = u / heads, h = u - k * heads;
-            const int64_t col = (int64_t)h * p.d;
             float a[V], b[V];
-            load_heads_row<T>(a, b, p.x, (first + k) * p.ldx + col, c);
+            next.values(a, b);
+            fetch(u + step);
             if constexpr (NORM) {
                 float sq = 0.f;
 #pragma unroll
                 for (int i = 0; i < V; ++i) sq = fmaf(a[i], a[i], fmaf(b[i], b[i], sq));
                 sq = head_sum(sq, log);
                 const float rs = 1.0f / sqrtf(sq / (float)p.d + p.eps);
-                const bool q = h < p.nq;
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    a[i] = a[i] * rs * (q ? gq[0][i] : gk[0][i]);
-                    b[i] = b[i] * rs * (q ? gq[1][i] : gk[1][i]);
+                    a[i] = a[i] * rs * g[0][i];
+                    b[i] = b[i] * rs * g[1][i];
                 }
             }
             if (c.turn) turn<HALF, false>(a, b, table + k * stride + c.pair);
-            T* y = (T*)p.y + (first + k) * p.ldy + col;
-            store_row(y + c.a, a, c.na);
-            store_row(y + c.b, b, c.nb);
+            T* y = (T*)p.y + (first + k) * p.ldy + (int64_t)(part.first + h) * p.d;
+            store_row<WHOLE>(y + c.a, a, c.na);
+            store_row<WHOLE>(y + c.b, b, c.nb);
         }
     }
 }
 
-template <class T, int V, bool HALF, bool NORM>
+template <class T, int V, bool HALF, bool NORM, bool WHOLE>
 __global__ __launch_bounds__(NT) void backward_kernel(Rot p) {
     __shared__ float2 table[kTable];
-    __shared__ float sums[2 * kMostHead];
-    const int log = p.log_lanes, lane = threadIdx.x & ((1 << log) - 1), heads = p.nq + p.nk;
+    __shared__ float sums[kMostHead];
+    const Part part = my_part(p);
+    const int log = p.log_lanes, lane = threadIdx.x & ((1 << log) - 1), heads = part.heads, step = NT >> log;
     const Cols c = my_cols<HALF, V>(lane, p.d, p.r);
     const int stride = (p.r / 2 + V - 1) / V * V;
-    float g[2][2][V], acc[2][2][V];     // (queries and keys, the two vectors)
+    float g[2][V], acc[2][V];
     if constexpr (NORM) {
 #pragma unroll
-        for (int w = 0; w < 2; ++w)
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                g[w][0][i] = i < c.na ? weight(w ? p.gk : p.gq, p.gtype, c.a + i) : 0.f;
-                g[w][1][i] = i < c.nb ? weight(w ? p.gk : p.gq, p.gtype, c.b + i) : 0.f;
-                acc[w][0][i] = acc[w][1][i] = 0.f;
-            }
+        for (int i = 0; i < V; ++i) {
+            g[0][i] = i < c.na ? weight(part.g, p.gtype, c.a + i) : 0.f;
+            g[1][i] = i < c.nb ? weight(part.g, p.gtype, c.b + i) : 0.f;
+            acc[0][i] = acc[1][i] = 0.f;
+        }
     }
-    for (int64_t first = (int64_t)blockIdx.x * p.tile; first < p.t; first += (int64_t)gridDim.x * p.tile) {
+    for (int64_t first = part.block * p.tile; first < p.t; first += part.blocks * p.tile) {
         const int tokens = (int)min((int64_t)p.tile, p.t - first), units = tokens * heads;
+        Raw<T, V, WHOLE> next, next_x;
+        auto fetch = [&](int u) __attribute__((always_inline)) {
+            const int k = u / heads, h = u - k * heads;
+            const int64_t col = (int64_t)(part.first + h) * p.d;
+            if (u < units) {
+                next.load(p.yb, (first + k) * p.ldyb + col, c);
+                if constexpr (NORM) next_x.load(p.x, (first + k) * p.ldx + col, c);
+            }
+        };
+        int u = threadIdx.x >> log;
+        fetch(u);
         __syncthreads();
         fill_table(p, first, tokens, stride, table);
         __syncthreads();
-        for (int u = threadIdx.x >> log; u < units; u += NT >> log) {
+        for (; u < units; u += step) {
             const int k = u / heads, h = u - k * heads;
-            const int64_t col = (int64_t)h * p.d;
             float a[V], b[V], xa[V], xb[V];
-            load_heads_row<T>(a, b, p.yb, (first + k) * p.ldyb + col, c);
-            if constexpr (NORM) load_heads_row<T>(xa, xb, p.x, (first + k) * p.ldx + col, c);
+            next.values(a, b);
+            if constexpr (NORM) next_x.values(xa, xb);
+            fetch(u + step);
             if (c.turn) turn<HALF, true>(a, b, table + k * stride + c.pair);
             if constexpr (NORM) {
-                const int w = h < p.nq ? 0 : 1;
                 float sq = 0.f, dot = 0.f, ga[V], gb[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    ga[i] = a[i] * (w ? g[1][0][i] : g[0][0][i]);
-                    gb[i] = b[i] * (w ? g[1][1][i] : g[0][1][i]);
+                    ga[i] = a[i] * g[0][i];
+                    gb[i] = b[i] * g[1][i];
                     sq = fmaf(xa[i], xa[i], fmaf(xb[i], xb[i], sq));
                     dot = fmaf(ga[i], xa[i], fmaf(gb[i], xb[i], dot));
                 }
@@ -216,69 +266,68 @@ __global__ __launch_bounds__(NT) void backward_kernel(Rot p) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     const float ha = xa[i] * rs, hb = xb[i] * rs;
-                    const float wa = a[i] * ha, wb = b[i] * hb;
-                    acc[0][0][i] += w ? 0.f : wa;
-                    acc[0][1][i] += w ? 0.f : wb;
-                    acc[1][0][i] += w ? wa : 0.f;
-                    acc[1][1][i] += w ? wb : 0.f;
+                    acc[0][i] = fmaf(a[i], ha, acc[0][i]);
+                    acc[1][i] = fmaf(b[i], hb, acc[1][i]);
                     a[i] = rs * fmaf(-ha, m, ga[i]);
                     b[i] = rs * fmaf(-hb, m, gb[i]);
                 }
             }
             if (p.y) {
-                T* y = (T*)p.y + (first + k) * p.ldy + col;
+                T* y = (T*)p.y + (first + k) * p.ldy + (int64_t)(part.first + h) * p.d;
                 if (p.add) {
                     float oa[V], ob[V];
-                    load_row(oa, y + c.a, c.na);
-                    load_row(ob, y + c.b, c.nb);
+                    load_row<WHOLE>(oa, y + c.a, c.na);
+                    load_row<WHOLE>(ob, y + c.b, c.nb);
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
                         a[i] += oa[i];
                         b[i] += ob[i];
                     }
                 }
-                store_row(y + c.a, a, c.na);
-                store_row(y + c.b, b, c.nb);
+                store_row<WHOLE>(y + c.a, a, c.na);
+                store_row<WHOLE>(y + c.b, b, c.nb);
             }
         }
     }
     if constexpr (NORM) {
         if (!p.part) return;
-        // the block's groups of lanes joined, one after the other
-        for (int k = 0; k < NT >> log; ++k) {
+        // the block's groups of lanes joined: those of a wave by steps of twice as many, then the waves one after the other
+        for (int o = 1 << log; o < 64; o <<= 1)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                acc[0][i] += __shfl_xor(acc[0][i], o, 64);
+                acc[1][i] += __shfl_xor(acc[1][i], o, 64);
+            }
+        for (int k = 0; k < NT / 64; ++k) {
             __syncthreads();
-            if ((int)(threadIdx.x >> log) == k) {
+            if ((int)(threadIdx.x >> 6) == k && (int)(threadIdx.x & 63) == lane) {
 #pragma unroll
-                for (int w = 0; w < 2; ++w)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        if (i < c.na) sums[w * p.d + c.a + i] = (k ? sums[w * p.d + c.a + i] : 0.f) + acc[w][0][i];
-                        if (i < c.nb) sums[w * p.d + c.b + i] = (k ? sums[w * p.d + c.b + i] : 0.f) + acc[w][1][i];
-                    }
+                for (int i = 0; i < V; ++i) {
+                    if (i < c.na) sums[c.a + i] = (k ? sums[c.a + i] : 0.f) + acc[0][i];
+                    if (i < c.nb) sums[c.b + i] = (k ? sums[c.b + i] : 0.f) + acc[1][i];
+                }
             }
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < 2 * p.d; i += NT) p.part[(int64_t)blockIdx.x * 2 * p.d + i] = sums[i];
+        for (int i = threadIdx.x; i < p.d; i += NT) p.part[(int64_t)blockIdx.x * p.d + i] = sums[i];
     }
 }
 
-// gqb and gkb from the blocks' sums, in order: 16 columns a block, 16 strips of the blocks each
-__global__ __launch_bounds__(NT) void weight_sum_kernel(const float* part, int parts, int d, float* gqb, float* gkb, int add) {
+// gqb and gkb (blockIdx.y) from their blocks' sums, in order: 16 columns a block, 16 strips of the blocks each
+__global__ __launch_bounds__(NT) void weight_sum_kernel(const float* part, int q_blocks, int blocks, int d, float* gqb, float* gkb, int add) {
     __shared__ float lds[16][17];
     const int c = threadIdx.x & 15, strip = threadIdx.x >> 4, i = blockIdx.x * 16 + c;
+    const int from = blockIdx.y ? q_blocks : 0, to = blockIdx.y ? blocks : q_blocks;
     float v = 0.f;
-    if (i < 2 * d)
+    if (i < d)
 #pragma unroll 8
-        for (int b = strip; b < parts; b += 16) v += part[(int64_t)b * 2 * d + i];
+        for (int b = from + strip; b < to; b += 16) v += part[(int64_t)b * d + i];
     lds[strip][c] = v;
     __syncthreads();
-    if (strip == 0 && i < 2 * d) {
+    if (strip == 0 && i < d) {
         for (int k = 1; k < 16; ++k) v += lds[k][c];
-        float* out = i < d ? gqb : gkb;
-        if (out) {
-            out += i < d ? i : i - d;
-            *out = add ? *out + v : v;
-        }
+        float* out = blockIdx.y ? gkb : gqb;
+        if (out) out[i] = add ? out[i] + v : v;
     }
 }
 
@@ -300,10 +349,11 @@ int32_t check(const char* fn, int64_t tx, int64_t tg, const void* gq, const void
 }
 
 template <class F>
-int32_t with_form(int64_t tx, int64_t half, int64_t norm, F&& f) {
+int32_t with_form(int64_t tx, int64_t half, int64_t norm, bool whole, F&& f) {
     return with_type(tx, [&](auto t) -> int32_t {
-        if (half) return norm ? f(t, std::true_type{}, std::true_type{}) : f(t, std::true_type{}, std::false_type{});
-        return norm ? f(t, std::false_type{}, std::true_type{}) : f(t, std::false_type{}, std::false_type{});
+        auto with_whole = [&](auto h, auto n) -> int32_t { return whole ? f(t, h, n, std::true_type{}) : f(t, h, n, std::false_type{}); };
+        if (half) return norm ? with_whole(std::true_type{}, std::true_type{}) : with_whole(std::true_type{}, std::false_type{});
+        return norm ? with_whole(std::false_type{}, std::true_type{}) : with_whole(std::false_type{}, std::false_type{});
     });
 }
 
@@ -315,10 +365,22 @@ inline int log_lanes(int64_t type, int64_t d, int64_t r) {
     while ((1 << log) < lanes) ++log;
     return log;
 }
+// (two vectors of a lane are full or empty together, in both layouts)
+inline bool whole_vectors(int64_t type, int64_t d, int64_t r) {
+    const int v = values_of(type);
+    return r % (2 * v) == 0 && (d - r) % (2 * v) == 0;
+}
 // tokens of a block at a time: some eight rounds of its lanes, and a table that fits
 inline int tile_of(const Rot& p, int v) {
-    const int stride = std::max(1, (p.r / 2 + v - 1) / v * v), lanes = (p.nq + p.nk) << p.log_lanes;
+    const int stride = std::max(1, (p.r / 2 + v - 1) / v * v), lanes = std::max(p.nq, p.nk) << p.log_lanes;
     return std::max(1, std::min({kTable / stride, 8 * NT / lanes, 64}));
+}
+// `blocks` of them for all heads, as many for queries as they have of the heads
+inline void share(Rot& p, int64_t blocks, int64_t tiles, unsigned& grid) {
+    const int64_t heads = p.nq + p.nk, q = p.nq ? std::max<int64_t>(1, std::min(tiles, (blocks * p.nq + heads / 2) / heads)) : 0;
+    const int64_t k = p.nk ? std::max<int64_t>(1, std::min(tiles, blocks - q)) : 0;
+    p.q_blocks = (int)q;
+    grid = (unsigned)(q + k);
 }
 
 }  // namespace
@@ -359,17 +421,20 @@ int32_t stade_hip_head_rotary(int64_t tx, int64_t tg, void* y, int64_t ldy, cons
     WsCall call(stream, false);
     if (!call.ok()) return call.error();
     Rot p{x, ldx, y, ldy, nullptr, 0, gq, gk, (int)tg, pos, freq, nullptr, (int)i_d, (int)i_q, (int)i_k, (int)i_r, i_t, 1, log_lanes(tx, i_d, i_r),
-          (float)eps, (float)s, 0};
+          (float)eps, (float)s, 0, 0};
     // (Few tokens: a block for each, and its heads over as many blocks as have work for their lanes.)
-    const int64_t lanes = (i_q + i_k) << p.log_lanes;
+    const int64_t lanes = std::max(i_q, i_k) << p.log_lanes;
     const bool few = i_t <= 256;
     p.tile = few ? 1 : tile_of(p, values_of(tx));
     const unsigned parts = few ? (unsigned)std::min<int64_t>((lanes + NT - 1) / NT, 64) : 1;
-    const unsigned grid = (unsigned)std::min<int64_t>((i_t + p.tile - 1) / p.tile, 1 << 20);
-    return with_form(tx, half, norm, [&](auto t, auto h, auto n) -> int32_t {
+    const int64_t tiles = (i_t + p.tile - 1) / p.tile;
+    unsigned grid;
+    share(p, 2 * tiles, tiles, grid);
+    return with_form(tx, half, norm, whole_vectors(tx, i_d, i_r), [&](auto t, auto h, auto n, auto w) -> int32_t {
         using T = decltype(t);
         STADE_TIMED("head_rotary", stream,
-                    forward_kernel<T, 16 / sizeof(T), decltype(h)::value, decltype(n)::value><<<dim3(grid, parts), NT, 0, stream>>>(p));
+                    forward_kernel<T, 16 / sizeof(T), decltype(h)::value, decltype(n)::value, decltype(w)::value>
+                        <<<dim3(grid, parts), NT, 0, stream>>>(p));
         STADE_LAUNCHED("head_rotary forward_kernel");
         return STADE_HIP_OK;
     });
@@ -396,17 +461,19 @@ int32_t stade_hip_head_rotary_b(int64_t tx, int64_t tg, const void* yb, int64_t 
     WsCall call(stream, sums);   // (the workspace for the partial sums only)
     if (!call.ok()) return call.error();
     Rot p{x, ldx, xb, ldxb, yb, ldyb, gq, gk, (int)tg, pos, freq, nullptr, (int)i_d, (int)i_q, (int)i_k, (int)i_r, i_t, 1, log_lanes(tx, i_d, i_r),
-          (float)eps, (float)s, add != 0};
+          (float)eps, (float)s, add != 0, 0};
     p.tile = some ? tile_of(p, values_of(tx)) : 1;
     const int64_t tiles = (i_t + p.tile - 1) / p.tile;
-    const unsigned grid = (unsigned)std::min<int64_t>(tiles, sums ? kSumParts : 1 << 20);
+    unsigned grid = 0;
+    // (with sums not more blocks than they are added up fast; queries' and keys' shadows each have blocks of their own)
+    if (some) share(p, sums ? std::min<int64_t>(2 * tiles, kSumParts) : 2 * tiles, tiles, grid);
     // (as much as the largest call takes, so that any call is captured after an eager one)
-    if (sums && !(p.part = (float*)scratch((size_t)kSumParts * 2 * kMostHead * sizeof(float)))) return scratch_error();
+    if (sums && !(p.part = (float*)scratch((size_t)(kSumParts + 2) * kMostHead * sizeof(float)))) return scratch_error();
     if (some) {
-        const int32_t rc = with_form(tx, half, norm, [&](auto t, auto h, auto n) -> int32_t {
+        const int32_t rc = with_form(tx, half, norm, whole_vectors(tx, i_d, i_r), [&](auto t, auto h, auto n, auto w) -> int32_t {
             using T = decltype(t);
             STADE_TIMED("head_rotary_b", stream,
-                        backward_kernel<T, 16 / sizeof(T), decltype(h)::value, decltype(n)::value><<<grid, NT, 0, stream>>>(p));
+                        backward_kernel<T, 16 / sizeof(T), decltype(h)::value, decltype(n)::value, decltype(w)::value><<<grid, NT, 0, stream>>>(p));
             STADE_LAUNCHED("head_rotary backward_kernel");
             return STADE_HIP_OK;
         });
@@ -414,7 +481,8 @@ int32_t stade_hip_head_rotary_b(int64_t tx, int64_t tg, const void* yb, int64_t 
     }
     if (sums) {
         STADE_TIMED("head_rotary_sum", stream,
-                    weight_sum_kernel<<<(unsigned)((2 * i_d + 15) / 16), NT, 0, stream>>>(p.part, some ? (int)grid : 0, (int)i_d, gqb, gkb, add != 0));
+                    weight_sum_kernel<<<dim3((unsigned)((i_d + 15) / 16), 2), NT, 0, stream>>>(p.part, some ? p.q_blocks : 0, (int)grid, (int)i_d, gqb, gkb,
+                                                                                              add != 0));
         STADE_LAUNCHED("head_rotary weight_sum_kernel");
     }
     return STADE_HIP_OK;
