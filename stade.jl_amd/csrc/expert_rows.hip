@@ -25,6 +25,126 @@ constexpr int64_t kMostSlots = 64, kMostExperts = 4096;
 
 int32_t* error_flag(Workspace* ws) { return (int32_t*)(ws->dscalars + kErrFlagSlot); }
 
+// ------------------------------------------------------------------------------------------
+// the order, by counting (up to kFewExperts): every block has a stretch of the slots
+// ------------------------------------------------------------------------------------------
+constexpr int kOrderNT = 512, kOrderWaves = kOrderNT / 64, kStretch = 256 * kOrderWaves;   // slots of a block: four of a lane, wave after wave
+constexpr int kFewExperts = 1024, kBinsAThread = 3;
+constexpr int64_t kMostCounts = 1 << 16;     // of all blocks, as each block reads them all
+
+struct Order {
+    const int64_t* ids;
+    int64_t* order; int64_t* place; int64_t* start;
+    int e, n, blocks;
+    int32_t* counts;     // by block: e + 1 (the last: of no expert)
+    int32_t* flag;
+};
+__device__ __forceinline__ int bin_of(const Order& p, int64_t slot) {
+    const int64_t id = p.ids[slot];
+    if (id >= 1 && id <= p.e) return (int)(id - 1);
+    if (id != 0) *p.flag = kErrIndex;
+    return p.e;
+}
+// a wave's four stretches of 64 slots in their bins, counted
+__device__ __forceinline__ void count(const Order& p, int64_t first, int (&bin)[4], int* mine) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t slot = first + 64 * i + lane;
+        bin[i] = slot < p.n ? bin_of(p, slot) : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (bin[i] >= 0) atomicAdd(&mine[bin[i]], 1);     // (whole numbers: in any order the same)
+}
+
+__global__ __launch_bounds__(kOrderNT) void count_kernel(Order p) {
+    __shared__ int bins[kFewExperts + 1];
+    for (int i = threadIdx.x; i <= p.e; i += kOrderNT) bins[i] = 0;
+    __syncthreads();
+    int bin[4];
+    count(p, (int64_t)blockIdx.x * kStretch + (threadIdx.x >> 6) * 256, bin, bins);
+    __syncthreads();
+    for (int i = threadIdx.x; i <= p.e; i += kOrderNT) p.counts[(int64_t)blockIdx.x * (p.e + 1) + i] = bins[i];
+}
+
+// A slot's place: those of earlier experts, of its expert in earlier blocks, in earlier waves of the block, and before it in
+// its wave (64 slots at a time: the lanes whose bins' bits all agree).
+__global__ __launch_bounds__(kOrderNT) void order_kernel(Order p) {
+    __shared__ int bins[kOrderWaves][kFewExperts + 1];
+    __shared__ int sums[kOrderWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b0 = threadIdx.x * kBinsAThread;
+    for (int i = threadIdx.x; i < kOrderWaves * (kFewExperts + 1); i += kOrderNT) bins[0][i] = 0;
+    __syncthreads();
+    int bin[4];
+    count(p, (int64_t)blockIdx.x * kStretch + wave * 256, bin, bins[wave]);
+    __syncthreads();
+    // of this thread's bins: all slots, and those in earlier blocks
+    int all[kBinsAThread], before[kBinsAThread], total = 0;
+#pragma unroll
+    for (int i = 0; i < kBinsAThread; ++i) {
+        all[i] = before[i] = 0;
+        const int b = b0 + i;
+        if (b > p.e) continue;
+        if (p.blocks > 1) {
+#pragma unroll 8
+            for (int n = 0; n < p.blocks; ++n) {
+                const int c = p.counts[(int64_t)n * (p.e + 1) + b];
+                all[i] += c;
+                before[i] += n < (int)blockIdx.x ? c : 0;
+            }
+        } else {
+            for (int w = 0; w < kOrderWaves; ++w) all[i] += bins[w][b];
+        }
+        total += all[i];
+    }
+    int sum = total;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += up;
+    }
+    if (lane == 63) sums[wave] = sum;
+    __syncthreads();
+    int at = sum - total;
+    for (int w = 0; w < wave; ++w) at += sums[w];
+#pragma unroll
+    for (int i = 0; i < kBinsAThread; ++i) {
+        const int b = b0 + i;
+        if (b > p.e) continue;
+        if (blockIdx.x == 0) p.start[b] = at;          // (start[e]: where those of no expert begin)
+        int here = at + before[i];
+        for (int w = 0; w < kOrderWaves; ++w) {
+            const int c = bins[w][b];
+            bins[w][b] = here;
+            here += c;
+        }
+        at += all[i];
+    }
+    __syncthreads();
+    int* mine = bins[wave];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint64_t same = __ballot(bin[i] >= 0);
+        for (int bit = 0; (p.e >> bit) != 0; ++bit) {
+            const uint64_t set = __ballot(bin[i] >= 0 && (bin[i] >> bit & 1));
+            same &= bin[i] >> bit & 1 ? set : ~set;
+        }
+        const int64_t slot = (int64_t)blockIdx.x * kStretch + wave * 256 + 64 * i + lane;
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        int first = 0;
+        if (bin[i] >= 0) {
+            first = mine[bin[i]];
+            p.order[first + rank] = slot + 1;
+            p.place[slot] = bin[i] < p.e ? first + rank + 1 : 0;
+        }
+        // (all of the wave's reads come before the writes: it is one wave, and its LDS work goes in order)
+        __builtin_amdgcn_wave_barrier();
+        if (bin[i] >= 0 && rank == 0) mine[bin[i]] = first + __popcll(same);
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
 // the inverse of the order: slots behind the last expert's rows have no place
 __global__ __launch_bounds__(NT) void place_kernel(const int64_t* order, const int64_t* start, int64_t e, int64_t n, int64_t* place) {
     const int64_t here = start[e];
@@ -204,6 +324,21 @@ int32_t stade_hip_expert_order(const int64_t* ids, int64_t* order, int64_t* plac
     const int64_t n = i_k * i_t;
     if (int32_t rc = check_extent(fn, "i_k * i_t", n, kMostRows)) return rc;
     if (!start || (n > 0 && (!ids || !order || !place))) return bad(fn, "null pointer");
+    // Few experts: by counting, a launch or two (16384 slots of 64 experts: 7 us, by sorting 28).
+    const int64_t blocks = (n + kStretch - 1) / kStretch;
+    if (n > 0 && i_e <= kFewExperts && blocks * (i_e + 1) <= kMostCounts) {
+        WsCall call(stream);
+        if (!call.ok()) return call.error();
+        Order p{ids, order, place, start, (int)i_e, (int)n, (int)blocks, nullptr, error_flag(call.ws)};
+        if (blocks > 1) {
+            if (!(p.counts = (int32_t*)scratch(kMostCounts * sizeof(int32_t)))) return scratch_error();
+            STADE_TIMED("expert_count", stream, count_kernel<<<(unsigned)blocks, kOrderNT, 0, stream>>>(p));
+            STADE_LAUNCHED("expert_rows count_kernel");
+        }
+        STADE_TIMED("expert_order", stream, order_kernel<<<(unsigned)blocks, kOrderNT, 0, stream>>>(p));
+        STADE_LAUNCHED("expert_rows order_kernel");
+        return STADE_HIP_OK;
+    }
     if (int32_t rc = stade_hip_token_order(ids, order, start, i_e, n, stream)) return rc;
     if (n == 0) return STADE_HIP_OK;
     WsCall call(stream, false);
