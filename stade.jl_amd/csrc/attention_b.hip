@@ -2,7 +2,7 @@
 // with the heads of a group side by side), and delta = yb . y for each row:
 //   vb (+)= P^T yb,   S = P (yb v^T - delta),   qb (+)= s S k,   kb (+)= s S^T q
 // P is formed again from lse; nothing of the size of the scores is kept.  Two launches (three with sinks):
-//   rows_kernel   a block has 128 rows and goes over their keys: delta, and qb.  Scores as keys x rows, so that lse and
+//   rows_kernel   a block has 128 rows and goes over their keys: delta (as the sum of P (yb v^T), and yb . y), and qb.  Scores as keys x rows, so that lse and
 //                 delta are one value a lane, and S, rounded, is the operand of K^T S as it lies.
 //   keys_kernel   a block has 128 keys and goes over the rows that see them, all heads of the group: kb and vb.  Scores as
 //                 rows x keys; P and S are the operands of yb^T P and q^T S as they lie.
@@ -47,6 +47,7 @@ struct Back {
 };
 
 constexpr int kRows = 128, kKeys = 128;
+constexpr int kFewTiles = 4;      // of keys, where delta is formed from the weights
 
 
 template <class T>
@@ -113,9 +114,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void rows_kernel(Back 
             for (int i = 0; i < kCE<T>; ++i) delta = fmaf((float)a[i], (float)b[i], delta);
         }
         delta += other_half(delta);
-        if (here && h == 0) p.delta[t * (p.heads * s.group) + head] = delta;
     }
-    if (!p.qb) return;
     row_fragments<T, DT, DIRECT>(qf, (const T*)p.q + t * p.ldq + col, here, p.d);
     const int p0 = r0 / s.group + q.shift(), p1 = min(r0 + kRows - 1, rows - 1) / s.group + q.shift();
     const int w0 = uniform((r0 + 32 * wave) / s.group + q.shift()), w1 = uniform(min(r0 + 32 * wave + 31, rows - 1) / s.group + q.shift());
@@ -138,78 +137,108 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void rows_kernel(Back 
         sk.load(k + key * p.ldk, from, to, at);
         sv.load(v + key * p.ldv, from, to, at + TILE);
     };
-    if (keys.count > 0) {
-        load(0, lds);
-        sk.store(lds);
-        sv.store(lds + TILE);
-        if constexpr (DIRECT) wait_loads<0>();
-    }
-    settle_loads();
-    __syncthreads();
-    for (int i = 0; i < keys.count; ++i) {
-        char* now = lds + (i & 1) * 2 * TILE;
-        char* next = lds + (~i & 1) * 2 * TILE;
-        if (i + 1 < keys.count) load(i + 1, next);
-        const int key = keys.key(i);
-        if (working && ((key < mine.high && key + BN > mine.low) || key < mine.sinks)) {
-            const bool whole = key + BN - 1 <= w0 && (w1 - key < s.window || key + BN <= s.sinks);
-            const int high = pos - key - 4 * h, low = high - s.window, sink = s.sinks - key - 4 * h;
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                floatx16 x, g;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = g[e] = 0.f;
-#pragma unroll
-                for (int f = 0; f < FR; ++f) x = multiply<T>(along_head<T, DP>(now, 32 * b, f), qf[f], x);
-#pragma unroll
-                for (int f = 0; f < FR; ++f) g = multiply<T>(along_head<T, DP>(now + TILE, 32 * b, f), of[f], g);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], c, base)) * (g[e] - delta);
-                if (!whole) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int at = 32 * b + 8 * (e >> 2) + (e & 3);
-                        if (!(at <= high && (at > low || at < sink))) x[e] = 0.f;
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < kParts<T>; ++u) {
-                    const v4u part = part_of<T>(x, u);
-#pragma unroll
-                    for (int m = 0; m < DT; ++m) acc[m] = multiply<T>(along_rows<T, DP>(now, 32 * b + u * 2 * kCE<T>, 32 * m), part, acc[m]);
-                }
-            }
-        }
-        if (i + 1 < keys.count) {
-            sk.store(next);
-            sv.store(next + TILE);
+    // yb . y is delta but for y's rounding, which few keys do not make small beside the differences yb v^T - delta (y is as large as they
+    // are: qb of 16 bits would be off by 1.7 roundings, not 1.4).  There a pass before forms it from P and yb v^T; kb gets it so in
+    // any case.
+    const bool exact = keys.count <= kFewTiles;
+    float sum = 0.f;
+    for (int pass = exact ? 0 : 1; pass < 2; ++pass) {
+        if (keys.count > 0) {
+            load(0, lds);
+            sk.store(lds);
+            sv.store(lds + TILE);
             if constexpr (DIRECT) wait_loads<0>();
         }
+        settle_loads();
         __syncthreads();
+        for (int i = 0; i < keys.count; ++i) {
+            char* now = lds + (i & 1) * 2 * TILE;
+            char* next = lds + (~i & 1) * 2 * TILE;
+            if (i + 1 < keys.count) load(i + 1, next);
+            const int key = keys.key(i);
+            if (working && ((key < mine.high && key + BN > mine.low) || key < mine.sinks)) {
+                const bool whole = key + BN - 1 <= w0 && (w1 - key < s.window || key + BN <= s.sinks);
+                const int high = pos - key - 4 * h, low = high - s.window, sink = s.sinks - key - 4 * h;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    floatx16 x, g;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] = g[e] = 0.f;
+#pragma unroll
+                    for (int f = 0; f < FR; ++f) x = multiply<T>(along_head<T, DP>(now, 32 * b, f), qf[f], x);
+#pragma unroll
+                    for (int f = 0; f < FR; ++f) g = multiply<T>(along_head<T, DP>(now + TILE, 32 * b, f), of[f], g);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], c, base));
+                    if (!whole) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int at = 32 * b + 8 * (e >> 2) + (e & 3);
+                            if (!(at <= high && (at > low || at < sink))) x[e] = 0.f;
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        sum = fmaf(x[e], g[e], sum);
+                        x[e] *= g[e] - delta;
+                    }
+                    if (pass) {
+#pragma unroll
+                        for (int u = 0; u < kParts<T>; ++u) {
+                            const v4u part = part_of<T>(x, u);
+#pragma unroll
+                            for (int m = 0; m < DT; ++m) acc[m] = multiply<T>(along_rows<T, DP>(now, 32 * b + u * 2 * kCE<T>, 32 * m), part, acc[m]);
+                        }
+                    }
+                }
+            }
+            if (i + 1 < keys.count) {
+                sk.store(next);
+                sv.store(next + TILE);
+                if constexpr (DIRECT) wait_loads<0>();
+            }
+            __syncthreads();
+        }
+        if (!pass) {
+            delta = sum + other_half(sum);
+            sum = 0.f;
+        }
     }
-    if (any_not_finite<DT>(acc)) {
+    sum += other_half(sum);
+    if (here && h == 0) p.delta[t * (p.heads * s.group) + head] = sum;
+    // (what is not finite: products with what is not seen among it.  Of what is seen, it reaches the other keys by y alone.)
+    if (any_not_finite<DT>(acc) || __any(here && sum * 0.f != 0.f)) {
         for (int i = 0; i < 32; ++i) {
             const int ri = r0 + 32 * wave + i, ji = ri / s.group, hi = kvh * s.group + ri - ji * s.group;
             if (ji >= q.nq) break;
             const Range seen = seen_by(s, ji + q.shift(), ji + q.shift());
             const int64_t ti = q.q0 + ji, ci = (int64_t)hi * p.d, at = ti * (p.heads * s.group) + hi;
             const Two x = load_two((const T*)p.q + ti * p.ldq + ci, p.d), g = load_two((const T*)p.yb + ti * p.ldyb + ci, p.d);
-            const float li = p.lse[at], di = dot(g, load_two((const T*)p.y + ti * p.ldy + ci, p.d));
-            float a = 0.f, b = 0.f;
-            for (int part = 0; part < 2; ++part) {
-                const int end = part ? seen.high : seen.sinks;
-                for (int n = part ? seen.low : 0; n < end; ++n) {
-                    const Two kn = load_two(k + n * p.ldk, p.d), vn = load_two(v + n * p.ldv, p.d);
-                    const float w = exp2f((dot(x, kn) * p.s - li) * kLog2e) * (dot(g, vn) - di);
-                    a = fmaf(w, kn.a, a);
-                    b = fmaf(w, kn.b, b);
+            const float li = p.lse[at];
+            float di = 0.f, a = 0.f, b = 0.f;
+            for (int step = 0; step < 2; ++step) {
+                if (step == 1 && di * 0.f != 0.f) di = dot(g, load_two((const T*)p.y + ti * p.ldy + ci, p.d));
+                for (int part = 0; part < 2; ++part) {
+                    const int end = part ? seen.high : seen.sinks;
+                    for (int n = part ? seen.low : 0; n < end; ++n) {
+                        const Two kn = load_two(k + n * p.ldk, p.d), vn = load_two(v + n * p.ldv, p.d);
+                        const float w = exp2f((dot(x, kn) * p.s - li) * kLog2e), gv = dot(g, vn);
+                        if (step == 0) {
+                            di = fmaf(w, gv, di);
+                        } else {
+                            a = fmaf(w * (gv - di), kn.a, a);
+                            b = fmaf(w * (gv - di), kn.b, b);
+                        }
+                    }
                 }
             }
+            if (lane == 0) p.delta[at] = di;
+            if (!p.qb) continue;
             store_two((T*)p.qb + ti * p.ldqb + ci, a * p.s, b * p.s, p.d, p.add);
         }
         return;
     }
-    if (!here) return;
+    if (!here || !p.qb) return;
     T* out = (T*)p.qb + t * p.ldqb + col;
 #pragma unroll
     for (int m = 0; m < DT; ++m)
@@ -419,11 +448,13 @@ __global__ __launch_bounds__((64 * kGroups<T, FAR> * kRowWaves<T, FAR>), (sizeof
         else so.template load<N - S::PER>(p.ldyb, p.d, s.group, p.magic, at + TILE);
     };
     auto load_all = [&](char* at) INLINE { static_for<CHUNKS>([&](auto n) INLINE { load(n, at); }); };
-    // The products start from what belongs to a row: scores from -lse / s, yb v^T from -delta.
+    // The products start from what belongs to a row: yb v^T from -delta, scores of 16-bit types from -lse / s (in fp32 the sum would lose by
+    // it: they start from zero, and -lse comes behind).
+    constexpr bool FROM_LSE = sizeof(T) == 2;
     auto keep = [&](int i, char* at) INLINE {
         sq.store(at);
         so.store(at + TILE);
-        if (threadIdx.x < 2 * BM) reinterpret_cast<float*>(st + (i & 1) * STATS)[threadIdx.x] = threadIdx.x < BM ? stat * per_s : -stat;
+        if (threadIdx.x < 2 * BM) reinterpret_cast<float*>(st + (i & 1) * STATS)[threadIdx.x] = threadIdx.x < BM ? stat * (FROM_LSE ? per_s : -kLog2e) : -stat;
         if constexpr (DIRECT) wait_loads<0>();
     };
     if (tiles > 0) {
@@ -459,7 +490,14 @@ __global__ __launch_bounds__((64 * kGroups<T, FAR> * kRowWaves<T, FAR>), (sizeof
             };
             // The scores block by block, then yb v^T.  Between the first block's products go the loads of the next tile, between all that
             // follow the exponentials, none before its scores are there.
-            start(x[0], 0);
+            if constexpr (FROM_LSE) {
+                start(x[0], 0);
+            } else {
+#pragma unroll
+                for (int b = 0; b < RB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[b][e] = 0.f;
+            }
             products<2 * RB * FR, 6>(
                 [&](auto n) INLINE {
                     constexpr int N = decltype(n)::value, PH = N / FR;
@@ -477,14 +515,15 @@ __global__ __launch_bounds__((64 * kGroups<T, FAR> * kRowWaves<T, FAR>), (sizeof
                         static_for<(F + 1) * CHUNKS / FR - FROM>([&](auto k) INLINE { load(std::integral_constant<int, FROM + decltype(k)::value>{}, next); });
                     }
                     if constexpr (F == FR - 3 && PH + 1 < 2 * RB) {
-                        if constexpr (PH + 1 < RB) start(x[PH + 1], 32 * (PH + 1));
-                        else start(g[PH + 1 - RB], BM + 32 * (PH + 1 - RB));
+                        if constexpr (PH + 1 >= RB) start(g[PH + 1 - RB], BM + 32 * (PH + 1 - RB));
+                        else if constexpr (FROM_LSE) start(x[PH + 1], 32 * (PH + 1));
                     }
                     if constexpr (N > FR) {
                         constexpr int STEPS = (2 * RB - 1) * FR - 1, FROM = (N - FR - 1) * 16 * RB / STEPS;
                         static_for<(N - FR) * 16 * RB / STEPS - FROM>([&](auto k) INLINE {
                             constexpr int E = FROM + decltype(k)::value;
-                            x[E / 16][E % 16] = __builtin_amdgcn_exp2f(x[E / 16][E % 16] * c);
+                            const float l = FROM_LSE ? 0.f : stats[32 * (E / 16) + 8 * (E % 16 / 4) + 4 * h + E % 4];
+                            x[E / 16][E % 16] = __builtin_amdgcn_exp2f(FROM_LSE ? x[E / 16][E % 16] * c : fmaf(x[E / 16][E % 16], c, l));
                         });
                     }
                 });
