@@ -165,13 +165,6 @@ __device__ __forceinline__ void negate_all(v4u* f, int n) {
     for (int i = 0; i < n; ++i) f[i] ^= bits;
 }
 
-// four consecutive values of the head
-template <class T>
-__device__ __forceinline__ void store4(T* p, float a, float b, float c, float e, int left) {
-    const float v[4] = {a, b, c, e};
-    store_row(p, v, left);
-}
-
 // a wave's finished rows: y and lse
 template <class T, int DT>
 __device__ __forceinline__ void store_rows(const Att& p, const floatx16 (&o)[DT], const Row& w, float m, float l) {
@@ -226,22 +219,6 @@ __device__ __forceinline__ void store_nothing(const Att& p, const Seq& q, int kv
         if (!w.here) continue;
         for (int i = 0; i < p.d; ++i) ((T*)p.y)[w.t * p.ldy + (int64_t)w.head * p.d + i] = (T)0.f;
         if (p.lse) p.lse[w.t * (p.heads * p.seqs.group) + w.head] = -INFINITY;
-    }
-}
-
-// a block's place: blocks go round the 8 XCDs, each with an L2 of its own; blocks of one key head
-// go to one XCD, or a key head's blocks go round the XCDs that have it
-__device__ __forceinline__ void place_of(int64_t block, int64_t slots, int heads, int64_t& slot, int& kvh) {
-    if (heads % 8 == 0) {
-        const int64_t in = block >> 3;
-        kvh = (int)(block & 7) + 8 * (int)(in / slots);
-        slot = in % slots;
-    } else if (8 % heads == 0) {
-        kvh = (int)(block % heads);
-        slot = block / heads;
-    } else {
-        kvh = (int)(block / slots);
-        slot = block % slots;
     }
 }
 
@@ -421,15 +398,6 @@ __global__ __launch_bounds__(256) void join_kernel(Att p, int64_t blocks) {
     }
 }
 
-int32_t* error_flag(Workspace* ws) { return (int32_t*)(ws->dscalars + kErrFlagSlot); }
-
-template <class F>
-int32_t with_width(int64_t d, F&& f) {
-    if (d <= 64) return f(std::integral_constant<int, 2>{});
-    if (d <= 96) return f(std::integral_constant<int, 3>{});
-    return f(std::integral_constant<int, 4>{});
-}
-
 }  // namespace
 }  // namespace stade
 
@@ -447,23 +415,25 @@ int32_t stade_hip_attention(int64_t tx, void* y, int64_t ldy, float* lse, const 
     if (int32_t rc = check_ld(fn, "ldq", ldq, i_d * i_q)) return rc;
     if (int32_t rc = check_ld(fn, "ldk", ldk, i_d * i_k)) return rc;
     if (int32_t rc = check_ld(fn, "ldv", ldv, i_d * i_k)) return rc;
+    const int64_t slots = slots_of(i_t, seqs.group, kWideRows, i_n + 1), blocks = slots * i_k;
+    if (int32_t rc = check_extent(fn, "blocks of 128 rows of a key head", blocks, kMostBlocks)) return rc;
     if (i_d == 0 || i_q == 0 || i_t == 0) return STADE_HIP_OK;
     if (!y || !q || (i_tk > 0 && (!k || !v))) return bad(fn, "null pointer");
     WsCall call(stream);
     if (!call.ok()) return call.error();
     Att p{y, ldy, lse, q, ldq, k, ldk, v, ldv, seqs, (int)i_d, (int)i_k, (float)fabs(s), s < 0.0};
     p.seqs.flag = error_flag(call.ws);
-    p.slots = slots_of(i_t, p.seqs.group, kWideRows, i_n + 1);
+    p.slots = slots;
     // Blocks for two rounds of two a CU, eight tiles of keys each (a tile takes a microsecond, the second launch with what it reads some
     // ten), and no more than 32 (which the second launch reads one after the other).  A sequence is taken to be up to twice as long as the
     // mean.  One token of 8192 keys, 8 key heads: 135 us alone, 22 by 16 blocks; of 65536: 1167 and 75 by 32; 4 chunks of 512 behind
     // 8192, 4 key heads: 319 and 229 by three; 2 prompts of 300, 2 key heads: 17, and 25 by two.
     // (Two slots more than sequences, for columns of none, usually are empty.)
-    const int64_t blocks = p.slots * i_k, full = std::max<int64_t>(1, (p.slots - 2) * i_k);
+    const int64_t full = std::max<int64_t>(1, (p.slots - 2) * i_k);
     const int64_t longest = std::min({i_tk, 2 * i_tk / std::max<int64_t>(i_n, 1) + 1, (int64_t)seqs.window + kMostSinks + kWideRows});
     p.splits = (int)std::max<int64_t>(1, std::min({kSplitBlocks / full, 2 * kSplitBlocks / blocks, longest / (8 * kWideKeys), (int64_t)32}));
-    // (as much as any call takes, so that each is captured after an eager one)
-    if (p.splits > 1 && !(p.part = (float*)scratch((size_t)2 * kSplitBlocks * kWideRows * (kMostHead + 2) * 4))) return scratch_error();
+    // (as much as any call takes, and by each, so that every other is captured after it)
+    if (!(p.part = (float*)scratch((size_t)2 * kSplitBlocks * kWideRows * (kMostHead + 2) * 4))) return scratch_error();
     return with_type(tx, [&](auto t) -> int32_t {
         return with_width(i_d, [&](auto dt) -> int32_t {
             using T = decltype(t);

@@ -16,6 +16,8 @@ namespace attn {
 
 using namespace rows;
 
+// (a launch's threads are counted in 32 bits, and blocks have up to 512)
+constexpr int64_t kMostBlocks = (1 << 23) - 1;
 constexpr int64_t kMostHead = 128, kMostHeads = 4096, kMostSeqs = 1 << 20, kMostSinks = 64;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
@@ -189,12 +191,6 @@ __device__ __forceinline__ void wait_loads() {
 // compiler sees.  Without it the compiler waits for them at their first use inside the loop, in every round, and with them
 // for all that is under way to LDS.
 __device__ __forceinline__ void settle_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }   // vmcnt(0)
-// before a buffer is written again: this wave's reads of it are through
-__device__ __forceinline__ void wait_reads() {
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-}
 
 // 16 bytes at any alignment: the first `left` values, and zeros
 template <class T>
@@ -395,12 +391,50 @@ __device__ __forceinline__ void row_fragments(v4u (&f)[DT * 32 / (2 * kCE<T>)], 
     }
 }
 
+// a block's place: blocks go round the 8 XCDs, each with an L2 of its own; blocks of one key head
+// go to one XCD, or a key head's blocks go round the XCDs that have it
+__device__ __forceinline__ void place_of(int64_t block, int64_t slots, int heads, int64_t& slot, int& kvh) {
+    if (heads % 8 == 0) {
+        const int64_t in = block >> 3;
+        kvh = (int)(block & 7) + 8 * (int)(in / slots);
+        slot = in % slots;
+    } else if (8 % heads == 0) {
+        kvh = (int)(block % heads);
+        slot = block / heads;
+    } else {
+        kvh = (int)(block / slots);
+        slot = block % slots;
+    }
+}
+
+// four consecutive values of the head
+template <class T>
+__device__ __forceinline__ void store4(T* p, float a, float b, float c, float e, int left, bool add = false) {
+    float v[4] = {a, b, c, e};
+    if (add) {
+        float o[4];
+        load_row(o, p, left);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += o[i];
+    }
+    store_row(p, v, left);
+}
+
 // ------------------------------------------------------------------------------------------
 // host
 // ------------------------------------------------------------------------------------------
 // rows that go straight to LDS: 16-byte aligned, whole chunks, and a tile's offsets within 31 bits
 inline bool straight(const void* p, int64_t ld, int64_t d, int64_t size) {
     return (uintptr_t)p % 16 == 0 && ld * size % 16 == 0 && d * size % 16 == 0 && ld * size < (int64_t)1 << 23;
+}
+
+inline int32_t* error_flag(Workspace* ws) { return (int32_t*)(ws->dscalars + kErrFlagSlot); }
+
+template <class F>
+inline int32_t with_width(int64_t d, F&& f) {
+    if (d <= 64) return f(std::integral_constant<int, 2>{});
+    if (d <= 96) return f(std::integral_constant<int, 3>{});
+    return f(std::integral_constant<int, 4>{});
 }
 
 // the checks of both functions; the sequences with everything but the flag

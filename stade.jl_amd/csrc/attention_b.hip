@@ -50,33 +50,6 @@ constexpr int kRows = 128, kKeys = 128;
 constexpr int kFewTiles = 4;      // of keys, where delta is formed from the weights
 
 
-template <class T>
-__device__ __forceinline__ void store4(T* p, float a, float b, float c, float e, int left, bool add) {
-    float v[4] = {a, b, c, e};
-    if (add) {
-        float o[4];
-        load_row(o, p, left);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += o[i];
-    }
-    store_row(p, v, left);
-}
-
-// blocks of one key head go to one XCD, or a key head's blocks go round the XCDs that have it
-__device__ __forceinline__ void place_of(int64_t block, int64_t slots, int heads, int64_t& slot, int& kvh) {
-    if (heads % 8 == 0) {
-        const int64_t in = block >> 3;
-        kvh = (int)(block & 7) + 8 * (int)(in / slots);
-        slot = in % slots;
-    } else if (8 % heads == 0) {
-        kvh = (int)(block % heads);
-        slot = block / heads;
-    } else {
-        kvh = (int)(block / slots);
-        slot = block % slots;
-    }
-}
-
 // ------------------------------------------------------------------------------------------
 // qb, and delta
 // ------------------------------------------------------------------------------------------
@@ -736,15 +709,6 @@ int cu_count() {
     return cus > 0 ? cus : 256;
 }
 
-int32_t* error_flag(Workspace* ws) { return (int32_t*)(ws->dscalars + kErrFlagSlot); }
-
-template <class F>
-int32_t with_width(int64_t d, F&& f) {
-    if (d <= 64) return f(std::integral_constant<int, 2>{});
-    if (d <= 96) return f(std::integral_constant<int, 3>{});
-    return f(std::integral_constant<int, 4>{});
-}
-
 // blocks of far rows for each key head of a sequence: about one a CU in all
 constexpr int64_t kFarBlocks = 256;
 
@@ -773,25 +737,33 @@ int32_t stade_hip_attention_b(int64_t tx, const void* yb, int64_t ldyb, const vo
         if (int32_t rc = check_ld(fn, "ldkb", ldkb, i_d * i_k)) return rc;
     if (vb)
         if (int32_t rc = check_ld(fn, "ldvb", ldvb, i_d * i_k)) return rc;
-    if (i_d == 0 || i_q == 0 || (i_t == 0 && (add || i_tk == 0)) || (!qb && !kb && !vb)) return STADE_HIP_OK;
+    const int64_t row_slots = slots_of(i_t, seqs.group, kRows, i_n + 1), slots = slots_of(i_tk, 1, kKeys, i_n + 1), units = slots * i_k;
+    if (int32_t rc = check_extent(fn, "blocks of 128 rows of a key head", row_slots * i_k, kMostBlocks)) return rc;
+    if (int32_t rc = check_extent(fn, "blocks of 128 keys of a key head", units, kMostBlocks)) return rc;
+    const bool far = sinks > 0 && window >= 0 && window < i_tk && (kb || vb);
+    const int64_t pairs = i_n * i_k, far_blocks = pairs * ((sinks * 2 * i_d + 255) / 256);
+    if (far)
+        if (int32_t rc = check_extent(fn, "i_n * i_k with sinks", far_blocks, kMostBlocks)) return rc;
+    if (i_q == 0 && i_k > 0) return bad(fn, "i_q is zero");
+    if (i_d == 0 || i_k == 0 || (i_t == 0 && (add || i_tk == 0)) || (!qb && !kb && !vb)) return STADE_HIP_OK;
     if ((i_t > 0 && (!yb || !y || !lse || !q)) || (i_tk > 0 && (!k || !v))) return bad(fn, "null pointer");
     WsCall call(stream);
     if (!call.ok()) return call.error();
     Back p{yb, ldyb, y, ldy, lse, q, ldq, qb, ldqb, k, ldk, kb, ldkb, v, ldv, vb, ldvb, nullptr, seqs, (int)i_d, (int)i_k, (float)s, add != 0};
     p.seqs.flag = error_flag(call.ws);
     p.magic = (uint32_t)((((uint64_t)1 << 31) + seqs.group - 1) / seqs.group);
-    const bool far = sinks > 0 && window >= 0 && window < i_tk && (kb || vb);
     const size_t deltas = ((size_t)i_t * i_q * 4 + 256) / 256 * 256;
-    const int64_t pairs = i_n * i_k, sink_bytes = (int64_t)std::max<int64_t>(sinks, 1) * 2 * i_d * 4;
-    const size_t fars = far ? (size_t)(std::max(pairs, kFarBlocks) * sink_bytes) : 0;
+    const int64_t sink_bytes = (int64_t)std::max<int64_t>(sinks, 1) * 2 * i_d * 4;
+    // (what any call of up to kFarBlocks pairs takes is taken by each, so that every smaller one is captured after an eager one)
+    const size_t fars = std::max((size_t)kFarBlocks * kMostSinks * 2 * kMostHead * 4, far ? (size_t)(pairs * sink_bytes) : 0);
     // Tiles of keys that fill no whole round of the CUs go over as many blocks as make two rounds (a block has a CU to
     // itself), or as have six tiles of rows each.
-    const int64_t cus = cu_count(), slots = slots_of(i_tk, 1, kKeys, i_n + 1), units = slots * i_k;
+    const int64_t cus = cu_count();
     p.whole = units / cus * cus;
     const int64_t rest = units - p.whole, longest = std::min<int64_t>(i_t, (int64_t)seqs.window + kKeys) * seqs.group;
     p.splits = rest ? (int)std::min<int64_t>(2 * cus / rest, std::max<int64_t>(1, longest / (6 * 32 * 2))) : 1;
     if (p.splits <= 1) p.whole = units;
-    const size_t parts = (kb || vb) && i_t > 0 ? (size_t)(2 * cus) * kKeys * 2 * kMostHead * 4 : 0;
+    const size_t parts = (size_t)(2 * cus) * kKeys * 2 * kMostHead * 4;
     char* work = (char*)scratch(deltas + fars + parts);
     if (!work) return scratch_error();
     p.delta = (float*)work;
@@ -809,7 +781,7 @@ int32_t stade_hip_attention_b(int64_t tx, const void* yb, int64_t ldyb, const vo
                                 straight(yb, ldyb, i_d, size) && straight(y, ldy, i_d, size);
             if (i_t > 0) {
                 Back r = p;
-                r.slots = slots_of(i_t, seqs.group, kRows, i_n + 1);
+                r.slots = row_slots;
                 STADE_TIMED("attention_b_rows", stream, {
                     if (direct) rows_kernel<T, DT, true><<<(unsigned)(r.slots * i_k), 256, 0, stream>>>(r);
                     else rows_kernel<T, DT, false><<<(unsigned)(r.slots * i_k), 256, 0, stream>>>(r);
@@ -824,7 +796,7 @@ int32_t stade_hip_attention_b(int64_t tx, const void* yb, int64_t ldyb, const vo
                         else keys_kernel<T, DT, false, true><<<dim3((unsigned)(pairs * p.far_parts), sinks > 32 ? 2 : 1), NTF, 0, stream>>>(p);
                     });
                     STADE_LAUNCHED("attention keys_kernel (sinks)");
-                    STADE_TIMED("attention_b_sinks", stream, far_kernel<<<(unsigned)(pairs * ((sinks * 2 * i_d + 255) / 256)), 256, 0, stream>>>(p, (kTileRows<T, true>)));
+                    STADE_TIMED("attention_b_sinks", stream, far_kernel<<<(unsigned)far_blocks, 256, 0, stream>>>(p, (kTileRows<T, true>)));
                     STADE_LAUNCHED("attention far_kernel");
                 }
                 p.slots = slots;

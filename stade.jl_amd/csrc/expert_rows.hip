@@ -324,20 +324,24 @@ int32_t stade_hip_expert_order(const int64_t* ids, int64_t* order, int64_t* plac
     const int64_t n = i_k * i_t;
     if (int32_t rc = check_extent(fn, "i_k * i_t", n, kMostRows)) return rc;
     if (!start || (n > 0 && (!ids || !order || !place))) return bad(fn, "null pointer");
-    // Few experts: by counting, a launch or two (16384 slots of 64 experts: 7 us, by sorting 28).
     const int64_t blocks = (n + kStretch - 1) / kStretch;
-    if (n > 0 && i_e <= kFewExperts && blocks * (i_e + 1) <= kMostCounts) {
+    if (n > 0) {
         WsCall call(stream);
         if (!call.ok()) return call.error();
-        Order p{ids, order, place, start, (int)i_e, (int)n, (int)blocks, nullptr, error_flag(call.ws)};
-        if (blocks > 1) {
-            if (!(p.counts = (int32_t*)scratch(kMostCounts * sizeof(int32_t)))) return scratch_error();
-            STADE_TIMED("expert_count", stream, count_kernel<<<(unsigned)blocks, kOrderNT, 0, stream>>>(p));
-            STADE_LAUNCHED("expert_rows count_kernel");
+        // (taken by every call, so that each smaller one is captured after an eager one)
+        int32_t* counts = (int32_t*)scratch(kMostCounts * sizeof(int32_t));
+        if (!counts) return scratch_error();
+        // Few experts: by counting, a launch or two (16384 slots of 64 experts: 11 us, by sorting 28).
+        if (i_e <= kFewExperts && blocks * (i_e + 1) <= kMostCounts) {
+            const Order p{ids, order, place, start, (int)i_e, (int)n, (int)blocks, counts, error_flag(call.ws)};
+            if (blocks > 1) {
+                STADE_TIMED("expert_count", stream, count_kernel<<<(unsigned)blocks, kOrderNT, 0, stream>>>(p));
+                STADE_LAUNCHED("expert_rows count_kernel");
+            }
+            STADE_TIMED("expert_order", stream, order_kernel<<<(unsigned)blocks, kOrderNT, 0, stream>>>(p));
+            STADE_LAUNCHED("expert_rows order_kernel");
+            return STADE_HIP_OK;
         }
-        STADE_TIMED("expert_order", stream, order_kernel<<<(unsigned)blocks, kOrderNT, 0, stream>>>(p));
-        STADE_LAUNCHED("expert_rows order_kernel");
-        return STADE_HIP_OK;
     }
     if (int32_t rc = stade_hip_token_order(ids, order, start, i_e, n, stream)) return rc;
     if (n == 0) return STADE_HIP_OK;

@@ -377,6 +377,7 @@ inline int tile_of(const Rot& p, int v) {
 }
 // `blocks` of them for all heads, as many for queries as they have of the heads
 inline void share(Rot& p, int64_t blocks, int64_t tiles, unsigned& grid) {
+    blocks = std::min<int64_t>(blocks, 1 << 20);   // (a launch's threads are counted in 32 bits)
     const int64_t heads = p.nq + p.nk, q = p.nq ? std::max<int64_t>(1, std::min(tiles, (blocks * p.nq + heads / 2) / heads)) : 0;
     const int64_t k = p.nk ? std::max<int64_t>(1, std::min(tiles, blocks - q)) : 0;
     p.q_blocks = (int)q;
