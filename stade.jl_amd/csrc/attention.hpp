@@ -437,6 +437,13 @@ inline int32_t with_width(int64_t d, F&& f) {
     return f(std::integral_constant<int, 4>{});
 }
 
+// The scores' factor as the kernels divide by it and multiply -Inf with it: not below 2^-100 in size (in place of 0 it moves weights by less
+// than a rounding while q . k is below 2^76)
+inline float factor(double s) {
+    const float f = (float)s;
+    return fabsf(f) >= 0x1p-100f ? f : f < 0.f ? -0x1p-100f : 0x1p-100f;
+}
+
 // the checks of both functions; the sequences with everything but the flag
 inline int32_t check_attention(const char* fn, int64_t tx, double s, int64_t i_d, int64_t i_q, int64_t i_k, int64_t i_t, int64_t i_tk, int64_t i_n,
                                int64_t window, int64_t sinks, const int64_t* qstart, const int64_t* kstart, Seqs& seqs) {

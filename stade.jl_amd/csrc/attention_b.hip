@@ -37,6 +37,7 @@ struct Back {
     int d, heads;          // of the keys
     float s;
     int add;
+    float factor;          // of the scores: s, not 0
     int64_t slots;
     uint32_t magic;        // ceil(2^31 / group)
     float* far;            // partial sums of the sinks; null: none
@@ -96,7 +97,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void rows_kernel(Back 
     const KeyTiles<BN> keys(range);
     const T* k = (const T*)p.k + q.k0 * p.ldk + (int64_t)kvh * p.d;
     const T* v = (const T*)p.v + q.k0 * p.ldv + (int64_t)kvh * p.d;
-    const float c = p.s * kLog2e, base = -lse * kLog2e;
+    const float c = p.factor * kLog2e, base = -lse * kLog2e;
     floatx16 acc[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i)
@@ -386,7 +387,7 @@ __global__ __launch_bounds__((64 * kGroups<T, FAR> * kRowWaves<T, FAR>), (sizeof
     for (int i = 0; i < DT; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) ka[i][e] = va[i][e] = 0.f;
-    const float c = p.s * kLog2e;
+    const float c = p.factor * kLog2e;
     const int heads = p.heads * s.group, tiles = r_end > r_first ? (r_end - r_first + BM - 1) / BM : 0;
     // (the query and the head in its group of a tile's first row: of the one at work and of the one on its way)
     int now_j = uniform(r_first / s.group), now_h = uniform(r_first - now_j * s.group), next_j = now_j, next_h = now_h;
@@ -395,7 +396,7 @@ __global__ __launch_bounds__((64 * kGroups<T, FAR> * kRowWaves<T, FAR>), (sizeof
     sq.places(p.ldq, p.d, s.group, p.magic, now_h);
     so.places(p.ldyb, p.d, s.group, p.magic, now_h);
     const bool fixed = BM % s.group == 0;      // (tiles of whole queries)
-    const float per_s = -1.f / p.s;
+    const float per_s = -1.f / p.factor;
     auto aim = [&](int i) INLINE {             // at tile i (behind the last: no rows)
         const int64_t t = q.q0 + next_j, head = (int64_t)kvh * s.group;
         const int rows = min(BM, r_end - (r_first + i * BM));
@@ -749,7 +750,7 @@ int32_t stade_hip_attention_b(int64_t tx, const void* yb, int64_t ldyb, const vo
     if ((i_t > 0 && (!yb || !y || !lse || !q)) || (i_tk > 0 && (!k || !v))) return bad(fn, "null pointer");
     WsCall call(stream);
     if (!call.ok()) return call.error();
-    Back p{yb, ldyb, y, ldy, lse, q, ldq, qb, ldqb, k, ldk, kb, ldkb, v, ldv, vb, ldvb, nullptr, seqs, (int)i_d, (int)i_k, (float)s, add != 0};
+    Back p{yb, ldyb, y, ldy, lse, q, ldq, qb, ldqb, k, ldk, kb, ldkb, v, ldv, vb, ldvb, nullptr, seqs, (int)i_d, (int)i_k, (float)s, add != 0, factor(s)};
     p.seqs.flag = error_flag(call.ws);
     p.magic = (uint32_t)((((uint64_t)1 << 31) + seqs.group - 1) / seqs.group);
     const size_t deltas = ((size_t)i_t * i_q * 4 + 256) / 256 * 256;
@@ -757,11 +758,12 @@ int32_t stade_hip_attention_b(int64_t tx, const void* yb, int64_t ldyb, const vo
     // (what any call of up to kFarBlocks pairs takes is taken by each, so that every smaller one is captured after an eager one)
     const size_t fars = std::max((size_t)kFarBlocks * kMostSinks * 2 * kMostHead * 4, far ? (size_t)(pairs * sink_bytes) : 0);
     // Tiles of keys that fill no whole round of the CUs go over as many blocks as make two rounds (a block has a CU to
-    // itself), or as have six tiles of rows each.
+    // itself), or as have six tiles of rows each (fp32, whose products take eight times as long: four of half the size.  3 sequences of
+    // 500, 2 key heads: 111 us by three blocks a tile, 50 by ten).
     const int64_t cus = cu_count();
     p.whole = units / cus * cus;
     const int64_t rest = units - p.whole, longest = std::min<int64_t>(i_t, (int64_t)seqs.window + kKeys) * seqs.group;
-    p.splits = rest ? (int)std::min<int64_t>(2 * cus / rest, std::max<int64_t>(1, longest / (6 * 32 * 2))) : 1;
+    p.splits = rest ? (int)std::min<int64_t>(2 * cus / rest, std::max<int64_t>(1, longest / (tx == STADE_HIP_F32 ? 4 * 32 : 6 * 64))) : 1;
     if (p.splits <= 1) p.whole = units;
     const size_t parts = (size_t)(2 * cus) * kKeys * 2 * kMostHead * 4;
     char* work = (char*)scratch(deltas + fars + parts);

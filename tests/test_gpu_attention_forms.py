@@ -101,3 +101,18 @@ def test_past_the_rounds_of_the_card(dt):
     y, lse = _forward(c, want, err)
     for a, v in zip("qkv", c.backward(y, lse)):
         within(a + "b", v, want[a + "b"], err[a + "b"] + 2 * U * want[a + "b"].abs(), dt)
+
+
+@pytest.mark.parametrize("s", [0.0, 1e-42, -1e-30, -0.7])
+@pytest.mark.parametrize("dt", TYPES, ids=IDS.get)
+@pytest.mark.parametrize("seqs", [[(400, 400), (5, 5), (260, 300)], [(1, 4096), (1, 64)], [(64, 64), (1, 128)]], ids=str)
+def test_factors_that_leave_no_scores(seqs, dt, s):
+    """Scores of 0 or nearly: equal weights, also over whole tiles of keys and over several blocks."""
+    c = Case(seqs, 4, 1, 128, 70 if seqs[0][0] == 400 else None, 4, dt, s=s)
+    want, err = formula(c)
+    print(f"factor {s} {IDS[dt]}", flush=True)
+    y, lse = _forward(c, want, err)
+    # s is taken in fp32: qb and kb, multiples of it, are off by its rounding, for 1e-42 by up to 2^-150 / 1e-42 = 7e-4 of them
+    off = abs(float(torch.tensor(s, dtype=torch.float32)) - s) / abs(s) if s else 0.0
+    for a, v in zip("qkv", c.backward(y, lse)):
+        within(a + "b", v, want[a + "b"], err[a + "b"] + (2 * U + off) * want[a + "b"].abs(), dt)
