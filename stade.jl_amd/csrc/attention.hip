@@ -12,6 +12,9 @@
 // A block has 128 rows, four waves of 32, which share tiles of 64 keys and values in two buffers.  Where the rows do not make two
 // blocks a CU (single tokens, chunks behind a long context) the keys of each go over several blocks, whose maxima, sums and values a
 // second launch joins in order.
+//
+// bf16, heads of 128: 5 sequences of 3300, 32 heads of queries and 8 of keys, a window of 1024: 320 us, 733 TFLOP/s of what is seen; causal
+// without a window 952 (the clock then falls to 1.6 GHz).  64 single tokens of 4096 keys, 8 key heads: 228 us, 4.7 TB/s.
 #include "attention.hpp"
 
 #include <algorithm>
