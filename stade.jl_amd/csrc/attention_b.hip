@@ -10,7 +10,7 @@
 // sums go in a fixed order, and the same call gives the same bits.
 // Sinks are seen by every later row: rows past the window of the first tile of keys go over blocks of their own, which leave
 // partial sums that the tile's block adds.
-// 4 sequences of 2048, 16 heads of 128 and 4 of keys, a window of 1024, 4 sinks, bf16: rows 121 us, keys 194, sinks 31, joins 9: some 640
+// 4 sequences of 2048, 16 heads of 128 and 4 of keys, a window of 1024, 4 sinks, bf16: rows 121 us, keys 194, sinks 31, joins 9: some 590
 // TFLOP/s of the products formed for what is seen.
 // Sums are fp32; P and S are rounded to the type as factors of products (to nearest), as the values they meet are.
 #include "attention.hpp"
