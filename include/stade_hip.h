@@ -306,11 +306,12 @@ int32_t stade_hip_head_rotary_b(int64_t tx, int64_t tg, const void* yb, int64_t 
  * p sees the keys i <= p with p - i < window (window < 0: all) or i < sinks.  y = sum of softmax(s q . k) v over what it
  * sees; lse (i_q, i_t) Float32, if not null: the logarithm of the sum of exp(s q . k), which the adjoint takes.  A query that sees nothing,
  * and a column of no sequence, gets zeros and -Inf.  A product with keys that are not seen is never formed into the result,
- * whatever they hold.  Offsets that decrease or lie outside the columns raise the device error flag.  i_d <= 128, sinks <= 64. */
+ * whatever they hold.  Offsets that decrease or lie outside the columns raise the device error flag.  i_d <= 128, sinks <= 64,
+ * i_t * i_q / i_k <= 2^30, and of tiles of 128 rows or keys, a few for each sequence, times i_k at most 2^23. */
 int32_t stade_hip_attention(int64_t tx, void* y, int64_t ldy, float* lse, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
                             int64_t ldv, const int64_t* qstart, const int64_t* kstart, double s, int64_t i_d, int64_t i_q, int64_t i_k,
                             int64_t i_t, int64_t i_tk, int64_t i_n, int64_t window, int64_t sinks, hipStream_t stream);
-/* its adjoint: qb, kb, vb from yb and what the forward call took and gave; each may be null. */
+/* its adjoint: qb, kb, vb from yb and what the forward call took and gave; each may be null.  i_q is not 0. */
 int32_t stade_hip_attention_b(int64_t tx, const void* yb, int64_t ldyb, const void* y, int64_t ldy, const float* lse, const void* q, int64_t ldq,
                               void* qb, int64_t ldqb, const void* k, int64_t ldk, void* kb, int64_t ldkb, const void* v, int64_t ldv, void* vb,
                               int64_t ldvb, const int64_t* qstart, const int64_t* kstart, double s, int64_t i_d, int64_t i_q, int64_t i_k,

@@ -52,7 +52,6 @@ struct Back {
 constexpr int kRows = 128, kKeys = 128;
 constexpr int kFewTiles = 4;      // of keys, where delta is formed from the weights
 
-
 // ------------------------------------------------------------------------------------------
 // qb, and delta
 // ------------------------------------------------------------------------------------------
@@ -114,9 +113,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void rows_kernel(Back 
         sv.load(v + key * p.ldv, from, to, at + TILE);
     };
     // yb . y is delta but for y's rounding, which few keys do not make small beside the differences yb v^T - delta (y is as large as they
-    // are: qb of 16 bits would be off by 1.7 roundings, not 1.4).  There a pass before forms it from P and yb v^T; kb gets it so in
-    // any case.
-    const bool exact = keys.count <= kFewTiles;
+    // are: qb of 16-bit types would be off by 1.7 of the plain form's error, not 1.4).  There a pass before forms it from P and yb v^T;
+    // kb gets it so in any case.
+    const bool exact = sizeof(T) == 2 && keys.count <= kFewTiles;
     float sum = 0.f;
     for (int pass = exact ? 0 : 1; pass < 2; ++pass) {
         if (keys.count > 0) {

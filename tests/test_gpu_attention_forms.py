@@ -68,6 +68,12 @@ JOINED = {
     "short ones": ([(300, 300), (1, 200), (700, 700)], 6, 2, 80, None, 0),
     "with sinks": ([(900, 900), (40, 50)], 4, 2, 128, 300, 7),
     "many sinks": ([(1200, 1200)], 2, 1, 24, 64, 64),
+    # many rows past the window that see the sinks: in blocks of their own
+    "far rows": ([(1500, 1500)], 4, 1, 64, 100, 4),
+    "far rows of several": ([(2000, 2100), (700, 700), (1, 5), (0, 9)], 4, 2, 128, 64, 9),
+    "far rows, sinks past 32": ([(1300, 1300)], 2, 2, 40, 30, 40),
+    "far rows of one among short ones": ([(5, 5)] * 40 + [(1100, 1100)], 8, 1, 80, 20, 3),
+    "few far rows of one among short ones": ([(5, 5)] * 40 + [(700, 700)], 8, 1, 80, 20, 3),
 }
 
 
