@@ -428,11 +428,11 @@ int32_t stade_hip_attention(int64_t tx, void* y, int64_t ldy, float* lse, const 
     Att p{y, ldy, lse, q, ldq, k, ldk, v, ldv, seqs, (int)i_d, (int)i_k, fabsf(factor(s)), s < 0.0};
     p.seqs.flag = error_flag(call.ws);
     p.slots = slots;
-    // Blocks for two rounds of two a CU, eight tiles of keys each (a tile takes a microsecond, the second launch with what it reads some
-    // ten; fp32: two tiles, which take twelve each), and no more than 32 (which the second launch reads one after the other).  A sequence is taken to be up to twice as long as the
-    // mean.  One token of 8192 keys, 8 key heads: 135 us alone, 22 by 16 blocks; of 65536: 1167 and 75 by 32; 4 chunks of 512 behind
-    // 8192, 4 key heads: 319 and 229 by three; 2 prompts of 300, 2 key heads: 17, and 25 by two; in
-    // fp32 3 of 500, 2 key heads, a window of 300: 82 and 43 + 11 by three.
+    // Blocks for two rounds of two a CU, eight tiles of keys each (a tile takes a microsecond, the second launch with what it reads
+    // some ten; fp32: two tiles, which take twelve each), and no more than 32 (which the second launch reads one after the other).
+    // A sequence is taken to be up to twice as long as the mean.  One token of 8192 keys, 8 key heads: 135 us alone, 22 by 16
+    // blocks; of 65536: 1167 and 75 by 32; 4 chunks of 512 behind 8192, 4 key heads: 319 and 229 by three; 2 prompts of 300, 2 key
+    // heads: 17, and 25 by two; in fp32 3 of 500, 2 key heads, a window of 300: 82 and 43 + 11 by three.
     // (Two slots more than sequences, for columns of none, usually are empty.)
     const int64_t full = std::max<int64_t>(1, (p.slots - 2) * i_k);
     const int64_t longest = std::min({i_tk, 2 * i_tk / std::max<int64_t>(i_n, 1) + 1, (int64_t)seqs.window + kMostSinks + kWideRows});

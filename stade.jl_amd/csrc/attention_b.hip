@@ -758,9 +758,9 @@ int32_t stade_hip_attention_b(int64_t tx, const void* yb, int64_t ldyb, const vo
     const int64_t sink_bytes = (int64_t)std::max<int64_t>(sinks, 1) * 2 * i_d * 4;
     // (what any call of up to kFarBlocks pairs takes is taken by each, so that every smaller one is captured after an eager one)
     const size_t fars = std::max((size_t)kFarBlocks * kMostSinks * 2 * kMostHead * 4, far ? (size_t)(pairs * sink_bytes) : 0);
-    // Tiles of keys that fill no whole round of the CUs go over as many blocks as make two rounds (a block has a CU to
-    // itself), or as have six tiles of rows each (fp32, whose products take eight times as long: four of half the size.  3 sequences of
-    // 500, 2 key heads: 111 us by three blocks a tile, 50 by ten).
+    // Tiles of keys that fill no whole round of the CUs go over as many blocks as make two rounds (a block has a CU to itself), or
+    // as have six tiles of rows each (fp32, whose products take eight times as long: four of half the size.  3 sequences of 500, 2
+    // key heads: 111 us by three blocks a tile, 50 by ten).
     const int64_t cus = cu_count();
     p.whole = units / cus * cus;
     const int64_t rest = units - p.whole, longest = std::min<int64_t>(i_t, (int64_t)seqs.window + kKeys) * seqs.group;
