@@ -349,9 +349,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void wide_kernel(Att p
     }
     if (odd) {
         exact_rows<T>(p, q, kvh, r0 + 32 * wave, 0, q.nk, [&](const Row& x, float m, float sum, Two o) INLINE {
-            const float inv = 1.f / sum;
+            const float inv = sum != 0.f ? 1.f / sum : 0.f;     // (rows that see nothing; a NaN stays one)
             store_two((T*)p.y + x.t * p.ldy + (int64_t)x.head * p.d, o.a * inv, o.b * inv, p.d, false);
-            if (p.lse && lane == 0) p.lse[x.t * (p.heads * s.group) + x.head] = m + logf(sum);
+            if (p.lse && lane == 0) p.lse[x.t * (p.heads * s.group) + x.head] = sum != 0.f ? m + logf(sum) : -INFINITY;
         });
         return;
     }
