@@ -275,6 +275,7 @@ __global__ __launch_bounds__(NT) void join_back_kernel(Moves m) {
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
                 dot[k] = wave_sum(dot[k]);
+                if (row[k] < 0) dot[k] = 0.f;     // (also where `a` is not finite)
                 float* pb = m.pb + t * m.k + k0 + k;
                 if (lane == 0 && k0 + k < m.k) *pb = ADD ? *pb + dot[k] : dot[k];
             }
