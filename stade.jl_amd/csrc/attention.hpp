@@ -459,7 +459,7 @@ inline int32_t check_attention(const char* fn, int64_t tx, double s, int64_t i_d
     // (rows of a sequence are counted in 32 bits)
     const int64_t group = i_k ? i_q / i_k : 0;
     if (int32_t rc = check_extent(fn, "i_t * i_q / i_k", i_t * group, kMostRows)) return rc;
-    if (!(s - s == 0.0)) return bad(fn, "s is not finite");
+    if (!(fabsf((float)s) < INFINITY)) return bad(fn, "s is not finite in Float32");
     if (!qstart || !kstart) return bad(fn, "null pointer");
     const int most = 1 << 30;
     seqs = Seqs{qstart, kstart, (int)i_n, i_t, i_tk, (int)group, window < 0 || window > most ? most : (int)window, (int)sinks, nullptr};

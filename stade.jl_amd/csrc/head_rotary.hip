@@ -344,8 +344,9 @@ int32_t check(const char* fn, int64_t tx, int64_t tg, const void* gq, const void
     if (int32_t rc = check_extent(fn, "i_t", i_t, kMostRows)) return rc;
     if (i_r % 2) return bad(fn, "i_r is odd");
     if (!norm && (gq || gk)) return bad(fn, "weights without the norm");
-    if (norm && !(eps >= 0.0)) return bad(fn, "eps is negative or NaN");
-    if (!(fabs(s) < INFINITY)) return bad(fn, "s is not finite");
+    // (both are taken in Float32)
+    if (norm && !(eps >= 0.0 && (float)eps < INFINITY)) return bad(fn, "eps is negative or not finite in Float32");
+    if (!(fabsf((float)s) < INFINITY)) return bad(fn, "s is not finite in Float32");
     return 0;
 }
 
