@@ -6,8 +6,8 @@
 //   gb (+)= sum over tokens and heads of hb xh,   xb (+)= rs (a - xh mean(a xh)).
 // rs is formed again from x, which the adjoint reads anyway: nothing is kept between the sweeps.
 //
-// Angles are formed in fp64 as turns, pos * (freq / 2 pi), and only the fraction of a turn goes on to fp32 (an fp32
-// angle of position 10^5 is off by 10^-2).  A block forms its tokens' cosines and sines once, in LDS, for all
+// Angles are formed in fp64 as turns, pos * (freq / 2 pi), and only the fraction of a turn goes on to fp32, in two parts (an
+// fp32 angle of position 10^5 is off by 10^-2).  A block forms its tokens' cosines and sines once, in LDS, for all
 // heads.  Sums are fp32.
 //
 // Bound by HBM.  A group of lanes takes a head of a token: a lane has two vectors of it that belong together (the
@@ -110,10 +110,12 @@ __device__ __forceinline__ void fill_table(const Rot& p, int64_t first, int toke
         float2 cs = {0.f, 0.f};
         if (j < p.r / 2) {
             const double turns = (double)p.pos[first + k] * (p.freq[j] * 0.15915494309189533577);   // 1 / 2 pi
-            const float f = (float)(2.0 * (turns - rint(turns)));
+            const double whole = 2.0 * (turns - rint(turns));
+            // (what its rounding leaves out, to the first order: a sine near half a turn is as small as that)
+            const float f = (float)whole, rest = 3.14159265358979f * (float)(whole - (double)f);
             float sn, c;
             sincospif(f, &sn, &c);
-            cs = {c * p.s, sn * p.s};
+            cs = {fmaf(-rest, sn, c) * p.s, fmaf(rest, c, sn) * p.s};
         }
         table[i] = cs;
     }
