@@ -2,7 +2,8 @@
 //   y = sum over the seen keys of softmax(s q . k) v,   lse = log sum exp(s q . k)
 // One pass over the keys with the running maximum m and sum l of a row's exponentials: a tile of keys whose scores go
 // up to m' > m scales what was summed before by exp(m - m').  (The sums are scaled only where some row's maximum grows by
-// more than 8 in the exponent of 2; until then exponentials are up to 2^8, which every type holds.)
+// more than 8 in the exponent of 2; until then exponentials are up to 2^8, which every type holds.  f16 has few exponents below 1, and
+// many small weights may make up a row: its exponentials and their sum are 2^7 times as large, so that 2^-31 of a row's largest counts.)
 //
 // Scores are formed as K Q^T, keys along the registers: a lane has one query and half of a tile's keys, so
 // maxima and sums are lane by lane and one exchange of the half waves.  Exponentials are rounded to the
@@ -42,6 +43,8 @@ struct Att {
 };
 
 constexpr float kGrow = 8.f;     // of the maximum, in the exponent of 2, before sums are scaled
+// what is added to the exponents (of 2): the largest exponential, 2^(kGrow + kLift), is below f16's 65504
+template <class T> constexpr float kLift = std::is_same<T, f16>::value ? 7.f : 0.f;
 
 // a lane's query
 struct Row {
@@ -142,7 +145,7 @@ struct Sums {
 
     // the scores' weights, and the values by them
     __device__ __forceinline__ void add(Scores& s, const char* vt, float c) {
-        const float base = m == -INFINITY ? 0.f : -m * c;
+        const float base = (m == -INFINITY ? 0.f : -m * c) + kLift<T>;
         float sum = 0.f;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -182,7 +185,7 @@ __device__ __forceinline__ void store_rows(const Att& p, const floatx16 (&o)[DT]
             const int col = 32 * i + 8 * g + 4 * h;
             store4(y + col, o[i][4 * g] * inv, o[i][4 * g + 1] * inv, o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv, p.d - col);
         }
-    if (p.lse && h == 0) p.lse[w.t * (p.heads * p.seqs.group) + w.head] = l > 0.f ? m * p.s + kLn2 * __builtin_amdgcn_logf(l) : -INFINITY;
+    if (p.lse && h == 0) p.lse[w.t * (p.heads * p.seqs.group) + w.head] = l > 0.f ? m * p.s + kLn2 * (__builtin_amdgcn_logf(l) - kLift<T>) : -INFINITY;
 }
 
 // One row after the other, from the keys of [from, to) that it sees: done(row, m, l, its two values of the sum).
@@ -342,7 +345,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void wide_kernel(Att p
                 store4(part + col, sums.o[i][4 * g], sums.o[i][4 * g + 1], sums.o[i][4 * g + 2], sums.o[i][4 * g + 3], p.d - col);
             }
         if (h == 0) {
-            part[p.d] = sums.m == -INFINITY ? sums.m : sums.m * p.s;
+            part[p.d] = sums.m == -INFINITY ? sums.m : sums.m * p.s - kLn2 * kLift<T>;
             part[p.d + 1] = l;
         }
         return;
