@@ -11,8 +11,8 @@
 // Sinks are seen by every later row: rows past the window of the first tile of keys go over blocks of their own, which leave
 // partial sums that the tile's block adds.
 // 4 sequences of 2048, 16 heads of 128 and 4 of keys, a window of 1024, 4 sinks, bf16: rows 121 us, keys 194, sinks 31, joins 9: some 590
-// TFLOP/s of the products formed for what is seen.
-// Sums are fp32; P and S are rounded to the type as factors of products (to nearest), as the values they meet are.
+// TFLOP/s of the products formed for what is seen.  f16 pays for the powers of two (below) with some 11 us of the rows, 4 of the keys.
+// Sums are fp32; P and S are rounded to the type as factors of products (to nearest), as the values they meet are; in f16 times powers of two.
 #include "attention.hpp"
 
 #include <algorithm>
@@ -47,10 +47,42 @@ struct Back {
     int64_t whole;         // tiles of keys that a block has alone; the others go over `splits` blocks each
     int splits;
     float* part;           // those blocks' sums
+    float* most;           // f16: the largest S of each 32 rows
 };
 
 constexpr int kRows = 128, kKeys = 128;
 constexpr int kFewTiles = 4;      // of keys, where delta is formed from the weights
+
+// ------------------------------------------------------------------------------------------
+// factors in f16
+// ------------------------------------------------------------------------------------------
+// f16 holds 2^-24 to 65504.  P is 1 / keys and S = P (yb v^T - delta) a shadow's size of that, or far above 65504: rounded as they are, they
+// vanish or overflow where the results, sums of thousands of them, do not.  So for kb and vb P stands for P 2^14 and S for that by
+// 2^k, k from the largest S of the block's rows, which rows_kernel leaves; and for qb both stand for 2^k of them, k of each row by itself:
+// its largest S so far is below 2^15, and sums are scaled where a larger one comes, as the forward sweep's are.  What is
+// 2^-36 of the largest and more counts.  P's powers come into its exponent for nothing.
+template <class T> constexpr bool kNarrow = std::is_same<T, f16>::value;
+template <class T> constexpr int kWeightLift = kNarrow<T> ? 14 : 0;
+constexpr int kMostLift = 60;     // of a row whose S are all below 2^-45 so far (yb v^T is below 2^39)
+__device__ __forceinline__ float power(int k) { return __builtin_amdgcn_ldexpf(1.f, k); }
+
+// where the largest S of the 32 rows from r on of a key head is (sequence i): as many places as rows_kernel's waves have
+__device__ __forceinline__ int64_t most_at(const Seqs& s, int i, int r, int heads, int kvh) {
+    return ((first_slot(s.qstart, s.t, s.group, kRows, i + 1) + r / kRows) * heads + kvh) * (kRows / 32) + r % kRows / 32;
+}
+// k for the rows [r, end): their S are below 2^14 (and yb v^T - delta, rounded another way here, may be larger where it is next
+// to 0), times 2^kWeightLift as P has it
+template <class T>
+__device__ __forceinline__ int lift_of(const float* most, const Seqs& s, int i, int r, int end, int heads, int kvh) {
+    float top = 0.f;
+    for (int w = r / 32 + (int)(threadIdx.x & 63); 32 * w < end; w += 64) {
+        const float v = most[most_at(s, i, 32 * w, heads, kvh)];
+        if (v < INFINITY) top = fmaxf(top, v);     // (what is not finite makes sums that are formed again)
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    return uniform(min(14 - __builtin_amdgcn_frexp_expf(top) - kWeightLift<T>, kMostLift));
+}
 
 // ------------------------------------------------------------------------------------------
 // qb, and delta
@@ -98,7 +130,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void rows_kernel(Back 
     const KeyTiles<BN> keys(range);
     const T* k = (const T*)p.k + q.k0 * p.ldk + (int64_t)kvh * p.d;
     const T* v = (const T*)p.v + q.k0 * p.ldv + (int64_t)kvh * p.d;
-    const float c = p.factor * kLog2e, base = -lse * kLog2e;
+    int lift = kNarrow<T> ? kMostLift : 0;
+    const float c = p.factor * kLog2e;
+    float base = -lse * kLog2e + (float)lift;
     floatx16 acc[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i)
@@ -158,6 +192,25 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void rows_kernel(Back 
                         x[e] *= g[e] - delta;
                     }
                     if (pass) {
+                        if constexpr (kNarrow<T>) {
+                            float top = 0.f;
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(x[e]));    // (NaN and Inf make sums that are formed again)
+                            top = fmaxf(top, other_half(top));
+                            if (__any(top > 0x1p15f)) {
+                                const int less = top > 0x1p15f ? max(__builtin_amdgcn_frexp_expf(top) - 14, 0) : 0;   // (to 2^13 .. 2^14)
+                                const float f = power(-less);
+                                lift -= less;
+                                base -= (float)less;
+                                sum *= f;
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) x[e] *= f;
+#pragma unroll
+                                for (int m = 0; m < DT; ++m)
+#pragma unroll
+                                    for (int e = 0; e < 16; ++e) acc[m][e] *= f;
+                            }
+                        }
 #pragma unroll
                         for (int u = 0; u < kParts<T>; ++u) {
                             const v4u part = part_of<T>(x, u);
@@ -176,10 +229,23 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void rows_kernel(Back 
         }
         if (!pass) {
             delta = sum + other_half(sum);
+            if constexpr (kNarrow<T>) delta *= power(-lift);
             sum = 0.f;
         }
     }
     sum += other_half(sum);
+    float most = 0.f;
+    if constexpr (kNarrow<T>) {
+        sum *= power(-lift);
+        const float moved = fabsf(sum - delta);      // (keys_kernel has the sum)
+        most = (lift < kMostLift ? power(15 - lift) : 0.f) + (moved < INFINITY ? moved : 0.f);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+    }
+    auto leave_most = [&]() INLINE {
+        if constexpr (kNarrow<T>)
+            if (working && q.real && lane == 0) p.most[most_at(s, j - 1, r0 + 32 * wave, p.heads, kvh)] = most;
+    };
     if (here && h == 0) p.delta[t * (p.heads * s.group) + head] = sum;
     // (what is not finite: products with what is not seen among it.  Of what is seen, it reaches the other keys by y alone.)
     if (any_not_finite<DT>(acc) || __any(here && sum * 0.f != 0.f)) {
@@ -203,6 +269,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void rows_kernel(Back 
                         } else {
                             a = fmaf(w * (gv - di), kn.a, a);
                             b = fmaf(w * (gv - di), kn.b, b);
+                            if (kNarrow<T> && fabsf(w * (gv - di)) < INFINITY) most = fmaxf(most, fabsf(w * (gv - di)));
                         }
                     }
                 }
@@ -211,16 +278,22 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void rows_kernel(Back 
             if (!p.qb) continue;
             store_two((T*)p.qb + ti * p.ldqb + ci, a * p.s, b * p.s, p.d, p.add);
         }
+        leave_most();
         return;
     }
+    leave_most();
     if (!here || !p.qb) return;
     T* out = (T*)p.qb + t * p.ldqb + col;
+    const float by = power(-lift);     // (of f16: what the factors were multiplied by)
 #pragma unroll
     for (int m = 0; m < DT; ++m)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int at = 32 * m + 8 * g + 4 * h;
-            store4(out + at, acc[m][4 * g] * p.s, acc[m][4 * g + 1] * p.s, acc[m][4 * g + 2] * p.s, acc[m][4 * g + 3] * p.s, p.d - at, p.add);
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (kNarrow<T> ? acc[m][4 * g + e] * by : acc[m][4 * g + e]) * p.s;
+            store4(out + at, v[0], v[1], v[2], v[3], p.d - at, p.add);
         }
 }
 
@@ -317,15 +390,17 @@ __device__ __forceinline__ KeyTile key_tile(const Seqs& s, int j, int64_t tile) 
 __device__ __forceinline__ int part_rows(int rows, int parts, int BM) { return (rows / parts / BM + 1) * BM; }
 
 // A split block's sums, and a far block's: (kb, vb) of its keys, d values each, one key after the other
-template <int DT>
-__device__ __forceinline__ void store_part(float* out, int d, const floatx16 (&a)[DT]) {
+template <bool SCALED, int DT>
+__device__ __forceinline__ void store_part(float* out, int d, const floatx16 (&a)[DT], float by) {
     const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
     for (int m = 0; m < DT; ++m)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int at = 32 * m + 8 * g + 4 * h;
-            const float v[4] = {a[m][4 * g], a[m][4 * g + 1], a[m][4 * g + 2], a[m][4 * g + 3]};
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = SCALED ? a[m][4 * g + e] * by : a[m][4 * g + e];
             store_row(out + at, v, d - at);
         }
 }
@@ -389,6 +464,8 @@ __global__ __launch_bounds__((64 * kGroups<T, FAR> * kRowWaves<T, FAR>), (sizeof
 #pragma unroll
         for (int e = 0; e < 16; ++e) ka[i][e] = va[i][e] = 0.f;
     const float c = p.factor * kLog2e;
+    const int lift = kNarrow<T> && q.real ? lift_of<T>(p.most, s, j - 1, r_first, r_end, p.heads, kvh) : 0;
+    const float lift_by = power(lift);
     const int heads = p.heads * s.group, tiles = r_end > r_first ? (r_end - r_first + BM - 1) / BM : 0;
     // (the query and the head in its group of a tile's first row: of the one at work and of the one on its way)
     int now_j = uniform(r_first / s.group), now_h = uniform(r_first - now_j * s.group), next_j = now_j, next_h = now_h;
@@ -429,7 +506,9 @@ __global__ __launch_bounds__((64 * kGroups<T, FAR> * kRowWaves<T, FAR>), (sizeof
     auto keep = [&](int i, char* at) INLINE {
         sq.store(at);
         so.store(at + TILE);
-        if (threadIdx.x < 2 * BM) reinterpret_cast<float*>(st + (i & 1) * STATS)[threadIdx.x] = threadIdx.x < BM ? stat * (FROM_LSE ? per_s : -kLog2e) : -stat;
+        if (threadIdx.x < 2 * BM)
+            reinterpret_cast<float*>(st + (i & 1) * STATS)[threadIdx.x] =
+                threadIdx.x < BM ? (stat - kLn2 * kWeightLift<T>) * (FROM_LSE ? per_s : -kLog2e) : -stat;
         if constexpr (DIRECT) wait_loads<0>();
     };
     if (tiles > 0) {
@@ -532,7 +611,7 @@ __global__ __launch_bounds__((64 * kGroups<T, FAR> * kRowWaves<T, FAR>), (sizeof
                     if constexpr (PH < RB) {
                         static_for<(F + 1) * 16 / PER - FROM>([&](auto k) INLINE {
                             constexpr int E = FROM + decltype(k)::value;
-                            x[PH][E] *= g[PH][E];
+                            x[PH][E] *= kNarrow<T> ? g[PH][E] * lift_by : g[PH][E];
                         });
                         if constexpr (F == PER - 1) {
 #pragma unroll
@@ -572,8 +651,8 @@ __global__ __launch_bounds__((64 * kGroups<T, FAR> * kRowWaves<T, FAR>), (sizeof
                     const int from = (32 * m + 8 * (e >> 2) + 4 * h + (e & 3)) & 63;
                     const float x = __shfl(m < 2 ? a.a : a.b, from, 64), y = __shfl(m < 2 ? b.a : b.b, from, 64);
                     if ((lane & 31) == n) {
-                        ka[m][e] = x;
-                        va[m][e] = y;
+                        ka[m][e] = kNarrow<T> ? x * power(lift + kWeightLift<T>) : x;
+                        va[m][e] = kNarrow<T> ? y * power(kWeightLift<T>) : y;
                     }
                 }
         }
@@ -604,19 +683,21 @@ __global__ __launch_bounds__((64 * kGroups<T, FAR> * kRowWaves<T, FAR>), (sizeof
         if (first_row != 0) return;
     }
     if (!here) return;
+    // (of f16: what the factors were multiplied by)
+    float ka_by = kNarrow<T> ? power(-lift - kWeightLift<T>) : 1.f, va_by = kNarrow<T> ? power(-kWeightLift<T>) : 1.f;
     // partial sums of the sinks: (sequence, head), part, sink, kb and vb, the head's values
     const int64_t far_at = ((int64_t)(j - 1) * p.heads + kvh) * p.far_parts * s.sinks * 2 * p.d, far_next = (int64_t)s.sinks * 2 * p.d;
     if constexpr (FAR) {
         if (key >= s.sinks) return;
         float* out = p.far + far_at + tile * far_next + (int64_t)key * 2 * p.d;
-        store_part<DT>(out, p.d, ka);
-        store_part<DT>(out + p.d, p.d, va);
+        store_part<kNarrow<T>>(out, p.d, ka, ka_by);
+        store_part<kNarrow<T>>(out + p.d, p.d, va, va_by);
         return;
     }
     if (split >= 0) {
         float* out = p.part + ((int64_t)(blockIdx.x - p.whole) * kKeys + key - key0) * 2 * p.d;
-        store_part<DT>(out, p.d, ka);
-        store_part<DT>(out + p.d, p.d, va);
+        store_part<kNarrow<T>>(out, p.d, ka, ka_by);
+        store_part<kNarrow<T>>(out + p.d, p.d, va, va_by);
         return;
     }
     if (p.far && q.real && key0 == 0 && key < s.sinks && kt.far_rows > 0) {
@@ -631,10 +712,11 @@ __global__ __launch_bounds__((64 * kGroups<T, FAR> * kRowWaves<T, FAR>), (sizeof
                 load_row(b, in + p.d + at, p.d - at);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    ka[m][4 * g + e] += a[e];
-                    va[m][4 * g + e] += b[e];
+                    ka[m][4 * g + e] = kNarrow<T> ? fmaf(ka[m][4 * g + e], ka_by, a[e]) : ka[m][4 * g + e] + a[e];
+                    va[m][4 * g + e] = kNarrow<T> ? fmaf(va[m][4 * g + e], va_by, b[e]) : va[m][4 * g + e] + b[e];
                 }
             }
+        ka_by = va_by = 1.f;
     }
     T* kb = p.kb ? (T*)p.kb + kcol * p.ldkb + hcol : nullptr;
     T* vb = p.vb ? (T*)p.vb + kcol * p.ldvb + hcol : nullptr;
@@ -643,8 +725,15 @@ __global__ __launch_bounds__((64 * kGroups<T, FAR> * kRowWaves<T, FAR>), (sizeof
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int at = 32 * m + 8 * g + 4 * h;
-            if (kb) store4(kb + at, ka[m][4 * g] * p.s, ka[m][4 * g + 1] * p.s, ka[m][4 * g + 2] * p.s, ka[m][4 * g + 3] * p.s, p.d - at, p.add);
-            if (vb) store4(vb + at, va[m][4 * g], va[m][4 * g + 1], va[m][4 * g + 2], va[m][4 * g + 3], p.d - at, p.add);
+            const floatx16 &x = ka[m], &y = va[m];
+            const int i = 4 * g;
+            if constexpr (kNarrow<T>) {
+                if (kb) store4(kb + at, x[i] * ka_by * p.s, x[i + 1] * ka_by * p.s, x[i + 2] * ka_by * p.s, x[i + 3] * ka_by * p.s, p.d - at, p.add);
+                if (vb) store4(vb + at, y[i] * va_by, y[i + 1] * va_by, y[i + 2] * va_by, y[i + 3] * va_by, p.d - at, p.add);
+            } else {
+                if (kb) store4(kb + at, x[i] * p.s, x[i + 1] * p.s, x[i + 2] * p.s, x[i + 3] * p.s, p.d - at, p.add);
+                if (vb) store4(vb + at, y[i], y[i + 1], y[i + 2], y[i + 3], p.d - at, p.add);
+            }
         }
 }
 
@@ -767,14 +856,18 @@ int32_t stade_hip_attention_b(int64_t tx, const void* yb, int64_t ldyb, const vo
     p.splits = rest ? (int)std::min<int64_t>(2 * cus / rest, std::max<int64_t>(1, longest / (tx == STADE_HIP_F32 ? 4 * 32 : 6 * 64))) : 1;
     if (p.splits <= 1) p.whole = units;
     const size_t parts = (size_t)(2 * cus) * kKeys * 2 * kMostHead * 4;
-    char* work = (char*)scratch(deltas + fars + parts);
+    const size_t mosts = ((size_t)row_slots * i_k * (kRows / 32) * 4 + 256) / 256 * 256;
+    char* work = (char*)scratch(deltas + mosts + fars + parts);
     if (!work) return scratch_error();
     p.delta = (float*)work;
+    work += deltas;
+    p.most = (float*)work;
+    work += mosts;
     if (far) {
-        p.far = (float*)(work + deltas);
+        p.far = (float*)work;
         p.far_parts = (int)std::max<int64_t>(1, kFarBlocks / std::max<int64_t>(pairs, 1));
     }
-    p.part = (float*)(work + deltas + fars);
+    p.part = (float*)(work + fars);
     return with_type(tx, [&](auto t) -> int32_t {
         return with_width(i_d, [&](auto dt) -> int32_t {
             using T = decltype(t);
