@@ -306,8 +306,13 @@ int32_t stade_hip_head_rotary_b(int64_t tx, int64_t tg, const void* yb, int64_t 
  * p sees the keys i <= p with p - i < window (window < 0: all) or i < sinks.  y = sum of softmax(s q . k) v over what it
  * sees; lse (i_q, i_t) Float32, if not null: the logarithm of the sum of exp(s q . k), which the adjoint takes.  A query that sees nothing,
  * and a column of no sequence, gets zeros and -Inf.  A product with keys that are not seen is never formed into the result,
- * whatever they hold.  Offsets that decrease or lie outside the columns raise the device error flag.  i_d <= 128, sinks <= 64,
- * i_t * i_q / i_k <= 2^30, and of tiles of 128 rows or keys, a few for each sequence, times i_k at most 2^23. */
+ * whatever they hold; rows (of the adjoint: keys) whose sums are not finite, and up to 31 beside them, are formed one by one, which is slow.
+ * Offsets that decrease or lie outside the columns raise the device error flag (of calls with queries).  i_d <= 128, sinks <= 64,
+ * i_t * i_q / i_k <= 2^30, and of tiles of 128 rows or keys, a few for each sequence, times i_k at most 2^23; s is finite in Float32.
+ * Scores, sums and lse are Float32.  The weights are factors of the values, and (in the adjoint) their shadows of keys and queries: in
+ * BF16 and F16 they are rounded to the type for that, before the sum.  The results' errors then are some 1.4 times those of one rounding
+ * of the exact result (Float32 has no such rounding).  In F16 weights of 2^-31 of a row's largest and more count, in the adjoint of
+ * 2^-39, and their shadows of 2^-36 of the largest of a query's row (for qb) or of the rows that a tile of 128 keys goes with (for kb). */
 int32_t stade_hip_attention(int64_t tx, void* y, int64_t ldy, float* lse, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
                             int64_t ldv, const int64_t* qstart, const int64_t* kstart, double s, int64_t i_d, int64_t i_q, int64_t i_k,
                             int64_t i_t, int64_t i_tk, int64_t i_n, int64_t window, int64_t sinks, hipStream_t stream);

@@ -433,7 +433,8 @@ int32_t stade_hip_attention(int64_t tx, void* y, int64_t ldy, float* lse, const 
     p.slots = slots;
     // Blocks for two rounds of two a CU, eight tiles of keys each (a tile takes a microsecond, the second launch with what it reads
     // some ten; fp32: two tiles, which take twelve each), and no more than 32 (which the second launch reads one after the other).
-    // A sequence is taken to be up to twice as long as the mean.  One token of 8192 keys, 8 key heads: 135 us alone, 22 by 16
+    // A sequence is taken to be up to twice as long as the mean (one of 131072 keys among 63 of 1000, a token each, is not split: 2360 us,
+    // where it alone takes 130 and they 45).  One token of 8192 keys, 8 key heads: 135 us alone, 22 by 16
     // blocks; of 65536: 1167 and 75 by 32; 4 chunks of 512 behind 8192, 4 key heads: 319 and 229 by three; 2 prompts of 300, 2 key
     // heads: 17, and 25 by two; in fp32 3 of 500, 2 key heads, a window of 300: 82 and 43 + 11 by three.
     // (Two slots more than sequences, for columns of none, usually are empty.)

@@ -1,15 +1,16 @@
 // The adjoint of attention.  With P = exp(s q . k - lse) over the seen keys, the rows as in the forward sweep (query after query
 // with the heads of a group side by side), and delta = yb . y for each row:
 //   vb (+)= P^T yb,   S = P (yb v^T - delta),   qb (+)= s S k,   kb (+)= s S^T q
-// P is formed again from lse; nothing of the size of the scores is kept.  Two launches (three with sinks):
+// P is formed again from lse; nothing of the size of the scores is kept.  Two launches, and up to three more (below):
 //   rows_kernel   a block has 128 rows and goes over their keys: qb, and delta as the sum of P (yb v^T).  Scores as keys x rows, so that
 //                 lse and delta are one value a lane, and S, rounded, is the operand of K^T S as it lies.
 //   keys_kernel   a block has 128 keys and goes over the rows that see them, all heads of the group: kb and vb.  Scores as
 //                 rows x keys; P and S are the operands of yb^T P and q^T S as they lie.
 // That forms the scores and yb v^T twice, 7 products for 5, and needs no atomics: each result has one writer, its
 // sums go in a fixed order, and the same call gives the same bits.
-// Sinks are seen by every later row: rows past the window of the first tile of keys go over blocks of their own, which leave
-// partial sums that the tile's block adds.
+// Sinks are seen by every later row: rows past the window of the first tile of keys go over blocks of their own (a launch), which leave
+// partial sums; far_kernel joins them, and the tile's block adds them.  Tiles of keys that fill no round of the CUs go over several
+// blocks, which join_kernel joins.
 // 4 sequences of 2048, 16 heads of 128 and 4 of keys, a window of 1024, 4 sinks, bf16: rows 121 us, keys 194, sinks 31, joins 9: some 590
 // TFLOP/s of the products formed for what is seen.  f16 pays for the powers of two (below) with some 11 us of the rows, 4 of the keys.
 // Sums are fp32; P and S are rounded to the type as factors of products (to nearest), as the values they meet are; in f16 times powers of two.

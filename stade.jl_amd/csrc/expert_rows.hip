@@ -10,8 +10,8 @@
 // All go by `place`, token by token: x and yb are read once for all of a token's slots (by the order of the
 // experts they would be read i_k times), and sums over slots go in the order of k, with no atomics.
 // Bound by HBM: a wave takes 512 columns of one token (the adjoint of the join: a token's whole rows, for the
-// dot products), four slots in flight.  Sums are fp32.  8192 tokens of 2048 values, two slots each, bf16: take 20 us (5.0 TB/s), join
-// 24 to 29, its adjoint 35 (4.8 TB/s), the order of 64 experts 11 in two launches.
+// dot products), four slots in flight.  Sums are fp32.  8192 tokens of 2048 values, two slots each, bf16: take 20 us (5.0 TB/s), its
+// adjoint 30, join 25, its adjoint 35 (4.8 TB/s), the order of 64 experts 11 in two launches.
 #include "rows.hpp"
 
 #include <algorithm>

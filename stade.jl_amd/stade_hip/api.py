@@ -849,7 +849,8 @@ def attention(y, lse, q, k, v, qstart, kstart, s, i_d, i_q, i_k, i_t, i_tk, i_n,
     kstart[n] <= t < kstart[n + 1] of k, v (i_d * i_k, i_tk) (Int64[i_n + 1], increasing).  Query head h goes with key head h // (i_q / i_k).  A
     sequence's last query stands at its last key; a query at key p sees the keys i <= p with p - i < window (None: all) or
     i < sinks.  lse (i_q, i_t) Float32: the logarithms of the sums, for the adjoint (None: not kept).  A query that sees nothing
-    and a column of no sequence get 0 and -Inf.  check=True raises StadeHipBoundsError for offsets that decrease or lie outside
+    and a column of no sequence get 0 and -Inf.  Scores and sums are Float32; bfloat16 and float16 round the weights, factors of the values, to
+    the type (some 1.4 times the error of one rounding).  check=True raises StadeHipBoundsError for offsets that decrease or lie outside
     the columns (one synchronisation)."""
     import torch
     d, hq, hk, t, tk, n, w, sk = sizes = _attention_sizes(i_d, i_q, i_k, i_t, i_tk, i_n, window, sinks)
