@@ -312,7 +312,7 @@ int32_t stade_hip_head_rotary_b(int64_t tx, int64_t tg, const void* yb, int64_t 
  * Scores, sums and lse are Float32.  The weights are factors of the values, and (in the adjoint) their shadows of keys and queries: in
  * BF16 and F16 they are rounded to the type for that, before the sum.  The results' errors then are some 1.4 times those of one rounding
  * of the exact result (Float32 has no such rounding).  In F16 weights of 2^-31 of a row's largest and more count, in the adjoint of
- * 2^-39, and their shadows of 2^-36 of the largest of a query's row (for qb) or of the rows that a tile of 128 keys goes with (for kb). */
+ * 2^-39, and their shadows of 2^-36 of the largest of a query's row (for qb) or of the rows that a tile of 128 keys goes with (for kb), or 2^-55. */
 int32_t stade_hip_attention(int64_t tx, void* y, int64_t ldy, float* lse, const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v,
                             int64_t ldv, const int64_t* qstart, const int64_t* kstart, double s, int64_t i_d, int64_t i_q, int64_t i_k,
                             int64_t i_t, int64_t i_tk, int64_t i_n, int64_t window, int64_t sinks, hipStream_t stream);

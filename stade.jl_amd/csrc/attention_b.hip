@@ -12,7 +12,8 @@
 // partial sums; far_kernel joins them, and the tile's block adds them.  Tiles of keys that fill no round of the CUs go over several
 // blocks, which join_kernel joins.
 // 4 sequences of 2048, 16 heads of 128 and 4 of keys, a window of 1024, 4 sinks, bf16: rows 121 us, keys 194, sinks 31, joins 9: some 590
-// TFLOP/s of the products formed for what is seen.  f16 pays for the powers of two (below) with some 11 us of the rows, 4 of the keys.
+// TFLOP/s of the products formed for what is seen.  f16 pays for the powers of two (below) with some 15 us of the rows', 7 of the
+// keys' and 2 of the sinks'.
 // Sums are fp32; P and S are rounded to the type as factors of products (to nearest), as the values they meet are; in f16 times powers of two.
 #include "attention.hpp"
 
@@ -48,7 +49,7 @@ struct Back {
     int64_t whole;         // tiles of keys that a block has alone; the others go over `splits` blocks each
     int splits;
     float* part;           // those blocks' sums
-    float* most;           // f16: the largest S of each 32 rows
+    float* most;           // f16: what the S of each 32 rows are below
 };
 
 constexpr int kRows = 128, kKeys = 128;
@@ -58,16 +59,16 @@ constexpr int kFewTiles = 4;      // of keys, where delta is formed from the wei
 // factors in f16
 // ------------------------------------------------------------------------------------------
 // f16 holds 2^-24 to 65504.  P is 1 / keys and S = P (yb v^T - delta) a shadow's size of that, or far above 65504: rounded as they are, they
-// vanish or overflow where the results, sums of thousands of them, do not.  So for kb and vb P stands for P 2^14 and S for that by
-// 2^k, k from the largest S of the block's rows, which rows_kernel leaves; and for qb both stand for 2^k of them, k of each row by itself:
-// its largest S so far is below 2^15, and sums are scaled where a larger one comes, as the forward sweep's are.  What is
-// 2^-36 of the largest and more counts.  P's powers come into its exponent for nothing.
+// vanish or overflow where the results, sums of thousands of them, do not.  So for kb and vb P stands for P 2^14, by its exponent, and S
+// for that by 2^k, k from the largest S of the block's rows, which rows_kernel leaves; and for qb S stands for S 2^k, k of each row by
+// itself: its largest S so far is below 2^15, and sums are scaled where a larger one comes, as the forward sweep's are.  S of
+// 2^-36 of the largest and more counts, and any of 2^-55 (which no sum of f16's values makes a value of).
 template <class T> constexpr bool kNarrow = std::is_same<T, f16>::value;
 template <class T> constexpr int kWeightLift = kNarrow<T> ? 14 : 0;
-constexpr int kMostLift = 60;     // of a row whose S are all below 2^-45 so far (yb v^T is below 2^39)
+constexpr int kMostLift = 32;     // of a row whose S are all below 2^-17 so far
 __device__ __forceinline__ float power(int k) { return __builtin_amdgcn_ldexpf(1.f, k); }
 
-// where the largest S of the 32 rows from r on of a key head is (sequence i): as many places as rows_kernel's waves have
+// where what the S of the 32 rows from r on of a key head are below is (sequence i): as many places as rows_kernel's waves have
 __device__ __forceinline__ int64_t most_at(const Seqs& s, int i, int r, int heads, int kvh) {
     return ((first_slot(s.qstart, s.t, s.group, kRows, i + 1) + r / kRows) * heads + kvh) * (kRows / 32) + r % kRows / 32;
 }
@@ -82,7 +83,7 @@ __device__ __forceinline__ int lift_of(const float* most, const Seqs& s, int i, 
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    return uniform(min(14 - __builtin_amdgcn_frexp_expf(top) - kWeightLift<T>, kMostLift));
+    return uniform(14 - __builtin_amdgcn_frexp_expf(top) - kWeightLift<T>);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -131,9 +132,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void rows_kernel(Back 
     const KeyTiles<BN> keys(range);
     const T* k = (const T*)p.k + q.k0 * p.ldk + (int64_t)kvh * p.d;
     const T* v = (const T*)p.v + q.k0 * p.ldv + (int64_t)kvh * p.d;
-    int lift = kNarrow<T> ? kMostLift : 0;
-    const float c = p.factor * kLog2e;
-    float base = -lse * kLog2e + (float)lift;
+    const float c = p.factor * kLog2e, base = -lse * kLog2e;
+    int lift = kMostLift;
     floatx16 acc[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i)
@@ -171,6 +171,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void rows_kernel(Back 
                 const int high = pos - key - 4 * h, low = high - s.window, sink = s.sinks - key - 4 * h;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
+                    const float lift_by = power(lift);
                     floatx16 x, g;
 #pragma unroll
                     for (int e = 0; e < 16; ++e) x[e] = g[e] = 0.f;
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void rows_kernel(Back 
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         sum = fmaf(x[e], g[e], sum);
-                        x[e] *= g[e] - delta;
+                        x[e] *= kNarrow<T> ? fmaf(g[e], lift_by, -delta * lift_by) : g[e] - delta;
                     }
                     if (pass) {
                         if constexpr (kNarrow<T>) {
@@ -202,8 +203,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void rows_kernel(Back 
                                 const int less = top > 0x1p15f ? max(__builtin_amdgcn_frexp_expf(top) - 14, 0) : 0;   // (to 2^13 .. 2^14)
                                 const float f = power(-less);
                                 lift -= less;
-                                base -= (float)less;
-                                sum *= f;
 #pragma unroll
                                 for (int e = 0; e < 16; ++e) x[e] *= f;
 #pragma unroll
@@ -230,16 +229,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void rows_kernel(Back 
         }
         if (!pass) {
             delta = sum + other_half(sum);
-            if constexpr (kNarrow<T>) delta *= power(-lift);
             sum = 0.f;
         }
     }
     sum += other_half(sum);
     float most = 0.f;
     if constexpr (kNarrow<T>) {
-        sum *= power(-lift);
         const float moved = fabsf(sum - delta);      // (keys_kernel has the sum)
-        most = (lift < kMostLift ? power(15 - lift) : 0.f) + (moved < INFINITY ? moved : 0.f);
+        most = power(15 - lift) + (moved < INFINITY ? moved : 0.f);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
     }
